@@ -38,7 +38,7 @@ RB200_API void* rb200_get_stream(void);
 /*
  * Reads (and clears) the device-side status words that bounded waits inside the kernels set
  * when they give up: the one in the library's per-device scratch block, the one in the static
- * array of rb200_gemm_fp16_intx_noalloc and that of rb200_encode_ft.  Synchronises the given stream.  0 = no error recorded,
+ * array of rb200_gemm_fp16_intx_noalloc, that of rb200_encode_ft and that of the 4-bit float entries.  Synchronises the given stream.  0 = no error recorded,
  * 1 = a wait ran out (the kernel skipped its remaining work and left outputs unwritten).
  * Allocates nothing: a status word that no call has created yet reads as 0.  After a non-zero
  * status it synchronises the device and puts the split-k flags, tickets and hand-over words back at rest.
@@ -314,6 +314,75 @@ RB200_API int rb200_interleave_gate_up(const void* src, void* dst, int64_t outer
  */
 RB200_API int rb200_encode_ft(const void* a, void* packed, void* scales, int64_t n, int64_t k, int weight_bits,
                               int64_t group_size, void* stream);
+
+/* ------------------------------------------------------------------ microscaled 4-bit floats */
+
+/*
+ * Weights and activations in 4-bit floats, the type the tensor cores multiply directly.  No counterpart in the
+ * reference, whose 4-bit weights are integers (tests/python/relax/test_codegen_cutlass.py:1358-1389); the places are those
+ * of its encode step, its matmul and its models' expert layers.
+ *
+ * A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times the scale of its block of consecutive k:
+ *   RB200_FP4_MX  blocks of 32, scale 2^(byte - 127), byte 255 = NaN
+ *   RB200_FP4_NV  blocks of 16, scale e4m3 (no sign, 0x7f = NaN), times one fp32 scale of the tensor (a device pointer,
+ *                 one per matrix of a batch; NULL: 1)
+ * Codes   uint8 [rows, k / 2], the even k in the lower nibble.  k % 32 == 0.
+ * Scales  tiles of 128 rows x 4 blocks, 512 bytes each: tile (row / 128) * ceil(blocks / 4) + block / 4, in it byte
+ *         (r % 32) * 16 + (r / 32) * 4 + b; rows and blocks past the matrix are zero.  rb200_fp4_scale_bytes(rows, k, format)
+ *         bytes a matrix, the matrices of a batch after one another.  rb200_encode_fp4 writes them so;
+ *         rb200_preprocess_fp4_scales makes them from a checkpoint's rows, uint8 [batch, rows, k / block].
+ *
+ * rb200_encode_fp4  x [batch, rows, k] (rows ldx elements apart) -> codes, scales.  In real numbers, RNE to the even code:
+ *   mx  e = max(floor(log2(max |x|)) - 2, -127), q = RNE(x / 2^e), |q| <= 6
+ *   nv  s = RNE_e4m3(max |x| / (6 ts)) <= 448, q = RNE(x / (s ts)), |q| <= 6; s = 0: q = 0
+ *   A code has the sign of its x, that of a zero too.  A block with an infinity or a NaN, or under a tensor scale that is
+ *   not positive and finite, gets the NaN scale and codes 0.
+ * rb200_decode_fp4  codes, scales -> code * scale * tensor scale, rounded to the element type.
+ */
+#define RB200_FP4_MX 0
+#define RB200_FP4_NV 1
+#define RB200_DTYPE_F16 0
+#define RB200_DTYPE_BF16 1
+#define RB200_DTYPE_F32 2
+RB200_API size_t rb200_fp4_scale_bytes(int64_t rows, int64_t k, int format);
+RB200_API int rb200_encode_fp4(const void* x, int dtype, int64_t batch, int64_t rows, int64_t k, int64_t ldx, int format,
+                               const float* tensor_scale, void* codes, void* scales, void* stream);
+RB200_API int rb200_decode_fp4(const void* codes, const void* scales, int64_t batch, int64_t rows, int64_t k, int format,
+                               const float* tensor_scale, void* out, int dtype, void* stream);
+RB200_API int rb200_preprocess_fp4_scales(const void* src, void* dst, int64_t batch, int64_t rows, int64_t k, int format,
+                                          void* stream);
+
+/*
+ * out[m, n] = unary(binary(act(ta tw sum_k a[m, k] w[n, k] + bias[n]), residual[m, n])), products of 4-bit floats summed in
+ * fp32 on the tensor cores, one rounding to out's type.  RB200_ACT_SWIGLU is refused.
+ *   rb200_gemm_fp4    both operands quantised already
+ *   rb200_linear_fp4  quantises x [m, k] (F16, BF16 or F32) first, as rb200_encode_fp4 does; desc->a and a_scales are not
+ *                     read; workspace: rb200_linear_fp4_workspace_bytes(m, k, format) bytes, 256-byte aligned, of the call's
+ *                     own until it has run.
+ * Nothing is allocated.  With launch overlap on, w and w_scales are read ahead of the previous kernel's end.
+ */
+typedef struct rb200_gemm_fp4_desc {
+  uint32_t struct_size;         /* sizeof(rb200_gemm_fp4_desc) */
+  int32_t format;               /* RB200_FP4_*, of both operands */
+  const void* a;                /* codes [m, k / 2] */
+  const void* a_scales;
+  const float* a_tensor_scale;  /* device, nv only; NULL = 1 */
+  const void* w;                /* codes [n, k / 2] */
+  const void* w_scales;
+  const float* w_tensor_scale;
+  const void* bias;             /* [n] of out's type, or NULL */
+  const void* residual;         /* [m, n] of out's type, or NULL */
+  void* out;                    /* [m, n], row stride ldo elements */
+  int64_t m, n, k, ldo;
+  int32_t out_dtype;            /* RB200_DTYPE_* */
+  int32_t activation;           /* RB200_ACT_IDENTITY .. RB200_ACT_GELU */
+  int32_t binary_op;            /* RB200_BIN_*: not NONE exactly when there is a residual */
+  int32_t unary_op;             /* RB200_UN_* */
+} rb200_gemm_fp4_desc;
+RB200_API int rb200_gemm_fp4(const rb200_gemm_fp4_desc* desc, void* stream);
+RB200_API size_t rb200_linear_fp4_workspace_bytes(int64_t m, int64_t k, int format);
+RB200_API int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb200_gemm_fp4_desc* desc, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ low-latency all-reduce */
 

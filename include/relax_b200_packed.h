@@ -129,6 +129,15 @@ RB200_API int RB200FuncListGlobalNames(int* out_size, const char*** out_array);
  *      the first row of expert 0 - how a rank that holds experts [e0, e1) of a sharded layer calls.
  *  "relax_b200.moe_gemm_q4f16"(x, w_pre [E, N, K/8] words, scales f16 [E, N, K/g], zeros|null,
  *       indptr i64 [E], group_size:int, zero_const:float, out)
+ *  Microscaled 4-bit floats (no counterpart in the reference; formats "mx" and "nv", codes and tiled scales as in relax_b200.h;
+ *  tensor scales f32 [1], or [batch], "nv" only):
+ *  "relax_b200.encode_fp4"(x f16|bf16|f32 [.., n, k], format:str, tensor_scale|null, codes u8 [.., n, k/2], scales u8)
+ *  "relax_b200.decode_fp4"(codes, scales, format:str, tensor_scale|null, out f16|bf16|f32 [.., n, k])
+ *  "relax_b200.preprocess_fp4_scales"(scales u8 [.., n, blocks], out u8)   a checkpoint's rows of scales into tiles
+ *  "relax_b200.gemm_fp4"(a, a_scales, w, w_scales, format:str, a_tensor_scale|null, w_tensor_scale|null, bias|null,
+ *       residual|null, activation:str, binary_op:str, unary_op:str, out f16|bf16|f32 [m, n])
+ *  "relax_b200.linear_fp4"(x f16|bf16|f32 [.., k], w, w_scales, format:str, x_tensor_scale|null, w_tensor_scale|null, bias|null,
+ *       residual|null, activation:str, binary_op:str, unary_op:str, workspace u8, out [.., n])
  *  "runtime.get_cuda_stream"() -> handle          src/runtime/cuda/cuda_device_api.cc:318-320
  *  "runtime.set_cuda_stream"(handle)
  */

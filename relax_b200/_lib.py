@@ -48,6 +48,20 @@ class GroupGemmDesc(ctypes.Structure):
     ]
 
 
+class GemmFp4Desc(ctypes.Structure):
+    """``rb200_gemm_fp4_desc`` of include/relax_b200.h."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("format", ctypes.c_int32),
+        ("a", ctypes.c_void_p), ("a_scales", ctypes.c_void_p), ("a_tensor_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p), ("w_scales", ctypes.c_void_p), ("w_tensor_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("ldo", ctypes.c_int64),
+        ("out_dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("binary_op", ctypes.c_int32),
+        ("unary_op", ctypes.c_int32),
+    ]
+
+
 class DLDevice(ctypes.Structure):
     _fields_ = [("device_type", ctypes.c_int32), ("device_id", ctypes.c_int32)]
 
@@ -109,6 +123,13 @@ SIGNATURES = {
                                                    _I, _I, _V, ctypes.c_size_t, _V]),
     "rb200_dequantize": (_I, [ctypes.POINTER(GemmDesc), _V, _V]),
     "rb200_group_gemm": (_I, [ctypes.POINTER(GroupGemmDesc), _V]),
+    "rb200_fp4_scale_bytes": (ctypes.c_size_t, [_I64, _I64, _I]),
+    "rb200_encode_fp4": (_I, [_V, _I, _I64, _I64, _I64, _I64, _I, _V, _V, _V, _V]),
+    "rb200_decode_fp4": (_I, [_V, _V, _I64, _I64, _I64, _I, _V, _V, _I, _V]),
+    "rb200_preprocess_fp4_scales": (_I, [_V, _V, _I64, _I64, _I64, _I, _V]),
+    "rb200_gemm_fp4": (_I, [ctypes.POINTER(GemmFp4Desc), _V]),
+    "rb200_linear_fp4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I]),
+    "rb200_linear_fp4": (_I, [_V, _I, _I64, ctypes.POINTER(GemmFp4Desc), _V, ctypes.c_size_t, _V]),
     "rb200_allreduce_workspace_bytes": (ctypes.c_size_t, [_I64]),
     "rb200_allreduce_oneshot": (_I, [ctypes.POINTER(_V), _I, _I, _V, _V, _I64, _I64, _V]),
     "rb200_allreduce_oneshot_selftest": (_I, [ctypes.POINTER(_V), ctypes.POINTER(_V), ctypes.POINTER(_V), _I,

@@ -1,0 +1,371 @@
+// Quantising to microscaled 4-bit floats, reading them back, and the layout of their scales.
+//
+// Definition, in real numbers with the named roundings only (RNE: to nearest, ties to the even code):
+//   kMx  e = max(floor(log2(max |x|)) - 2, -127),  scale 2^e,             q = RNE_e2m1(x / 2^e),      |q| <= 6
+//   kNv  s = RNE_e4m3(max |x| / (6 ts)) <= 448,    ts the tensor's scale, q = RNE_e2m1(x / (s ts)),   |q| <= 6
+// over the blocks of a row; a block whose s is 0 has codes 0, one with an infinity or a NaN the NaN scale and codes 0, and
+// where ts is not a positive finite number every block has the NaN scale.
+//
+// One pass over x: a lane takes 16 consecutive k, a warp 512.  kMx is exact in fp32 as it stands (division by a power of
+// two).  kNv divides by s * ts, which fp32 cannot hold: x is multiplied by 1 / (s ts) taken once 2^-21 too small and once too
+// large, and where the two codes differ - x lies next to the border between them - x and the border are compared in 64
+// bits, where border * s * ts is exact (3 + 4 + 24 bits).  The scale itself is rounded from a 64-bit quotient: see
+// e4m3_of.  Memory bounds it: 2 bytes read and 0.53 or 0.56 written per fp16 element.
+#include "../../include/relax_b200.h"
+#include "fp4_encode.h"
+
+namespace rb200 {
+namespace {
+using namespace f4;
+
+constexpr int kWarps = 8;
+
+template <class T>
+__device__ __forceinline__ void load16(const T* p, float (&v)[16]);
+template <>
+__device__ __forceinline__ void load16<__half>(const __half* p, float (&v)[16]) {
+  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <>
+__device__ __forceinline__ void load16<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[16]) {
+  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void load16<float>(const float* p, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 f = reinterpret_cast<const float4*>(p)[i];
+    v[4 * i] = f.x;
+    v[4 * i + 1] = f.y;
+    v[4 * i + 2] = f.z;
+    v[4 * i + 3] = f.w;
+  }
+}
+
+// RNE_e4m3 of amax / (6 ts), r = that quotient in 64 bits (off by a few 2^-53).  The borders between e4m3 values have five
+// bits, so the true quotient is on one or at least 2^-35 from it.  The detour through fp32 must not move it onto one:
+// it is cut to fp32 and, where something larger than the error was cut off, made odd.
+__device__ __forceinline__ uint32_t e4m3_of(double r) {
+  const double up = r * (1.0 + 0x1p-46);
+  float f = __double2float_rz(up);
+  if (up - (double)f > r * 0x1p-45) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return to_e4m3(f);
+}
+
+// The border between codes c and c + 1 (magnitudes).
+__device__ __forceinline__ double border_above(uint32_t c) {
+  return c < 4 ? 0.25 + 0.5 * c : c == 4 ? 2.5 : c == 5 ? 3.5 : 5.0;
+}
+// The code's magnitude of |x| / unit, by comparisons in 64 bits.
+__device__ __noinline__ uint32_t code_by_borders(double ax, double unit) {
+  uint32_t c = 0;
+  for (; c < 7; ++c) {
+    const double b = border_above(c) * unit;
+    if (!(ax > b || (ax == b && (c & 1u)))) break;  // on a border: the even one of the two
+  }
+  return c;
+}
+
+// codes of 16 elements
+template <int FMT>
+__device__ __forceinline__ void codes16(const float (&v)[16], uint32_t byte, float ts, uint32_t (&out)[2]) {
+  if (FMT == kMx) {
+    const float inv = __uint_as_float((254u - byte) << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i] * inv;
+      out[h] = to_codes8(y);
+    }
+    return;
+  }
+  const float s = e4m3_value(byte), unit = s * ts;
+  if (byte == 0u) {
+    out[0] = out[1] = 0u;
+    return;
+  }
+  const bool plain = unit >= 0x1p-100f && unit <= 0x1p100f;
+  const float inv = 1.0f / unit, below = inv * (1.0f - 0x1p-21f), above = inv * (1.0f + 0x1p-21f);
+  uint32_t hi[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i] * below;
+    out[h] = to_codes8(y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i] * above;
+    hi[h] = to_codes8(y);
+  }
+  if (out[0] == hi[0] && out[1] == hi[1] && plain) return;
+  const double exact_unit = (double)s * (double)ts;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int sh = 4 * (i & 7);
+    const uint32_t lo = (out[i >> 3] >> sh) & 15u, up = (hi[i >> 3] >> sh) & 15u;
+    if (lo != up || !plain) {
+      const double ax = fabs((double)v[i]);
+      uint32_t c;
+      if (plain) {
+        const double b = border_above(lo & 7u) * exact_unit;
+        c = ax > b || (ax == b && (lo & 1u)) ? up : lo;
+      } else {
+        c = code_by_borders(ax, exact_unit) | (v[i] < 0.0f ? 8u : 0u);
+      }
+      out[i >> 3] = (out[i >> 3] & ~(15u << sh)) | (c << sh);
+    }
+  }
+}
+
+struct EncodeParams {
+  const void* x;
+  int64_t ldx, batch_stride, rows, rows_padded, tasks;
+  int k, k_tiles, spans;
+  const float* ts;
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+template <int FMT, class T>
+__global__ void __launch_bounds__(kWarps * 32) encode_fp4_kernel(const EncodeParams p, bool activations) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  griddep_wait();
+  // (weights, scales and zero points are never written by a kernel that lets its dependents start: matmuls may read them
+  // ahead of their wait)
+  if (activations) griddep_launch_dependents();
+  if (task >= p.tasks) return;
+  const int64_t row_all = task / p.spans;  // rows of all batches, padded to whole tiles
+  const int span = (int)(task - row_all * p.spans);
+  const int64_t e = row_all / p.rows_padded, row = row_all - e * p.rows_padded;
+  const int seg = span * 32 + lane, k0 = seg * 16;
+  const bool real = row < p.rows && k0 < p.k;
+  uint32_t byte = 0u;
+  if (row < p.rows) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    if (real) load16(static_cast<const T*>(p.x) + e * p.batch_stride + row * p.ldx + k0, v);
+    uint32_t top = 0u;  // bits of max |x|: a NaN's are above infinity's
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    if (FMT == kMx) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const float ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
+    bool nan = top >= 0x7f800000u;
+    if (FMT == kMx) {
+      byte = top >> 23;
+      byte = byte > 2u ? byte - 2u : 0u;
+    } else {
+      nan = nan || !(ts > 0.0f && ts <= 3.402823466e38f);
+      byte = nan ? 0u : e4m3_of((double)__uint_as_float(top) / (6.0 * (double)ts));
+    }
+    uint32_t c[2] = {0u, 0u};
+    if (nan) byte = FMT == kMx ? 255u : 0x7fu;
+    else codes16<FMT>(v, byte, ts, c);
+    if (real)
+      *reinterpret_cast<uint2*>(p.codes + (e * p.rows + row) * (int64_t)(p.k / 2) + k0 / 2) = make_uint2(c[0], c[1]);
+    else byte = 0u;
+  }
+  // four blocks of a row are one word
+  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1;
+  uint32_t w = byte << (8 * ((lane / kLanesPerBlock) & 3));
+  w |= __shfl_xor_sync(0xffffffffu, w, kLanesPerBlock);
+  w |= __shfl_xor_sync(0xffffffffu, w, 2 * kLanesPerBlock);
+  const int q = seg / (4 * kLanesPerBlock);
+  if (lane % (4 * kLanesPerBlock) == 0 && q < p.k_tiles)
+    *reinterpret_cast<uint32_t*>(p.scales + e * (p.rows_padded / 128) * p.k_tiles * 512 + scale_word(row, q, p.k_tiles)) = w;
+}
+
+struct DecodeParams {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t rows, rows_padded, tasks;
+  int k, k_tiles, spans;
+  const float* ts;
+  void* out;
+};
+
+template <class T>
+__device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
+  constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 16 / kPer; ++i) {
+    __align__(16) T t[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) t[j] = narrow<T>(v[i * kPer + j]);
+    reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(t);
+  }
+}
+
+template <int FMT, class T>
+__global__ void __launch_bounds__(kWarps * 32) decode_fp4_kernel(const DecodeParams p) {
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (task >= p.tasks) return;
+  const int64_t row_all = task / p.spans;
+  const int seg = (int)(task - row_all * p.spans) * 32 + lane, k0 = seg * 16;
+  if (k0 >= p.k) return;
+  const int64_t e = row_all / p.rows, row = row_all - e * p.rows;
+  const uint2 c = *reinterpret_cast<const uint2*>(p.codes + row_all * (int64_t)(p.k / 2) + k0 / 2);
+  const int blk = FMT == kMx ? seg >> 1 : seg;
+  const uint32_t byte = p.scales[e * (p.rows_padded / 128) * p.k_tiles * 512 + scale_word(row, blk >> 2, p.k_tiles) + (blk & 3)];
+  const float s = scale_value<FMT>(byte), ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
+  float v[16];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[4];
+    from_codes8(h ? c.y : c.x, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[8 * h + 2 * i] = f.x * s * ts;  // code * scale is exact in fp32
+      v[8 * h + 2 * i + 1] = f.y * s * ts;
+    }
+  }
+  store16(static_cast<T*>(p.out) + row_all * (int64_t)p.k + k0, v);
+}
+
+// a thread per word of the result
+__global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* src, uint32_t* dst, int64_t words, int64_t rows, int row_tiles,
+                                                          int k_tiles, int blocks) {
+  griddep_wait();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= words) return;
+  const int in_tile = (int)(i & 127);
+  const int64_t tile = i >> 7, q = tile % k_tiles, rt = (tile / k_tiles) % row_tiles, e = tile / ((int64_t)k_tiles * row_tiles);
+  const int64_t row = rt * 128 + (in_tile & 3) * 32 + (in_tile >> 2);
+  uint32_t w = 0u;
+  if (row < rows) {
+    const uint8_t* s = src + (e * rows + row) * blocks + q * 4;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (q * 4 + b < blocks) w |= (uint32_t)s[b] << (8 * b);
+  }
+  dst[i] = w;
+}
+
+template <int FMT>
+int encode_typed(const EncodeParams& p, int dtype, bool activations, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.tasks + kWarps - 1) / kWarps));
+  if (dtype == kF16)
+    RB200_CUDA(launch_dependent(encode_fp4_kernel<FMT, __half>, grid, kWarps * 32, 0, stream, p, activations));
+  else if (dtype == kBf16)
+    RB200_CUDA(launch_dependent(encode_fp4_kernel<FMT, __nv_bfloat16>, grid, kWarps * 32, 0, stream, p, activations));
+  else
+    RB200_CUDA(launch_dependent(encode_fp4_kernel<FMT, float>, grid, kWarps * 32, 0, stream, p, activations));
+  return 0;
+}
+template <int FMT>
+int decode_typed(const DecodeParams& p, int dtype, cudaStream_t stream) {
+  const dim3 grid((unsigned)((p.tasks + kWarps - 1) / kWarps));
+  if (dtype == kF16) RB200_CUDA(launch_dependent(decode_fp4_kernel<FMT, __half>, grid, kWarps * 32, 0, stream, p));
+  else if (dtype == kBf16) RB200_CUDA(launch_dependent(decode_fp4_kernel<FMT, __nv_bfloat16>, grid, kWarps * 32, 0, stream, p));
+  else RB200_CUDA(launch_dependent(decode_fp4_kernel<FMT, float>, grid, kWarps * 32, 0, stream, p));
+  return 0;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+int fp4_encode_launch(const void* x, int dtype, int64_t batch, int64_t rows, int64_t k, int64_t ldx, int64_t batch_stride, int fmt,
+                      const float* tensor_scale, void* codes, void* scales, bool activations, cudaStream_t stream) {
+  EncodeParams p;
+  p.x = x;
+  p.ldx = ldx;
+  p.batch_stride = batch_stride;
+  p.rows = rows;
+  p.rows_padded = scale_row_tiles(rows) * 128;
+  p.k = (int)k;
+  p.k_tiles = (int)scale_k_tiles(k, fmt);
+  p.spans = (p.k_tiles * 4 * block_of(fmt) + 511) / 512;
+  p.tasks = batch * p.rows_padded * p.spans;
+  p.ts = tensor_scale;
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = static_cast<uint8_t*>(scales);
+  if (p.tasks == 0) return 0;
+  RB200_CHECK((p.tasks + kWarps - 1) / kWarps < (1ll << 31), "too many elements to quantise in one call");
+  return fmt == kMx ? encode_typed<kMx>(p, dtype, activations, stream) : encode_typed<kNv>(p, dtype, activations, stream);
+}
+
+}  // namespace rb200
+
+using namespace rb200;
+
+extern "C" {
+
+size_t rb200_fp4_scale_bytes(int64_t rows, int64_t k, int format) {
+  if ((format != f4::kMx && format != f4::kNv) || rows < 0 || k <= 0) return 0;
+  return (size_t)f4::scale_bytes(rows, k, format);
+}
+
+int rb200_encode_fp4(const void* x, int dtype, int64_t batch, int64_t rows, int64_t k, int64_t ldx, int format,
+                     const float* tensor_scale, void* codes, void* scales, void* stream) {
+  RB200_FP4_CHECK_SHAPE(format, rows, k);
+  RB200_CHECK(dtype >= f4::kF16 && dtype <= f4::kF32, "unknown element type %d", dtype);
+  RB200_CHECK(batch >= 0, "batch must not be negative");
+  if (batch == 0 || rows == 0) return 0;
+  RB200_CHECK(x && codes && scales, "x, codes and scales must be non-NULL");
+  RB200_CHECK(format == f4::kNv || !tensor_scale, "the mx format has no tensor scale");
+  const int64_t width = dtype == f4::kF32 ? 4 : 2;
+  RB200_CHECK(ldx >= k && ldx * width % 16 == 0 && aligned16(x) && aligned16(codes) && aligned16(scales),
+              "x rows, codes and scales must be 16-byte aligned (ldx=%lld)", (long long)ldx);
+  return fp4_encode_launch(x, dtype, batch, rows, k, ldx, rows * ldx, format, tensor_scale, codes, scales, false,
+                           static_cast<cudaStream_t>(stream));
+}
+
+int rb200_decode_fp4(const void* codes, const void* scales, int64_t batch, int64_t rows, int64_t k, int format,
+                     const float* tensor_scale, void* out, int dtype, void* stream) {
+  RB200_FP4_CHECK_SHAPE(format, rows, k);
+  RB200_CHECK(dtype >= f4::kF16 && dtype <= f4::kF32, "unknown element type %d", dtype);
+  RB200_CHECK(batch >= 0, "batch must not be negative");
+  if (batch == 0 || rows == 0) return 0;
+  RB200_CHECK(codes && scales && out, "codes, scales and out must be non-NULL");
+  RB200_CHECK(format == f4::kNv || !tensor_scale, "the mx format has no tensor scale");
+  RB200_CHECK(aligned16(codes) && aligned16(scales) && aligned16(out), "codes, scales and out must be 16-byte aligned");
+  DecodeParams p;
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = static_cast<const uint8_t*>(scales);
+  p.rows = rows;
+  p.rows_padded = f4::scale_row_tiles(rows) * 128;
+  p.k = (int)k;
+  p.k_tiles = (int)f4::scale_k_tiles(k, format);
+  p.spans = (int)((k + 511) / 512);
+  p.tasks = batch * rows * p.spans;
+  p.ts = tensor_scale;
+  p.out = out;
+  RB200_CHECK((p.tasks + kWarps - 1) / kWarps < (1ll << 31), "too many elements to read back in one call");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return format == f4::kMx ? decode_typed<f4::kMx>(p, dtype, s) : decode_typed<f4::kNv>(p, dtype, s);
+}
+
+int rb200_preprocess_fp4_scales(const void* src, void* dst, int64_t batch, int64_t rows, int64_t k, int format, void* stream) {
+  RB200_FP4_CHECK_SHAPE(format, rows, k);
+  RB200_CHECK(batch >= 0, "batch must not be negative");
+  if (batch == 0 || rows == 0) return 0;
+  RB200_CHECK(src && dst && src != dst, "src and dst must be non-NULL and different");
+  RB200_CHECK(aligned16(dst), "dst must be 16-byte aligned");
+  const int64_t row_tiles = f4::scale_row_tiles(rows), k_tiles = f4::scale_k_tiles(k, format), words = batch * row_tiles * k_tiles * 128;
+  RB200_CHECK((words + 255) / 256 < (1ll << 31), "too many scales for one call");
+  RB200_CUDA(launch_dependent(tile_scales_kernel, dim3((unsigned)((words + 255) / 256)), 256, 0, static_cast<cudaStream_t>(stream),
+                              static_cast<const uint8_t*>(src), static_cast<uint32_t*>(dst), words, rows, (int)row_tiles, (int)k_tiles,
+                              (int)(k / f4::block_of(format))));
+  return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,445 @@
+// out = unary(binary(act(ta tw sum_k a[m, k] w[n, k] + bias[n]), residual[m, n])) of two microscaled 4-bit operands.
+//
+// The tensor cores take codes and block scales as they are (tcgen05.mma, block_scale): nothing is decoded.  The tile is
+// out^T, 128 rows of w by nb rows of a, so that a batch of any size is the MMA's N; a stage is 256 k: two tensor-map loads of
+// codes and the scale tiles, which the MMA's thread copies into tensor memory ahead of the MMAs that read them.
+// With few tiles k is cut over the CTAs of a cluster: each keeps its partial tile in shared memory (the stages' memory, done
+// with by then), and each adds up its share of the batch rows in the order of the ranks, so that a result does not depend
+// on timing.
+#include <atomic>
+
+#include <cstring>
+
+#include "fp4_encode.h"
+#include "fp4_gemm.h"
+#include "fp4_mma.cuh"
+#include "tensormap.h"
+
+namespace rb200 {
+namespace f4 {
+namespace {
+
+using ug::elect_one;
+using ug::make_b_desc;
+using ug::tc_commit;
+using ug::tc_fence_after;
+using ug::tc_fence_before;
+using ug::tc_ld16;
+using ug::tmem_alloc;
+using ug::tmem_dealloc;
+using ug::tmem_relinquish;
+
+constexpr int kThreads = 192;
+constexpr int kTileN = 128;
+constexpr int kMaxStages = 8;
+constexpr int kWBytes = kTileN * 128;
+
+__device__ int g_status;
+
+struct Params {
+  const uint8_t* a_scales;
+  const uint8_t* w_scales;
+  const float* a_ts;
+  const float* w_ts;
+  const void* bias;
+  const void* residual;
+  void* out;
+  int64_t ldo, ld_res;
+  int m, n, k, k_tiles;
+  int act, binop, unop;
+  int nb, stages, tmem_cols, m_tiles, cluster, early;
+};
+
+size_t stage_bytes(int fmt, int nb) {
+  return (size_t)kWBytes + (size_t)nb * 128 + (size_t)stage_tiles(fmt) * 512 * (1 + (nb + 127) / 128);
+}
+size_t smem_bytes(int fmt, int nb, int stages) { return 1024 + stages * stage_bytes(fmt, nb) + (2 * kMaxStages + 2) * 8 + 32; }
+
+__device__ __forceinline__ float activation(float v, int act) {
+  switch (act) {
+    case RB200_ACT_RELU: return fmaxf(v, 0.0f);
+    case RB200_ACT_SILU: return v / (1.0f + __expf(-v));
+    case RB200_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    default: return v;
+  }
+}
+template <class T>
+__device__ __forceinline__ float finish(const Params& p, float v, float alpha, int m, int n) {
+  v *= alpha;
+  if (p.bias) v += widen(static_cast<const T*>(p.bias)[n]);
+  v = activation(v, p.act);
+  if (p.residual) {
+    const float r = widen(static_cast<const T*>(p.residual)[m * p.ld_res + n]);
+    v = p.binop == RB200_BIN_MULTIPLY ? v * r : v + r;
+  }
+  return p.unop == RB200_UN_RELU ? fmaxf(v, 0.0f) : v;
+}
+
+template <int FMT, class T>
+__global__ void __launch_bounds__(kThreads)
+    fp4_gemm_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a) {
+  constexpr int NT = stage_tiles(FMT);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int nb = p.nb, stages = p.stages, a_bytes = nb * 128, a_tiles = (nb + 127) / 128;
+  const int code_bytes = kWBytes + a_bytes, scale_bytes = NT * 512 * (1 + a_tiles);
+  uint8_t* codes = smem;                                   // [stage][w | a]
+  uint8_t* scales = smem + (size_t)stages * code_bytes;    // [stage][w tiles | a tiles of the first 128 rows | of the next]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + (size_t)stages * scale_bytes);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* d_full = empty + kMaxStages;
+  uint32_t* holder = reinterpret_cast<uint32_t*>(d_full + 2);  // [0] tensor memory, [1] a CTA of the cluster failed
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), tile = blockIdx.x / p.cluster;
+  const int m0 = (tile % p.m_tiles) * nb, n0 = (tile / p.m_tiles) * kTileN;
+  const int chunks = (p.k + kStageK - 1) / kStageK;
+  const int c0 = (int)((int64_t)chunks * rank / p.cluster), c1 = (int)((int64_t)chunks * (rank + 1) / p.cluster);
+
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(d_full, 1);
+    holder[1] = 0u;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(holder, (uint32_t)p.tmem_cols);
+    tmem_relinquish();
+  }
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch_dependents();
+  const uint32_t tmem = holder[0];
+  const int w_col = (nb + 31) / 32 * 32, a_col = w_col + 4 * NT;  // tensor memory columns of the scales
+  bool ok = true;
+
+  if (warp == 0) {
+    // ============================================================ loads
+    const bool leader = elect_one();
+    // bytes of the scale tiles of chunk c for 128 rows
+    auto tiles_of = [&](int c) { return (uint32_t)min(NT, p.k_tiles - c * NT) * 512u; };
+    auto load_w = [&](int s, int c) {
+      uint8_t* at = scales + (size_t)s * scale_bytes;
+      mbar_arrive_expect_tx(&full[s], (uint32_t)code_bytes + tiles_of(c) * (1 + a_tiles));
+      tma_load(codes + (size_t)s * code_bytes, &tmap_w, c * 128, n0, &full[s]);
+      bulk_g2s(at, p.w_scales + ((int64_t)(n0 >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c), &full[s]);
+    };
+    auto load_a = [&](int s, int c) {
+      uint8_t* at = scales + (size_t)s * scale_bytes + NT * 512;
+      tma_load(codes + (size_t)s * code_bytes + kWBytes, &tmap_a, c * 128, m0, &full[s]);
+      for (int i = 0; i < a_tiles; ++i)
+        // (a second tile of 128 rows that the batch does not reach: the first one again, its rows are never stored)
+        bulk_g2s(at + i * NT * 512, p.a_scales + ((int64_t)min((m0 >> 7) + i, (p.m - 1) >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c),
+                 &full[s]);
+    };
+    const int first = min(stages, c1 - c0);  // stages filled before any is free again
+    if (leader) {
+      if (p.early) {
+        for (int s = 0; s < first; ++s) load_w(s, c0 + s);
+      } else {
+        for (int s = 0; s < first; ++s) tma_prefetch(&tmap_w, (c0 + s) * 128, n0);
+      }
+    }
+    griddep_wait();
+    if (leader)
+      for (int s = 0; s < first; ++s) {
+        if (!p.early) load_w(s, c0 + s);
+        load_a(s, c0 + s);
+      }
+    int s = 0, issued = first;
+    uint32_t ph = 0;
+    for (int c = c0 + first; c < c1; ++c) {
+      if (!mbar_wait_parked(&empty[s], ph, &g_status)) {
+        ok = false;
+        break;
+      }
+      if (leader) {
+        load_w(s, c);
+        load_a(s, c);
+      }
+      ++issued;
+      __syncwarp();
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+    // nothing may be on its way into this CTA's memory when it leaves: the last fill of every stage
+    for (int i = max(0, issued - stages); i < issued; ++i)
+      ok = mbar_wait_parked(&full[i % stages], (uint32_t)(i / stages) & 1u, &g_status) && ok;
+  } else if (warp == 1) {
+    // ============================================================ scales into tensor memory, MMAs
+    const bool leader = elect_one();
+    const uint32_t idesc = mma_desc<FMT>(kTileN, nb);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int c = c0; c < c1; ++c) {
+      if (!mbar_wait_parked(&full[s], ph, &g_status)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (leader) {
+        const uint64_t w_desc = make_b_desc(smem_u32(codes + (size_t)s * code_bytes));
+        const uint64_t a_desc = w_desc + (uint64_t)(kWBytes >> 4);
+        const uint64_t sc = scale_desc(smem_u32(scales + (size_t)s * scale_bytes));
+        const int tiles = min(NT, p.k_tiles - c * NT), mmas = (min(kStageK, p.k - c * kStageK) + kMmaK - 1) / kMmaK;
+        for (int t = 0; t < tiles; ++t) copy_scales(tmem + w_col + 4 * t, sc + (uint64_t)(t * (512 >> 4)));
+        for (int t = 0; t < tiles; ++t)
+          for (int i = 0; i < a_tiles; ++i)
+            copy_scales(tmem + a_col + (t * a_tiles + i) * 4, sc + (uint64_t)((NT + i * NT + t) * (512 >> 4)));
+        for (int j = 0; j < mmas; ++j) {
+          const int t = FMT == kMx ? j >> 1 : j;
+          mma_scaled<FMT>(tmem, w_desc + j * 2, a_desc + j * 2, FMT == kMx && (j & 1) ? upper_half(idesc) : idesc, tmem + w_col + 4 * t,
+                          tmem + a_col + t * a_tiles * 4, (c > c0 || j > 0) ? 1u : 0u);
+        }
+        tc_commit(&empty[s]);
+      }
+      __syncwarp();
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+    if (ok && leader) tc_commit(d_full);
+    __syncwarp();
+  }
+
+  // ============================================================ the tile, by batch rows: [nb][128] fp32 where the stages were
+  float* part = reinterpret_cast<float*>(smem);
+  griddep_wait();
+  ok = mbar_wait_parked(d_full, 0, &g_status) && ok;  // every stage has been read
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) {
+    for (int r = 0; r < p.cluster; ++r) st_cluster(at_rank(smem_u32(holder + 1), r), 1u);
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp >= 2 && ok) {
+    const int quad = warp & 3;
+    const uint32_t lane_taddr = (uint32_t)(32 * quad) << 16;
+    for (int c = 0; c < nb; c += 16) {
+      if (m0 + c >= p.m) break;
+      float v[16];
+      tc_ld16(lane_taddr | (tmem + c), v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[(c + i) * kTileN + quad * 32 + lane] = v[i];
+    }
+  }
+  tc_fence_before();
+  if (p.cluster > 1) cluster_sync();
+  else __syncthreads();
+  if (holder[1] == 0u) {
+    const float alpha = (p.a_ts ? *p.a_ts : 1.0f) * (p.w_ts ? *p.w_ts : 1.0f);
+    const int rows = min(nb, p.m - m0), lo = rows * rank / p.cluster, hi = rows * (rank + 1) / p.cluster;
+    const int n = n0 + lane * 4;
+    T* out = static_cast<T*>(p.out);
+    const bool wide = n + 4 <= p.n && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && p.ldo % 4 == 0;
+    for (int r = lo + warp; r < hi; r += kThreads / 32) {
+      const uint32_t at = smem_u32(part + r * kTileN + lane * 4);
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int q = 0; q < p.cluster; ++q) {
+        const float4 o = ld_cluster4(p.cluster > 1 ? at_rank(at, q) : at);
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      const int m = m0 + r;
+      __align__(16) T t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = n + i < p.n ? narrow<T>(finish<T>(p, f[i], alpha, m, n + i)) : narrow<T>(0.0f);
+      T* dst = out + m * p.ldo + n;
+      if (wide) {
+        if (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
+        else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.n) dst[i] = t[i];
+      }
+    }
+  }
+  if (p.cluster > 1) cluster_sync();  // others may still be reading this CTA's part
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+  }
+}
+
+constexpr int kMaxDevices = 64;
+std::atomic<bool> g_launched[kMaxDevices];  // devices whose status word a wait may have set
+
+template <int FMT, class T>
+int launch_typed(Params& p, const CUtensorMap& tw, const CUtensorMap& ta, cudaStream_t stream) {
+  auto kern = fp4_gemm_kernel<FMT, T>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    RB200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    configured_device = dev;
+  }
+  const int n_tiles = (p.n + kTileN - 1) / kTileN, tiles = n_tiles * p.m_tiles, chunks = (p.k + kStageK - 1) / kStageK;
+  p.cluster = 1;
+  while (p.cluster < 8 && tiles * p.cluster * 2 <= 2 * sm_count_current() && chunks >= 4 * p.cluster) p.cluster *= 2;
+  p.stages = kMaxStages;
+  const size_t room = (size_t)(p.nb <= 64 ? 113 : 226) * 1024;  // two CTAs of an SM, or one
+  while (p.stages > 2 && smem_bytes(FMT, p.nb, p.stages) > room) --p.stages;
+  size_t smem = smem_bytes(FMT, p.nb, p.stages);
+  RB200_CHECK(smem <= 227 * 1024 && (size_t)p.nb * kTileN * 4 <= p.stages * stage_bytes(FMT, p.nb), "no room for the tile");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.cluster), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  RB200_CUDA(cudaLaunchKernelEx(&cfg, kern, p, tw, ta));
+  return 0;
+}
+
+template <int FMT>
+int launch_fmt(Params& p, int dtype, const CUtensorMap& tw, const CUtensorMap& ta, cudaStream_t stream) {
+  switch (dtype) {
+    case kF16: return launch_typed<FMT, __half>(p, tw, ta, stream);
+    case kBf16: return launch_typed<FMT, __nv_bfloat16>(p, tw, ta, stream);
+    default: return launch_typed<FMT, float>(p, tw, ta, stream);
+  }
+}
+
+}  // namespace
+}  // namespace f4
+
+int fp4_gemm_read_status(int* status_out) {
+  *status_out = 0;
+  int dev = -1;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= f4::kMaxDevices || !f4::g_launched[dev].load(std::memory_order_relaxed)) return 0;
+  int v = 0;
+  RB200_CUDA(cudaMemcpyFromSymbol(&v, f4::g_status, sizeof(int)));
+  if (v != 0) {
+    const int zero = 0;
+    RB200_CUDA(cudaMemcpyToSymbol(f4::g_status, &zero, sizeof(int)));
+  }
+  *status_out = v;
+  return 0;
+}
+
+int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
+  using namespace f4;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.a_scales = static_cast<const uint8_t*>(d.a_scales);
+  p.w_scales = static_cast<const uint8_t*>(d.w_scales);
+  p.a_ts = d.a_tensor_scale;
+  p.w_ts = d.w_tensor_scale;
+  p.bias = d.bias;
+  p.residual = d.residual;
+  p.out = d.out;
+  p.ldo = d.ldo;
+  p.ld_res = d.n;
+  p.m = (int)d.m;
+  p.n = (int)d.n;
+  p.k = (int)d.k;
+  p.k_tiles = (int)scale_k_tiles(d.k, d.format);
+  p.act = d.activation;
+  p.binop = d.residual ? d.binary_op : RB200_BIN_NONE;
+  p.unop = d.unary_op;
+  p.early = launch_overlap_enabled() ? 1 : 0;
+  p.nb = d.m <= 256 ? (int)((d.m + 15) / 16 * 16) : 256;
+  p.m_tiles = (int)((d.m + p.nb - 1) / p.nb);
+  const int cols = (p.nb + 31) / 32 * 32 + 4 * stage_tiles(d.format) * (1 + (p.nb + 127) / 128);
+  p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
+  CUtensorMap tw, ta;
+  if (make_tensor_map_2d(&tw, d.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.n,
+                         (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tensor_map_2d(&ta, d.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.m,
+                         (unsigned long long)d.k / 2, 128, (unsigned)p.nb, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+    return -1;
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < kMaxDevices) g_launched[dev].store(true, std::memory_order_relaxed);
+  return d.format == kMx ? launch_fmt<kMx>(p, d.out_dtype, tw, ta, stream) : launch_fmt<kNv>(p, d.out_dtype, tw, ta, stream);
+}
+
+}  // namespace rb200
+
+using namespace rb200;
+
+namespace {
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// what rb200_gemm_fp4 and rb200_linear_fp4 check alike
+int check_gemm(const rb200_gemm_fp4_desc* d) {
+  RB200_CHECK(d != nullptr && d->struct_size == sizeof(rb200_gemm_fp4_desc), "rb200_gemm_fp4_desc has a wrong struct_size");
+  RB200_FP4_CHECK_SHAPE(d->format, d->m, d->k);
+  RB200_CHECK(d->n > 0 && d->n < (1ll << 30), "n=%lld out of range", (long long)d->n);
+  RB200_CHECK(d->out_dtype >= f4::kF16 && d->out_dtype <= f4::kF32, "unknown element type %d", d->out_dtype);
+  RB200_CHECK(d->activation >= RB200_ACT_IDENTITY && d->activation <= RB200_ACT_GELU, "unknown activation %d", d->activation);
+  RB200_CHECK(d->binary_op >= RB200_BIN_NONE && d->binary_op <= RB200_BIN_MULTIPLY, "unknown binary op %d", d->binary_op);
+  RB200_CHECK(d->unary_op >= RB200_UN_IDENTITY && d->unary_op <= RB200_UN_RELU, "unknown unary op %d", d->unary_op);
+  RB200_CHECK((d->binary_op != RB200_BIN_NONE) == (d->residual != nullptr), "a residual needs a binary op, and the other way round");
+  RB200_CHECK(d->ldo >= d->n, "ldo=%lld is less than n", (long long)d->ldo);
+  RB200_CHECK(d->format == f4::kNv || (!d->a_tensor_scale && !d->w_tensor_scale), "the mx format has no tensor scale");
+  if (d->m == 0) return 0;
+  RB200_CHECK(d->w && d->w_scales && d->out, "w, w_scales and out must be non-NULL");
+  RB200_CHECK(aligned16(d->w) && aligned16(d->w_scales), "codes and scales must be 16-byte aligned");
+  const uintptr_t width = d->out_dtype == f4::kF32 ? 4 : 2;
+  RB200_CHECK(reinterpret_cast<uintptr_t>(d->out) % width == 0 && reinterpret_cast<uintptr_t>(d->bias) % width == 0 &&
+                  reinterpret_cast<uintptr_t>(d->residual) % width == 0,
+              "out, bias and residual must be aligned to their elements");
+  return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int rb200_gemm_fp4(const rb200_gemm_fp4_desc* d, void* stream) {
+  if (check_gemm(d) != 0) return -1;
+  if (d->m == 0) return 0;
+  RB200_CHECK(d->a && d->a_scales && aligned16(d->a) && aligned16(d->a_scales), "a and a_scales must be non-NULL and 16-byte aligned");
+  return fp4_gemm_launch(*d, static_cast<cudaStream_t>(stream));
+}
+
+size_t rb200_linear_fp4_workspace_bytes(int64_t m, int64_t k, int format) {
+  if ((format != f4::kMx && format != f4::kNv) || m <= 0 || k <= 0) return 0;
+  return (size_t)((m * (k / 2) + 255) / 256 * 256 + f4::scale_bytes(m, k, format));
+}
+
+int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb200_gemm_fp4_desc* desc, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (check_gemm(desc) != 0) return -1;
+  RB200_CHECK(x_dtype >= f4::kF16 && x_dtype <= f4::kF32, "unknown element type %d", x_dtype);
+  if (desc->m == 0) return 0;
+  rb200_gemm_fp4_desc d = *desc;
+  const int64_t width = x_dtype == f4::kF32 ? 4 : 2;
+  RB200_CHECK(x && ldx >= d.k && ldx * width % 16 == 0 && aligned16(x), "x must be non-NULL, its rows 16-byte aligned (ldx=%lld)",
+              (long long)ldx);
+  RB200_CHECK(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                  workspace_bytes >= rb200_linear_fp4_workspace_bytes(d.m, d.k, d.format),
+              "the workspace must be 256-byte aligned and hold rb200_linear_fp4_workspace_bytes");
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + (d.m * (d.k / 2) + 255) / 256 * 256;
+  if (fp4_encode_launch(x, x_dtype, 1, d.m, d.k, ldx, 0, d.format, d.a_tensor_scale, codes, scales, true,
+                        static_cast<cudaStream_t>(stream)) != 0)
+    return -1;
+  d.a = codes;
+  d.a_scales = scales;
+  return fp4_gemm_launch(d, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

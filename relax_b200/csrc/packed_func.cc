@@ -773,6 +773,208 @@ int pf_set_stream(RB200Value* v, int* tc, int n, RB200Value*, int* ret_tc, void*
   return 0;
 }
 
+// ------------------------------------------------------------------ microscaled 4-bit floats
+int fp4_format(const Args& a, int i, int* fmt) {
+  const char* s;
+  if (a.str(i, &s)) return -1;
+  PF_CHECK(strcmp(s, "mx") == 0 || strcmp(s, "nv") == 0, "%s: unknown 4-bit format '%s' (mx or nv)", a.fname, s);
+  *fmt = s[0] == 'm' ? RB200_FP4_MX : RB200_FP4_NV;
+  return 0;
+}
+int float_type(const char* fn, const char* what, const DLTensor* t, int* out) {
+  if (is_dtype(t, kDLFloat, 16)) *out = RB200_DTYPE_F16;
+  else if (is_dtype(t, kDLBfloat, 16)) *out = RB200_DTYPE_BF16;
+  else if (is_dtype(t, kDLFloat, 32)) *out = RB200_DTYPE_F32;
+  else PF_CHECK(false, "%s: %s must be float16, bfloat16 or float32", fn, what);
+  return 0;
+}
+int same_type(const char* fn, const char* what, const DLTensor* t, const DLTensor* like) {
+  return check_tensor(fn, what, t, like->dtype.code, like->dtype.bits);
+}
+// codes uint8 [.., rows, k / 2] of `batch` matrices with their scales and tensor scales
+struct Fp4Matrix {
+  int64_t batch, rows, k;
+  const void* codes;
+  const void* scales;
+  const float* ts;
+};
+int fp4_matrix(const char* fn, const char* what, int ndim, int fmt, const DLTensor* codes, const DLTensor* scales, const DLTensor* ts,
+               Fp4Matrix* out) {
+  if (check_tensor(fn, what, codes, kDLUInt, 8) || check_tensor(fn, "scales", scales, kDLUInt, 8)) return -1;
+  PF_CHECK((codes->ndim == 2 || codes->ndim == 3) && (ndim == 0 || codes->ndim == ndim), "%s: %s has %d dimensions", fn, what,
+           codes->ndim);
+  const int lead = codes->ndim - 2;
+  out->batch = lead ? codes->shape[0] : 1;
+  out->rows = codes->shape[lead];
+  out->k = codes->shape[lead + 1] * 2;
+  PF_CHECK(out->k > 0 && out->k % 32 == 0, "%s: %s needs k %% 32 == 0 (k=%lld)", fn, what, (long long)out->k);
+  const int64_t need = out->batch * (int64_t)rb200_fp4_scale_bytes(out->rows, out->k, fmt);
+  PF_CHECK(numel(scales) == need, "%s: the scales of %s hold %lld bytes, %lld expected in tiles of 128 rows x 4 blocks", fn, what,
+           (long long)numel(scales), (long long)need);
+  out->codes = data_of(codes);
+  out->scales = data_of(scales);
+  out->ts = nullptr;
+  if (ts) {
+    if (check_tensor(fn, "tensor scale", ts, kDLFloat, 32)) return -1;
+    PF_CHECK(numel(ts) == out->batch, "%s: %s has %lld tensor scales, expected %lld", fn, what, (long long)numel(ts),
+             (long long)out->batch);
+    out->ts = static_cast<const float*>(data_of(ts));
+  }
+  return 0;
+}
+// (x, format, tensor_scale|null, codes, scales)
+int pf_encode_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, void*) {
+  const char* fname = "relax_b200.encode_fp4";
+  Args a{v, tc, n_args, fname};
+  PF_CHECK(n_args == 5, "%s expects 5 arguments, got %d", fname, n_args);
+  const DLTensor *x, *ts, *codes, *scales;
+  int fmt, type;
+  if (a.tensor(0, &x) || fp4_format(a, 1, &fmt) || a.tensor(2, &ts, true) || a.tensor(3, &codes) || a.tensor(4, &scales) ||
+      float_type(fname, "x", x, &type))
+    return -1;
+  PF_CHECK(x->ndim == codes->ndim, "%s: codes must have the dimensions of x", fname);
+  Fp4Matrix q;
+  if (fp4_matrix(fname, "codes", 0, fmt, codes, scales, ts, &q)) return -1;
+  const int lead = x->ndim - 2;
+  PF_CHECK((!lead || x->shape[0] == q.batch) && x->shape[lead] == q.rows && x->shape[lead + 1] == q.k,
+           "%s: codes must be uint8 [.., n, k / 2] for x [.., n, k]", fname);
+  int64_t ldx = q.k;
+  if (!lead && x->strides && x->strides[1] == 1 && x->strides[0] >= q.k && q.rows > 1) {
+    ldx = x->strides[0];  // rows of a wider matrix
+    DLTensor row = *x;
+    row.strides = nullptr;
+    if (same_type(fname, "x", &row, x)) return -1;
+  } else if (same_type(fname, "x", x, x)) {
+    return -1;
+  }
+  if (ret_tc) *ret_tc = RB200_ARG_NULL;
+  return rb200_encode_fp4(data_of(x), type, q.batch, q.rows, q.k, ldx, fmt, q.ts, const_cast<void*>(q.codes),
+                          const_cast<void*>(q.scales), rb200_get_stream());
+}
+// (codes, scales, format, tensor_scale|null, out)
+int pf_decode_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, void*) {
+  const char* fname = "relax_b200.decode_fp4";
+  Args a{v, tc, n_args, fname};
+  PF_CHECK(n_args == 5, "%s expects 5 arguments, got %d", fname, n_args);
+  const DLTensor *codes, *scales, *ts, *out;
+  int fmt, type;
+  Fp4Matrix q;
+  if (a.tensor(0, &codes) || a.tensor(1, &scales) || fp4_format(a, 2, &fmt) || a.tensor(3, &ts, true) || a.tensor(4, &out) ||
+      float_type(fname, "out", out, &type) || same_type(fname, "out", out, out) || fp4_matrix(fname, "codes", 0, fmt, codes, scales, ts, &q))
+    return -1;
+  PF_CHECK(numel(out) == q.batch * q.rows * q.k, "%s: out must be [.., n, k]", fname);
+  if (ret_tc) *ret_tc = RB200_ARG_NULL;
+  return rb200_decode_fp4(q.codes, q.scales, q.batch, q.rows, q.k, fmt, q.ts, data_of(out), type, rb200_get_stream());
+}
+// (scales u8 [.., n, k / block], out)
+int pf_preprocess_fp4_scales(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, void*) {
+  const char* fname = "relax_b200.preprocess_fp4_scales";
+  Args a{v, tc, n_args, fname};
+  PF_CHECK(n_args == 2, "%s expects 2 arguments, got %d", fname, n_args);
+  const DLTensor *src, *out;
+  if (a.tensor(0, &src) || a.tensor(1, &out) || check_tensor(fname, "scales", src, kDLUInt, 8) ||
+      check_tensor(fname, "out", out, kDLUInt, 8))
+    return -1;
+  PF_CHECK(src->ndim == 2 || src->ndim == 3, "%s: scales must be [n, blocks] or [batch, n, blocks]", fname);
+  const int lead = src->ndim - 2;
+  const int64_t batch = lead ? src->shape[0] : 1, rows = src->shape[lead], blocks = src->shape[lead + 1];
+  // tiles are counted in blocks, so blocks of 32 stand for either format
+  const int64_t need = batch * (int64_t)rb200_fp4_scale_bytes(rows, blocks * 32, RB200_FP4_MX);
+  PF_CHECK(blocks > 0 && numel(out) == need, "%s: out holds %lld bytes, %lld expected", fname, (long long)numel(out), (long long)need);
+  if (ret_tc) *ret_tc = RB200_ARG_NULL;
+  return rb200_preprocess_fp4_scales(data_of(src), data_of(out), batch, rows, blocks * 32, RB200_FP4_MX, rb200_get_stream());
+}
+// bias, residual, activation, binary_op, unary_op from argument i on; `out` last
+int fp4_epilogue(const Args& a, int i, const DLTensor* out, rb200_gemm_fp4_desc* d) {
+  const DLTensor *bias, *res;
+  const char *act, *bin, *un;
+  if (a.tensor(i, &bias, true) || a.tensor(i + 1, &res, true) || a.str(i + 2, &act) || a.str(i + 3, &bin) || a.str(i + 4, &un) ||
+      float_type(a.fname, "out", out, &d->out_dtype) || same_type(a.fname, "out", out, out))
+    return -1;
+  PF_CHECK(numel(out) == d->m * d->n && (out->ndim == 0 || out->shape[out->ndim - 1] == d->n || d->m == 0), "%s: out must be [.., %lld]", a.fname,
+           (long long)d->n);
+  if (bias) {
+    if (same_type(a.fname, "bias", bias, out)) return -1;
+    PF_CHECK(numel(bias) == d->n, "%s: bias must be [n]", a.fname);
+    d->bias = data_of(bias);
+  }
+  if (res) {
+    if (same_type(a.fname, "residual", res, out)) return -1;
+    PF_CHECK(numel(res) == d->m * d->n, "%s: residual must have the shape of out", a.fname);
+    d->residual = data_of(res);
+  }
+  rb200_gemm_desc names;
+  if (parse_names(a.fname, act, bin, un, &names)) return -1;
+  d->activation = names.activation;
+  d->binary_op = names.binary_op;
+  d->unary_op = names.unary_op;
+  d->out = data_of(out);
+  d->ldo = d->n;
+  return 0;
+}
+// (a, a_scales, w, w_scales, format, a_tensor_scale|null, w_tensor_scale|null, bias|null, residual|null, activation, binary_op,
+//  unary_op, out)
+int pf_gemm_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, void*) {
+  const char* fname = "relax_b200.gemm_fp4";
+  Args a{v, tc, n_args, fname};
+  PF_CHECK(n_args == 13, "%s expects 13 arguments, got %d", fname, n_args);
+  const DLTensor *x, *xs, *w, *ws, *ats, *wts, *out;
+  Fp4Matrix qa, qw;
+  rb200_gemm_fp4_desc d;
+  memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  if (a.tensor(0, &x) || a.tensor(1, &xs) || a.tensor(2, &w) || a.tensor(3, &ws) || fp4_format(a, 4, &d.format) ||
+      a.tensor(5, &ats, true) || a.tensor(6, &wts, true) || a.tensor(12, &out) || fp4_matrix(fname, "a", 2, d.format, x, xs, ats, &qa) ||
+      fp4_matrix(fname, "w", 2, d.format, w, ws, wts, &qw))
+    return -1;
+  PF_CHECK(qa.k == qw.k, "%s: a has k=%lld, w k=%lld", fname, (long long)qa.k, (long long)qw.k);
+  d.m = qa.rows;
+  d.n = qw.rows;
+  d.k = qa.k;
+  if (fp4_epilogue(a, 7, out, &d)) return -1;
+  d.a = qa.codes;
+  d.a_scales = qa.scales;
+  d.a_tensor_scale = qa.ts;
+  d.w = qw.codes;
+  d.w_scales = qw.scales;
+  d.w_tensor_scale = qw.ts;
+  if (ret_tc) *ret_tc = RB200_ARG_NULL;
+  return rb200_gemm_fp4(&d, rb200_get_stream());
+}
+// (x, w, w_scales, format, x_tensor_scale|null, w_tensor_scale|null, bias|null, residual|null, activation, binary_op, unary_op,
+//  workspace, out)
+int pf_linear_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, void*) {
+  const char* fname = "relax_b200.linear_fp4";
+  Args a{v, tc, n_args, fname};
+  PF_CHECK(n_args == 13, "%s expects 13 arguments, got %d", fname, n_args);
+  const DLTensor *x, *w, *wsc, *xts, *wts, *ws, *out;
+  Fp4Matrix qw;
+  int type;
+  rb200_gemm_fp4_desc d;
+  memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  if (a.tensor(0, &x) || a.tensor(1, &w) || a.tensor(2, &wsc) || fp4_format(a, 3, &d.format) || a.tensor(4, &xts, true) ||
+      a.tensor(5, &wts, true) || a.tensor(11, &ws, true) || a.tensor(12, &out) || float_type(fname, "x", x, &type) ||
+      same_type(fname, "x", x, x) || fp4_matrix(fname, "w", 2, d.format, w, wsc, wts, &qw))
+    return -1;
+  PF_CHECK(x->ndim >= 1 && x->shape[x->ndim - 1] == qw.k, "%s: x inner extent != k=%lld", fname, (long long)qw.k);
+  d.m = lead_rows(x);
+  d.n = qw.rows;
+  d.k = qw.k;
+  if (fp4_epilogue(a, 6, out, &d)) return -1;
+  if (xts) {
+    if (check_tensor(fname, "x tensor scale", xts, kDLFloat, 32)) return -1;
+    PF_CHECK(numel(xts) == 1, "%s: x has one tensor scale", fname);
+    d.a_tensor_scale = static_cast<const float*>(data_of(xts));
+  }
+  if (ws && check_tensor(fname, "workspace", ws, kDLUInt, 8)) return -1;
+  d.w = qw.codes;
+  d.w_scales = qw.scales;
+  d.w_tensor_scale = qw.ts;
+  if (ret_tc) *ret_tc = RB200_ARG_NULL;
+  return rb200_linear_fp4(data_of(x), type, qw.k, &d, ws ? data_of(ws) : nullptr, ws ? (size_t)numel(ws) : 0, rb200_get_stream());
+}
+
 void register_builtin(const char* name, RB200PackedCFunc fn) {
   registry()[name] = new Entry{fn, nullptr, name};
 }
@@ -797,6 +999,11 @@ void ensure_builtins() {
   register_builtin("cutlass.group_gemm_fp16_sm90", pf_group_gemm_fp16);
   register_builtin("cutlass.moe_gemm", pf_moe_gemm);
   register_builtin("relax_b200.moe_gemm_q4f16", pf_moe_gemm_q4f16);
+  register_builtin("relax_b200.encode_fp4", pf_encode_fp4);
+  register_builtin("relax_b200.decode_fp4", pf_decode_fp4);
+  register_builtin("relax_b200.preprocess_fp4_scales", pf_preprocess_fp4_scales);
+  register_builtin("relax_b200.gemm_fp4", pf_gemm_fp4);
+  register_builtin("relax_b200.linear_fp4", pf_linear_fp4);
   register_builtin("runtime.get_cuda_stream", pf_get_stream);
   register_builtin("runtime.set_cuda_stream", pf_set_stream);
 }

@@ -19,6 +19,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -37,6 +38,7 @@ struct Lib {
   decltype(&rb200_moe_route_workspace_bytes) moe_route_workspace_bytes;
   decltype(&rb200_moe_gather) moe_gather;
   decltype(&rb200_moe_combine) moe_combine;
+  decltype(&rb200_linear_fp4_workspace_bytes) linear_fp4_workspace_bytes;
 } lib;
 PyObject* error_class = nullptr;
 
@@ -581,6 +583,164 @@ PyObject* encode_ft(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   GUARD_END
 }
 
+// ------------------------------------------------------------------ microscaled 4-bit floats
+// k of a block; 0 with a Python error set for another name than "mx" and "nv"
+int64_t fp4_block(PyObject* fmt) {
+  if (PyUnicode_Check(fmt)) {
+    if (PyUnicode_CompareWithASCIIString(fmt, "mx") == 0) return 32;
+    if (PyUnicode_CompareWithASCIIString(fmt, "nv") == 0) return 16;
+  }
+  PyErr_Format(PyExc_ValueError, "the 4-bit format must be 'mx' or 'nv', got %R", fmt);
+  return 0;
+}
+// [lead.., row tiles, k tiles, 512] for `blocks` blocks a row
+at::Tensor fp4_scales_for(const at::Tensor& like, c10::IntArrayRef lead, int64_t rows, int64_t blocks) {
+  c10::SmallVector<int64_t, 6> sizes(lead.begin(), lead.end());
+  sizes.push_back((rows + 127) / 128);
+  sizes.push_back((blocks + 3) / 4);
+  sizes.push_back(512);
+  return empty_on(sizes, c10::ScalarType::Byte, like);
+}
+// with rows the kernels can read: the tensor itself where it is compact and aligned, else a copy
+at::Tensor readable(const at::Tensor& t) {
+  if (!t.is_contiguous()) return t.contiguous();
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
+}
+PyObject* pair(at::Tensor a, at::Tensor b) {
+  PyObject* tup = PyTuple_New(2);
+  if (!tup) return nullptr;
+  PyTuple_SET_ITEM(tup, 0, THPVariable_Wrap(std::move(a)));
+  PyTuple_SET_ITEM(tup, 1, THPVariable_Wrap(std::move(b)));
+  return tup;
+}
+
+// encode_fp4(x, format, tensor_scale)
+PyObject* encode_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  GUARD_BEGIN
+  NEED_ARGS(3);
+  static Global fn("relax_b200.encode_fp4");
+  const at::Tensor* x = as_tensor(a[0], "x");
+  const int64_t block = x ? fp4_block(a[1]) : 0;
+  if (!block) return nullptr;
+  if (x->dim() != 2 && x->dim() != 3) return PyErr_SetString(PyExc_ValueError, "x must be [n, k] or [batch, n, k]"), nullptr;
+  const int64_t n = x->size(-2), k = x->size(-1);
+  if (k <= 0 || k % 32) return PyErr_Format(PyExc_ValueError, "4-bit floats need k %% 32 == 0, got k=%lld", (long long)k), nullptr;
+  const c10::IntArrayRef lead = x->sizes().slice(0, x->dim() - 2);
+  // rows of a wider matrix are read where they are
+  const int64_t width = x->element_size();
+  const bool rows = x->dim() == 2 && x->stride(1) == 1 && x->stride(0) >= k && x->stride(0) * width % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0;
+  const at::Tensor xr = rows ? *x : readable(*x);
+  c10::SmallVector<int64_t, 6> sizes(x->sizes().begin(), x->sizes().end());
+  sizes.back() = k / 2;
+  at::Tensor codes = empty_on(sizes, c10::ScalarType::Byte, *x), scales = fp4_scales_for(*x, lead, n, k / block);
+  Frame f;
+  if (!f.tensor(xr) || !f.object(a[1]) || !f.object(a[2]) || !f.tensor(codes) || !f.tensor(scales) || !f.call(fn.get())) return nullptr;
+  return pair(std::move(codes), std::move(scales));
+  GUARD_END
+}
+
+// preprocess_fp4_scales(scales)
+PyObject* preprocess_fp4_scales(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  GUARD_BEGIN
+  NEED_ARGS(1);
+  static Global fn("relax_b200.preprocess_fp4_scales");
+  const at::Tensor* s = as_tensor(a[0], "scales");
+  if (!s) return nullptr;
+  if (s->dim() != 2 && s->dim() != 3) return PyErr_SetString(PyExc_ValueError, "scales must be [n, blocks] or [batch, n, blocks]"), nullptr;
+  // (bytes by another name, as torch reads them from a checkpoint)
+  at::Tensor src = s->contiguous();
+  if (src.element_size() == 1 && src.scalar_type() != c10::ScalarType::Byte) src = src.view(c10::ScalarType::Byte);
+  at::Tensor out = fp4_scales_for(src, s->sizes().slice(0, s->dim() - 2), s->size(-2), s->size(-1));
+  Frame f;
+  if (!f.tensor(src) || !f.tensor(out) || !f.call(fn.get())) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  GUARD_END
+}
+
+bool as_float_type(PyObject* o, c10::ScalarType* out) {
+  if (!THPDtype_Check(o)) {
+    PyErr_Format(PyExc_TypeError, "dtype must be a torch.dtype, got %R", reinterpret_cast<PyObject*>(Py_TYPE(o)));
+    return false;
+  }
+  *out = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  return true;
+}
+
+// decode_fp4(codes, scales, format, tensor_scale, dtype)
+PyObject* decode_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  GUARD_BEGIN
+  NEED_ARGS(5);
+  static Global fn("relax_b200.decode_fp4");
+  const at::Tensor *c = as_tensor(a[0], "codes"), *s = c ? as_tensor(a[1], "scales") : nullptr;
+  c10::ScalarType type;
+  if (!s || !as_float_type(a[4], &type)) return nullptr;
+  if (c->dim() < 1) return PyErr_SetString(PyExc_IndexError, "codes need a dimension"), nullptr;
+  c10::SmallVector<int64_t, 6> sizes(c->sizes().begin(), c->sizes().end());
+  sizes.back() *= 2;
+  at::Tensor out = empty_on(sizes, type, *c);
+  Frame f;
+  if (!f.tensor(*c) || !f.tensor(*s) || !f.object(a[2]) || !f.object(a[3]) || !f.tensor(out) || !f.call(fn.get())) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  GUARD_END
+}
+
+// gemm_fp4(a, a_scales, w, w_scales, format, a_tensor_scale, w_tensor_scale, bias, residual, activation, binary_op, unary_op,
+//          dtype, out)
+PyObject* gemm_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  GUARD_BEGIN
+  NEED_ARGS(14);
+  static Global fn("relax_b200.gemm_fp4");
+  const at::Tensor *x = as_tensor(a[0], "a"), *w = x ? as_tensor(a[2], "w") : nullptr;
+  c10::ScalarType type;
+  Out out;
+  if (!w || !as_float_type(a[12], &type) || !out.take(a[13])) return nullptr;
+  if (x->dim() != 2 || w->dim() != 2) return PyErr_SetString(PyExc_ValueError, "a and w must be codes [rows, k / 2]"), nullptr;
+  if (!out.given) out.t = empty_on({x->size(0), w->size(0)}, type, *x);
+  Frame f;
+  for (int i = 0; i < 12; ++i)
+    if (!f.object(a[i])) return nullptr;
+  if (!f.tensor(out.t) || !f.call(fn.get())) return nullptr;
+  return out.give();
+  GUARD_END
+}
+
+// linear_fp4(x, w, w_scales, format, x_tensor_scale, w_tensor_scale, bias, residual, activation, binary_op, unary_op, workspace, out)
+PyObject* linear_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  GUARD_BEGIN
+  NEED_ARGS(13);
+  static Global fn("relax_b200.linear_fp4");
+  const at::Tensor *x = as_tensor(a[0], "x"), *w = x ? as_tensor(a[1], "w") : nullptr;
+  const int64_t block = w ? fp4_block(a[3]) : 0;
+  Out out;
+  if (!block || !out.take(a[12])) return nullptr;
+  if (x->dim() < 1 || w->dim() != 2) return PyErr_SetString(PyExc_ValueError, "x needs a dimension, w must be codes [n, k / 2]"), nullptr;
+  const int64_t k = x->size(-1);
+  if (!out.given) {
+    c10::SmallVector<int64_t, 6> sizes(x->sizes().begin(), x->sizes().end());
+    sizes.back() = w->size(0);
+    out.t = empty_on(sizes, x->scalar_type(), *x);
+  }
+  at::Tensor ws;
+  if (a[11] == Py_None) {
+    const int64_t m = k ? x->numel() / k : 0;
+    ws = empty_on({static_cast<int64_t>(lib.linear_fp4_workspace_bytes(m, k, block == 32 ? RB200_FP4_MX : RB200_FP4_NV))},
+                  c10::ScalarType::Byte, *x);
+  } else {
+    const at::Tensor* p = as_tensor(a[11], "workspace");
+    if (!p) return nullptr;
+    ws = *p;
+  }
+  const at::Tensor xr = readable(*x);
+  Frame f;
+  if (!f.tensor(xr) || !f.tensor(*w)) return nullptr;
+  for (int i = 2; i < 11; ++i)
+    if (!f.object(a[i])) return nullptr;
+  if (!f.tensor(ws) || !f.tensor(out.t) || !f.call(fn.get())) return nullptr;
+  return out.give();
+  GUARD_END
+}
+
 // init(error_class, {symbol: address})
 PyObject* init(PyObject*, PyObject* args) {
   PyObject *cls, *table;
@@ -603,6 +763,7 @@ PyObject* init(PyObject*, PyObject* args) {
   TAKE(moe_route_workspace_bytes, "rb200_moe_route_workspace_bytes")
   TAKE(moe_gather, "rb200_moe_gather")
   TAKE(moe_combine, "rb200_moe_combine")
+  TAKE(linear_fp4_workspace_bytes, "rb200_linear_fp4_workspace_bytes")
 #undef TAKE
   Py_RETURN_NONE;
 }
@@ -612,7 +773,7 @@ PyMethodDef methods[] = {
     {"init", init, METH_VARARGS, nullptr},
     FAST(call),      FAST(check),     FAST(call_like), FAST(gemm_ft),    FAST(gemm_q4),    FAST(gemm_gptq),   FAST(gather_columns),
     FAST(moe_ft),    FAST(moe_q4),    FAST(group_fp16), FAST(moe_route),  FAST(moe_gather),  FAST(moe_combine),
-    FAST(encode_ft), {nullptr, nullptr, 0, nullptr}};
+    FAST(encode_ft), FAST(encode_fp4), FAST(decode_fp4), FAST(preprocess_fp4_scales), FAST(gemm_fp4), FAST(linear_fp4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

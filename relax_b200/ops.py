@@ -169,3 +169,52 @@ def interleave_gate_up(t: torch.Tensor, n_axis: int = 0) -> torch.Tensor:
     out = torch.empty_like(t)
     get_global_func("relax_b200.interleave_gate_up")(t.contiguous(), int(n_axis), out)
     return out
+
+
+# ------------------------------------------------------------------ microscaled 4-bit floats
+
+def encode_fp4(x: torch.Tensor, fmt: str, tensor_scale: Optional[torch.Tensor] = None):
+    """Quantise to 4-bit floats (``rb200_encode_fp4``): ``x`` fp16, bf16 or fp32 [n, k] or [batch, n, k] with ``k % 32 == 0``
+    -> ``(codes uint8 [.., n, k/2], scales uint8 [.., ceil(n/128), tiles, 512])``.
+
+    ``fmt`` "mx": blocks of 32 along k, power-of-two scales.  "nv": blocks of 16, e4m3 scales, times ``tensor_scale``
+    (fp32 [1], or [batch]; 1 if not given), usually ``max |x| / (448 * 6)``.  The role of the reference tests' encode step
+    (tests/python/relax/test_codegen_cutlass.py:1391-1457)."""
+    return native.encode_fp4(x, fmt, tensor_scale)
+
+
+def decode_fp4(codes: torch.Tensor, scales: torch.Tensor, fmt: str, tensor_scale: Optional[torch.Tensor] = None,
+               dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The values that 4-bit codes and their scales stand for, rounded to ``dtype``."""
+    return native.decode_fp4(codes, scales, fmt, tensor_scale, dtype)
+
+
+def preprocess_fp4_scales(scales: torch.Tensor) -> torch.Tensor:
+    """A checkpoint's block scales (one byte each, [n, k/block] or [batch, n, k/block]) in the tiles that the products
+    read; the codes of a checkpoint (two a byte, the even k in the lower nibble) need no step of the kind."""
+    return native.preprocess_fp4_scales(scales)
+
+
+def gemm_fp4(a, a_scales, w, w_scales, fmt: str, a_tensor_scale=None, w_tensor_scale=None, bias=None, residual=None,
+             activation: str = "identity", binary_op: str = "", unary_op: str = "identity",
+             dtype: torch.dtype = torch.float16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(a @ w.T + bias)`` (optionally combined with a residual) of two operands in 4-bit floats, multiplied as they are
+    on the tensor cores: ``a`` codes [m, k/2], ``w`` codes [n, k/2], scales from :func:`encode_fp4` or
+    :func:`preprocess_fp4_scales`; fp32 sums, one rounding to ``dtype`` (bias and residual have it too)."""
+    return native.gemm_fp4(a, a_scales, w, w_scales, fmt, a_tensor_scale, w_tensor_scale, bias, residual, activation, binary_op,
+                           unary_op, dtype, out)
+
+
+def linear_fp4(x, w, w_scales, fmt: str, x_tensor_scale=None, w_tensor_scale=None, bias=None, residual=None,
+               activation: str = "identity", binary_op: str = "", unary_op: str = "identity",
+               workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A linear layer over a weight in 4-bit floats: ``x`` [.., k] is quantised as :func:`encode_fp4` does, then multiplied
+    as :func:`gemm_fp4` does; the result has ``x``'s type.  ``workspace`` (uint8, :func:`linear_fp4_workspace_bytes`) and
+    ``out`` make the call allocation-free."""
+    return native.linear_fp4(x, w, w_scales, fmt, x_tensor_scale, w_tensor_scale, bias, residual, activation, binary_op, unary_op,
+                             workspace, out)
+
+
+def linear_fp4_workspace_bytes(m: int, k: int, fmt: str) -> int:
+    from . import _lib
+    return int(_lib.load().rb200_linear_fp4_workspace_bytes(m, k, {"mx": 0, "nv": 1}[fmt]))
