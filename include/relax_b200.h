@@ -384,6 +384,39 @@ RB200_API size_t rb200_linear_fp4_workspace_bytes(int64_t m, int64_t k, int form
 RB200_API int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb200_gemm_fp4_desc* desc, void* workspace,
                                size_t workspace_bytes, void* stream);
 
+/*
+ * A whole expert layer for at most 32 tokens, in two kernels, over expert weights in 4-bit floats; x and the products in
+ * between keep 16 bits:
+ *   p = softmax(logits[t]); the top_k experts of largest logits (equal ones: lower index first; distinct);
+ *   gate_j = p_j, or p_j / (sum of the chosen p) with renormalize;
+ *   out[t] = sum_j gate_j (silu(x[t] Wg_j^T) * (x[t] Wu_j^T)) Wd_j^T,  fp32 sums, the factor in brackets rounded to fp16.
+ * A NaN among a token's logits, or a maximum that is infinite, makes its gates NaN, as in rb200_moe_route.
+ * x and out fp16 [tokens, hidden], logits fp32 [tokens, num_experts]; w_gate_up codes [num_experts, 2 ffn, hidden / 2], gate
+ * rows first; w_down codes [num_experts, hidden, ffn / 2]; scales of each expert in tiles, experts after one another;
+ * tensor scales [num_experts] (nv only; NULL: 1).  hidden and ffn multiples of 64, num_experts <= 256, top_k <= 8.
+ * workspace: rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, ffn) bytes, of the call's own until it has run.
+ * The weights, scales and logits must not be written between this call and its end.
+ * Takes the place of rb200_moe_route, rb200_moe_gather, two grouped matmuls and rb200_moe_combine.
+ */
+typedef struct rb200_moe_layer_fp4_desc {
+  uint32_t struct_size; /* sizeof(rb200_moe_layer_fp4_desc) */
+  int32_t format;       /* RB200_FP4_* */
+  const void* x;
+  const float* logits;
+  const void* w_gate_up;
+  const void* gate_up_scales;
+  const float* gate_up_tensor_scale;
+  const void* w_down;
+  const void* down_scales;
+  const float* down_tensor_scale;
+  void* out;
+  int64_t tokens, num_experts, top_k, hidden, ffn;
+  int32_t renormalize;
+  int32_t reserved;
+} rb200_moe_layer_fp4_desc;
+RB200_API size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t ffn);
+RB200_API int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ low-latency all-reduce */
 
 /*

@@ -138,6 +138,9 @@ RB200_API int RB200FuncListGlobalNames(int* out_size, const char*** out_array);
  *       residual|null, activation:str, binary_op:str, unary_op:str, out f16|bf16|f32 [m, n])
  *  "relax_b200.linear_fp4"(x f16|bf16|f32 [.., k], w, w_scales, format:str, x_tensor_scale|null, w_tensor_scale|null, bias|null,
  *       residual|null, activation:str, binary_op:str, unary_op:str, workspace u8, out [.., n])
+ *  "relax_b200.moe_layer_fp4"(x f16 [t, hidden], logits f32 [t, E], w_gate_up u8 [E, 2 ffn, hidden/2], gate_up_scales,
+ *       w_down u8 [E, hidden, ffn/2], down_scales, top_k:int, format:str, gate_up_tensor_scale f32 [E]|null,
+ *       down_tensor_scale f32 [E]|null, renormalize:int, workspace u8, out f16 [t, hidden])   at most 32 tokens
  *  "runtime.get_cuda_stream"() -> handle          src/runtime/cuda/cuda_device_api.cc:318-320
  *  "runtime.set_cuda_stream"(handle)
  */

@@ -13,7 +13,7 @@ from . import _lib, build
 _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_torch_host.so")
 _SYMBOLS = ("rb200_last_error", "rb200_set_stream", "RB200FuncCall", "RB200FuncGetGlobal", "rb200_encode_ft",
             "rb200_moe_route", "rb200_moe_route_workspace_bytes", "rb200_moe_gather", "rb200_moe_combine",
-            "rb200_linear_fp4_workspace_bytes")
+            "rb200_linear_fp4_workspace_bytes", "rb200_moe_layer_fp4_workspace_bytes")
 
 
 def check_abi(built_for, here):

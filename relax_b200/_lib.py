@@ -62,6 +62,21 @@ class GemmFp4Desc(ctypes.Structure):
     ]
 
 
+class MoeLayerFp4Desc(ctypes.Structure):
+    """``rb200_moe_layer_fp4_desc`` of include/relax_b200.h."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("format", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("logits", ctypes.c_void_p),
+        ("w_gate_up", ctypes.c_void_p), ("gate_up_scales", ctypes.c_void_p), ("gate_up_tensor_scale", ctypes.c_void_p),
+        ("w_down", ctypes.c_void_p), ("down_scales", ctypes.c_void_p), ("down_tensor_scale", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("num_experts", ctypes.c_int64), ("top_k", ctypes.c_int64),
+        ("hidden", ctypes.c_int64), ("ffn", ctypes.c_int64),
+        ("renormalize", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
 class DLDevice(ctypes.Structure):
     _fields_ = [("device_type", ctypes.c_int32), ("device_id", ctypes.c_int32)]
 
@@ -130,6 +145,8 @@ SIGNATURES = {
     "rb200_gemm_fp4": (_I, [ctypes.POINTER(GemmFp4Desc), _V]),
     "rb200_linear_fp4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I]),
     "rb200_linear_fp4": (_I, [_V, _I, _I64, ctypes.POINTER(GemmFp4Desc), _V, ctypes.c_size_t, _V]),
+    "rb200_moe_layer_fp4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "rb200_moe_layer_fp4": (_I, [ctypes.POINTER(MoeLayerFp4Desc), _V, ctypes.c_size_t, _V]),
     "rb200_allreduce_workspace_bytes": (ctypes.c_size_t, [_I64]),
     "rb200_allreduce_oneshot": (_I, [ctypes.POINTER(_V), _I, _I, _V, _V, _I64, _I64, _V]),
     "rb200_allreduce_oneshot_selftest": (_I, [ctypes.POINTER(_V), ctypes.POINTER(_V), ctypes.POINTER(_V), _I,

@@ -59,8 +59,9 @@ int fill_now(void* p, int byte, size_t bytes);
 int noalloc_read_status(int* status_out);
 // The same for the quantiser's waits.
 int encode_read_status(int* status_out);
-// And for the 4-bit float products.
+// And for the 4-bit float products and expert layers.
 int fp4_gemm_read_status(int* status_out);
+int fp4_moe_read_status(int* status_out);
 // Upper bound, in milliseconds, of the waits on flags written by other CTAs or other GPUs
 // (split-k fix-up, all-reduce); 0 = the default of about two seconds.  See rb200_set_wait_limit_ms.
 unsigned wait_limit_ms();

@@ -1,0 +1,740 @@
+// A whole expert layer for a few tokens over weights in microscaled 4-bit floats, in two kernels:
+//   up    routing; h[r] = silu(x Wg^T) * (x Wu^T) for the (token, expert) pairs r, ordered by expert
+//   down  out[t] = sum over the token's experts of gate * (h[r] Wd^T)
+//
+// What bounds it is reading the weights of the chosen experts once, so activations keep their 16 bits: codes become fp16
+// pairs in registers (one conversion per pair, exact) and go through mma.sync with up to eight rows as its columns, which
+// at these batch sizes costs less than the reading.  kMx scales multiply the fp32 sums of a block; kNv scales have too few
+// k for that and multiply the fp16 pairs, exactly (two and four significant bits, at least 2^-10, at most 2688).
+//
+// Routing is a few hundred clocks for a few tokens, so every CTA does it for itself from the logits: no kernel before these
+// two, no hand-over through memory.  `down` does it, and asks for its first weights, while `up` still runs.
+//
+// Weights come by tensor-map loads in 128-byte rows, swizzled; a lane's code words are then free of bank conflicts.  A
+// warp's lane (g, t) holds, of the 32 k of a chunk, k 8t .. 8t + 7 of rows g and g + 8: the MMAs' k slots are a permutation
+// of k, the same one for x, whose eight values are one 16-byte word.
+// `down` cuts the (expert, k) sequence of 64 output columns over the CTAs of a cluster; each adds gate times its sums in
+// shared memory, every word by one thread in the order of the sequence, and the cluster's parts are added in rank order:
+// nothing depends on timing.
+#include <atomic>
+#include <cstring>
+
+#include "../../include/relax_b200.h"
+#include "fp4_mma.cuh"
+#include "tensormap.h"
+
+namespace rb200 {
+namespace f4 {
+namespace {
+
+constexpr int kMaxTokens = 32, kMaxExperts = 256, kMaxTopK = 8, kMaxRows = kMaxTokens * kMaxTopK;
+constexpr int kConsumers = 8;  // warps: four blocks of 16 rows, two halves of k
+constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kTile = 64;      // rows of a weight box
+constexpr int kBox = kTile * 128;
+constexpr int kMaxStages = 6;
+
+__device__ int g_status;
+
+struct alignas(16) Routing {
+  uint32_t mask[kMaxExperts];       // tokens of an expert
+  int active[kMaxRows];             // experts with tokens, in order
+  int row_begin[kMaxRows + 1];      // their rows
+  uint8_t token_of_row[kMaxRows];
+  float gate_of_row[kMaxRows];
+  int expert_of[kMaxRows];          // by token and choice
+  float gate_of[kMaxRows];
+  int warp_sum[2][kConsumers];
+  int experts;                      // number of active ones
+  int failed;
+};
+
+struct Params {
+  const __half* x;
+  const float* logits;
+  const uint8_t* s1;
+  const uint8_t* s2;
+  const float* ts1;
+  const float* ts2;
+  __half* h;
+  __half* out;
+  int64_t s1_expert, s2_expert;  // bytes of an expert's scales
+  int tokens, experts, top_k, renormalize;
+  int hidden, ffn, k_tiles1, k_tiles2;
+  int stages, cluster;
+};
+
+// order of floats as unsigned numbers, NaN lowest
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return v == v ? ((b & 0x80000000u) ? ~b : b | 0x80000000u) : 0u;
+}
+
+// The routing by the eight consumer warps (256 threads; every thread of the CTA calls it).  The top_k largest logits of
+// a token (equal ones: lower expert first), gates softmax over all experts, or over the chosen ones.
+__device__ void route(const Params& p, Routing& r) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid < kMaxExperts) r.mask[tid] = 0u;
+  __syncthreads();
+  if (warp < kConsumers)
+    for (int t = warp; t < p.tokens; t += kConsumers) {
+      constexpr int kPer = kMaxExperts / 32;
+      const int per = (p.experts + 31) / 32;
+      float v[kPer];
+      uint32_t key[kPer];
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int e = i * 32 + lane;
+        v[i] = i < per && e < p.experts ? __ldcg(p.logits + t * p.experts + e) : -INFINITY;
+        top = fmaxf(top, v[i]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int e = i * 32 + lane;
+        const bool there = i < per && e < p.experts;
+        if (there) sum += expf(v[i] - top);
+        key[i] = there ? max(order_key(v[i]), 1u) : 0u;  // 0: not there, or taken
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      float chosen = 0.0f, mine = 0.0f;
+      int my_expert = 0;
+      for (int j = 0; j < p.top_k; ++j) {
+        uint32_t best = 0u;
+        int at = 0;
+        float val = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (key[i] > best) {
+            best = key[i];
+            at = i;
+            val = v[i];
+          }
+        const uint32_t all = __reduce_max_sync(0xffffffffu, best);
+        const int e = (int)__reduce_min_sync(0xffffffffu, best == all ? (uint32_t)(at * 32 + lane) : 0xffffu);
+        const float l = __shfl_sync(0xffffffffu, val, e & 31), w = expf(l - top);
+        chosen += w;
+        if (lane == j) {
+          mine = w;
+          my_expert = e;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (i * 32 + lane == e) key[i] = 0u;
+      }
+      // (a NaN among the logits, or nothing but -inf: sum is NaN, and so is every gate)
+      if (lane < p.top_k) {
+        r.expert_of[t * p.top_k + lane] = my_expert;
+        r.gate_of[t * p.top_k + lane] = p.renormalize && sum == sum ? mine / chosen : mine / sum;
+        atomicOr(&r.mask[my_expert], 1u << t);
+      }
+    }
+  __syncthreads();
+  // experts with tokens and their rows, in expert order
+  const uint32_t m = tid < kMaxExperts ? r.mask[tid] : 0u;
+  const int n = __popc(m);
+  const uint32_t ballot = __ballot_sync(0xffffffffu, n > 0);
+  int upto = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (warp < kConsumers && lane == 31) {
+    r.warp_sum[0][warp] = upto;
+    r.warp_sum[1][warp] = __popc(ballot);
+  }
+  __syncthreads();
+  if (warp < kConsumers) {
+    int row = upto - n, a = __popc(ballot & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) {
+      row += r.warp_sum[0][w];
+      a += r.warp_sum[1][w];
+    }
+    if (n > 0) {
+      r.active[a] = tid;
+      r.row_begin[a] = row;
+      uint32_t left = m;
+      for (int i = 0; i < n; ++i, left &= left - 1u) {
+        const int t = __ffs((int)left) - 1;
+        float gate = 0.0f;
+        for (int j = 0; j < p.top_k; ++j)
+          if (r.expert_of[t * p.top_k + j] == tid) gate = r.gate_of[t * p.top_k + j];
+        r.token_of_row[row + i] = (uint8_t)t;
+        r.gate_of_row[row + i] = gate;
+      }
+    }
+    if (tid == kMaxExperts - 1) {
+      r.experts = a + (n > 0);
+      r.row_begin[a + (n > 0)] = row + n;
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// arrives at the barrier when this thread's copies so far have landed (the barrier counts these arrivals)
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Rows g and g + 8 of a 16-row block over the 32 k of a chunk: sums of the products with the x words of NT column tiles.
+// w0, w8: code words.  kMx: f0, f8 scales of the block; kNv: p0, p8 this lane's scales as f16x2.
+template <int FMT, int NT>
+__device__ __forceinline__ void chunk(float (&acc)[NT][4], uint32_t w0, uint32_t w8, float f0, float f8, uint32_t p0, uint32_t p8,
+                                      const uint4 (&x)[NT], int tiles) {
+  uint32_t a0[4], a8[4];
+  from_codes8(w0, a0);
+  from_codes8(w8, a8);
+  if (FMT == kNv) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a0[i] = mul2(a0[i], p0);
+      a8[i] = mul2(a8[i], p8);
+    }
+  }
+  const uint32_t lo[4] = {a0[0], a8[0], a0[1], a8[1]}, hi[4] = {a0[2], a8[2], a0[3], a8[3]};
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    if (j > 0 && j >= tiles) break;
+    if (FMT == kNv) {
+      mma(acc[j], lo, x[j].x, x[j].y);
+      mma(acc[j], hi, x[j].z, x[j].w);
+    } else {
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      mma(part, lo, x[j].x, x[j].y);
+      mma(part, hi, x[j].z, x[j].w);
+      acc[j][0] = fmaf(part[0], f0, acc[j][0]);
+      acc[j][1] = fmaf(part[1], f0, acc[j][1]);
+      acc[j][2] = fmaf(part[2], f8, acc[j][2]);
+      acc[j][3] = fmaf(part[3], f8, acc[j][3]);
+    }
+  }
+}
+
+// Four chunks (128 k) of 16 rows: `codes` a box of 128-byte rows, swizzled, c0 its first 16-byte column; `words` the scale
+// tiles (one of kMx, two of kNv) at this lane's row g, `words8` at row g + 8.
+template <int FMT, int NT>
+struct Quarter {
+  const uint8_t* row0;
+  const uint8_t* words0;
+  const uint8_t* words8;
+  uint32_t s0, s8;
+  int g, t;
+  __device__ __forceinline__ void scales(int i) {
+    if (FMT == kMx ? i == 0 : (i & 1) == 0) {
+      const int at = FMT == kMx ? 0 : (i >> 1) * 512;
+      s0 = *reinterpret_cast<const uint32_t*>(words0 + at);
+      s8 = *reinterpret_cast<const uint32_t*>(words8 + at);
+    }
+  }
+  __device__ __forceinline__ void step(int i, int column, float (&acc)[NT][4], const uint4 (&x)[NT], int tiles) {
+    scales(i);
+    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(row0 + ((column ^ g) << 4) + t * 4);
+    const uint32_t w8 = *reinterpret_cast<const uint32_t*>(row0 + 8 * 128 + ((column ^ g) << 4) + t * 4);
+    if (FMT == kMx) {
+      chunk<FMT, NT>(acc, w0, w8, e8m0_value((s0 >> (8 * i)) & 0xffu), e8m0_value((s8 >> (8 * i)) & 0xffu), 0u, 0u, x, tiles);
+    } else {
+      const int sh = 16 * (i & 1) + 8 * (t >> 1);
+      const uint32_t two = from_e4m3x2(((s0 >> sh) & 0x7fu) | ((s8 >> sh) & 0x7fu) << 8);
+      chunk<FMT, NT>(acc, w0, w8, 0.0f, 0.0f, __byte_perm(two, 0u, 0x1010), __byte_perm(two, 0u, 0x3232), x, tiles);
+    }
+  }
+};
+
+// shared memory: [codes of all stages][scales][x][barriers][routing ..]
+struct Layout {
+  int code_bytes, scale_bytes, x_bytes;  // of a stage
+};
+template <int FMT, int NT>
+__host__ __device__ constexpr Layout layout_up() {
+  return {2 * kBox, 2 * stage_tiles(FMT) * 512, NT * 8 * kStageK * 2};
+}
+template <int FMT, int NT>
+__host__ __device__ constexpr Layout layout_down() {
+  return {2 * kBox, 2 * stage_tiles(FMT) * 512, NT * 8 * 2 * kStageK * 2};
+}
+
+// One kernel's ring of stages.
+struct Ring {
+  uint8_t* codes;
+  uint8_t* scales;
+  uint8_t* x;
+  uint64_t* full;
+  uint64_t* empty;
+  int stages, s;
+  uint32_t ph;
+  __device__ __forceinline__ void next() {
+    if (++s == stages) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+};
+__device__ __forceinline__ Ring make_ring(uint8_t* smem, const Layout& l, int stages) {
+  Ring r;
+  r.codes = smem;
+  r.scales = r.codes + stages * l.code_bytes;
+  r.x = r.scales + stages * l.scale_bytes;
+  r.full = reinterpret_cast<uint64_t*>(r.x + stages * l.x_bytes);
+  r.empty = r.full + kMaxStages;
+  r.stages = stages;
+  r.s = 0;
+  r.ph = 0u;
+  return r;
+}
+__device__ __forceinline__ void init_ring(const Ring& r) {
+  for (int i = 0; i < r.stages; ++i) {
+    mbar_init(&r.full[i], 1 + 32);       // the loads' bytes, a lane's copies of x each
+    mbar_init(&r.empty[i], kConsumers);
+  }
+  mbar_fence_init();
+}
+// No load may be on its way when the CTA leaves: the last fill of every stage.
+__device__ __forceinline__ bool drain_ring(const Ring& r, int issued) {
+  bool ok = true;
+  for (int i = max(0, issued - r.stages); i < issued; ++i)
+    ok = mbar_wait_parked(&r.full[i % r.stages], (uint32_t)(i / r.stages) & 1u, &g_status) && ok;
+  return ok;
+}
+// 16-byte column of x in its row's 512 bytes, so that a quarter-warp's reads (two rows, four columns) meet no bank twice
+__device__ __forceinline__ int x_column(int row, int column) { return column ^ ((row & 1) << 2); }
+
+constexpr int kRoutingOffset = 2 * kMaxStages * 8;
+
+template <int FMT, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+    moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
+  constexpr Layout L = layout_up<FMT, NT>();
+  constexpr int TILES = stage_tiles(FMT);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  Ring ring = make_ring(smem, L, p.stages);
+  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(ring.full) + kRoutingOffset);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    init_ring(ring);
+    r.failed = 0;
+  }
+  fence_proxy_async();
+  griddep_wait();
+  griddep_launch_dependents();
+  route(p, r);
+
+  const int f_tiles = p.ffn / kTile, items = r.experts * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
+  if (warp == kConsumers) {
+    // ============================================================ loads
+    int issued = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.active[a];
+      const int row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0;
+      const uint8_t* s_gate = p.s1 + e * p.s1_expert + (int64_t)(f0 >> 7) * p.k_tiles1 * 512;
+      const uint8_t* s_up = p.s1 + e * p.s1_expert + (int64_t)((p.ffn + f0) >> 7) * p.k_tiles1 * 512;
+      for (int c = 0; c < chunks; ++c) {
+        ok = mbar_wait_parked(&ring.empty[ring.s], ring.ph ^ 1u, &g_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint64_t* bar = &ring.full[ring.s];
+        if (lane == 0) {
+          const uint32_t tiles = (uint32_t)min(TILES, p.k_tiles1 - c * TILES) * 512u;
+          uint8_t* w = ring.codes + ring.s * L.code_bytes;
+          uint8_t* sc = ring.scales + ring.s * L.scale_bytes;
+          mbar_arrive_expect_tx(bar, 2 * kBox + 2 * tiles);
+          tma_load(w, &tmap_w, c * 128, e * 2 * p.ffn + f0, bar);
+          tma_load(w + kBox, &tmap_w, c * 128, e * 2 * p.ffn + p.ffn + f0, bar);
+          bulk_g2s(sc, s_gate + c * TILES * 512, tiles, bar);
+          bulk_g2s(sc + TILES * 512, s_up + c * TILES * 512, tiles, bar);
+        }
+        __syncwarp();
+        if (c * kStageK + lane * 8 < p.hidden)
+          for (int i = 0; i < rows; ++i)
+            cp_async16(ring.x + ring.s * L.x_bytes + i * (kStageK * 2) + x_column(i, lane) * 16,
+                       p.x + (int64_t)r.token_of_row[row0 + i] * p.hidden + c * kStageK + lane * 8);
+        cp_async_arrive(bar);
+        ++issued;
+        ring.next();
+      }
+    }
+    drain_ring(ring, issued);
+  } else {
+    // ============================================================ products
+    const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
+    float* red = reinterpret_cast<float*>(&r + 1);  // [fb][value][lane]
+    bool ok = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.active[a];
+      const int row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0, tiles = (rows + 7) / 8;
+      float gate[NT][4], up[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gate[j][i] = up[j][i] = 0.0f;
+      const int rg = (f0 & 127) + fb * 16 + g, ru = ((p.ffn + f0) & 127) + fb * 16 + g;  // rows in their scale tiles
+      for (int c = 0; c < chunks; ++c) {
+        if (ok) ok = mbar_wait_parked(&ring.full[ring.s], ring.ph, &g_status);
+        const uint8_t* w = ring.codes + ring.s * L.code_bytes + (fb * 16 + g) * 128;
+        const uint8_t* sc = ring.scales + ring.s * L.scale_bytes + kh * (TILES / 2) * 512;
+        Quarter<FMT, NT> qg = {w, sc + scale_word(rg, 0, 1), sc + scale_word(rg + 8, 0, 1), 0u, 0u, g, t};
+        Quarter<FMT, NT> qu = {w + kBox, sc + TILES * 512 + scale_word(ru, 0, 1), sc + TILES * 512 + scale_word(ru + 8, 0, 1), 0u, 0u, g, t};
+        const int left = (p.hidden - c * kStageK - kh * 128) / 32;  // chunks of 32 k there are
+        const uint8_t* xs = ring.x + ring.s * L.x_bytes + g * (kStageK * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i >= left) break;
+          const int column = kh * 4 + i;
+          uint4 x[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const uint4*>(xs + j * 8 * (kStageK * 2) + x_column(g, column * 4 + t) * 16);
+          qg.step(i, column, gate, x, tiles);
+          qu.step(i, column, up, x, tiles);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+        ring.next();
+      }
+      // the halves of k meet; rows g, g + 8 of columns 2t, 2t + 1
+      if (!ok) r.failed = 1;
+      if (kh == 1) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            red[((fb * NT + j) * 8 + i) * 32 + lane] = gate[j][i];
+            red[((fb * NT + j) * 8 + 4 + i) * 32 + lane] = up[j][i];
+          }
+      }
+      consumers_sync();
+      if (kh == 0 && r.failed == 0) {
+        const float ts = p.ts1 ? p.ts1[e] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float gv = (gate[j][i] + red[((fb * NT + j) * 8 + i) * 32 + lane]) * ts;
+            const float uv = (up[j][i] + red[((fb * NT + j) * 8 + 4 + i) * 32 + lane]) * ts;
+            const int row = j * 8 + 2 * t + (i & 1), f = f0 + fb * 16 + g + (i >> 1) * 8;
+            // (h is rounded to fp16: it is the next product's operand, 2^-11 of itself at most, the error of its sum is
+            // below that of the output's own rounding)
+            if (row < rows) p.h[(int64_t)(row0 + row) * p.ffn + f] = __float2half_rn(gv / (1.0f + __expf(-gv)) * uv);
+          }
+      }
+      consumers_sync();
+    }
+  }
+}
+
+template <int FMT, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+    moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
+  constexpr Layout L = layout_down<FMT, NT>();
+  constexpr int TILES = stage_tiles(FMT), kUnitK = 2 * kStageK;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  Ring ring = make_ring(smem, L, p.stages);
+  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(ring.full) + kRoutingOffset);
+  float* sums = reinterpret_cast<float*>(&r + 1);  // [half of k][token][64 columns]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.cluster) * kTile;
+  if (tid == 0) {
+    init_ring(ring);
+    r.failed = 0;
+  }
+  for (int i = tid; i < 2 * p.tokens * kTile; i += kThreads) sums[i] = 0.0f;
+  fence_proxy_async();
+  // The logits and the weights are older than the kernel before this one, which let this one start only after its own wait
+  // (the logits are read past L1, which may hold what was there before them).
+  route(p, r);
+
+  const int per = (p.ffn + kUnitK - 1) / kUnitK, units = r.experts * per;
+  const int u0 = (int)((int64_t)units * rank / p.cluster), u1 = (int)((int64_t)units * (rank + 1) / p.cluster);
+  if (warp == kConsumers) {
+    // ============================================================ loads
+    int issued = 0;
+    bool ok = true;
+    auto load_w = [&](int u, int s) {
+      const int a = u / per, c = u - a * per, e = r.active[a];
+      const uint32_t tiles = (uint32_t)min(2 * TILES, p.k_tiles2 - c * 2 * TILES) * 512u;
+      uint8_t* w = ring.codes + s * L.code_bytes;
+      const bool two = c * kUnitK + kStageK < p.ffn;
+      mbar_arrive_expect_tx(&ring.full[s], (two ? 2 * kBox : kBox) + tiles);
+      tma_load(w, &tmap_w, c * 256, e * p.hidden + n0, &ring.full[s]);
+      if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + n0, &ring.full[s]);
+      bulk_g2s(ring.scales + s * L.scale_bytes, p.s2 + e * p.s2_expert + ((int64_t)(n0 >> 7) * p.k_tiles2 + c * 2 * TILES) * 512, tiles,
+               &ring.full[s]);
+    };
+    const int first = min(p.stages, u1 - u0);
+    if (lane == 0)
+      for (int s = 0; s < first; ++s) load_w(u0 + s, s);
+    griddep_wait();  // h is the kernel before's
+    for (int u = u0; u < u1; ++u) {
+      if (u - u0 >= first) {
+        ok = mbar_wait_parked(&ring.empty[ring.s], ring.ph ^ 1u, &g_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) load_w(u, ring.s);
+      }
+      __syncwarp();
+      const int a = u / per, c = u - a * per, row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0;
+      for (int i = 0; i < rows; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int k = c * kUnitK + half * kStageK + lane * 8;
+          if (k < p.ffn)
+            cp_async16(ring.x + ring.s * L.x_bytes + (half * NT * 8 + i) * (kStageK * 2) + x_column(i, lane) * 16,
+                       p.h + (int64_t)(row0 + i) * p.ffn + k);
+        }
+      cp_async_arrive(&ring.full[ring.s]);
+      ++issued;
+      ring.next();
+    }
+    drain_ring(ring, issued);
+  } else {
+    // ============================================================ products
+    const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
+    bool ok = true;
+    float acc[NT][4];
+    const int rn = (n0 & 127) + fb * 16 + g;
+    for (int u = u0; u < u1; ++u) {
+      const int a = u / per, c = u - a * per;
+      const int row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0, tiles = (rows + 7) / 8;
+      if (u == u0 || c == 0) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+      }
+      if (ok) ok = mbar_wait_parked(&ring.full[ring.s], ring.ph, &g_status);
+      const uint8_t* w = ring.codes + ring.s * L.code_bytes + kh * kBox + (fb * 16 + g) * 128;
+      const uint8_t* xs = ring.x + ring.s * L.x_bytes + (kh * NT * 8 + g) * (kStageK * 2);
+      const int left = (p.ffn - c * kUnitK - kh * kStageK) / 32;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint8_t* sc = ring.scales + ring.s * L.scale_bytes + (kh * TILES + q * (TILES / 2)) * 512;
+        Quarter<FMT, NT> qd = {w, sc + scale_word(rn, 0, 1), sc + scale_word(rn + 8, 0, 1), 0u, 0u, g, t};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int column = q * 4 + i;
+          if (column >= left) break;
+          uint4 x[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const uint4*>(xs + j * 8 * (kStageK * 2) + x_column(g, column * 4 + t) * 16);
+          qd.step(i, column, acc, x, tiles);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+      ring.next();
+      if (u + 1 == u1 || c + 1 == per) {
+        // this expert's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane)
+        const float ts = p.ts2 ? p.ts2[r.active[a]] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = j * 8 + 2 * t + (i & 1);
+            if (row < rows) {
+              float* at = sums + ((kh * p.tokens + r.token_of_row[row0 + row]) * kTile + fb * 16 + g + (i >> 1) * 8);
+              *at = fmaf(r.gate_of_row[row0 + row] * ts, acc[j][i], *at);
+            }
+          }
+        __syncwarp();
+      }
+    }
+    if (!ok)
+      for (int q = 0; q < p.cluster; ++q) st_cluster(at_rank(smem_u32(&r.failed), q), 1u);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  __syncthreads();
+  cluster_sync();
+  if (r.failed == 0) {
+    // four columns of a token a thread
+    const int quads = p.tokens * (kTile / 4);
+    for (int i = rank * kThreads + tid; i < quads; i += p.cluster * kThreads) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int q = 0; q < p.cluster; ++q)
+        for (int half = 0; half < 2; ++half) {
+          const float4 o = ld_cluster4(at_rank(smem_u32(sums + half * p.tokens * kTile + i * 4), q));
+          v.x += o.x;
+          v.y += o.y;
+          v.z += o.z;
+          v.w += o.w;
+        }
+      const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+      const int token = i / (kTile / 4), n = n0 + (i % (kTile / 4)) * 4;
+      *reinterpret_cast<uint2*>(p.out + (int64_t)token * p.hidden + n) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+  }
+  cluster_sync();  // others may still be reading this CTA's sums
+}
+
+constexpr int kMaxDevices = 64;
+std::atomic<bool> g_launched[kMaxDevices];  // devices whose status word a wait may have set
+
+size_t smem_bytes(const Layout& l, int stages, size_t extra) {
+  return 1024 + (size_t)stages * (l.code_bytes + l.scale_bytes + l.x_bytes) + kRoutingOffset + sizeof(Routing) + extra;
+}
+
+template <int FMT, int NT>
+int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t stream) {
+  auto up = moe_fp4_up_kernel<FMT, NT>;
+  auto down = moe_fp4_down_kernel<FMT, NT>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    RB200_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    RB200_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    configured_device = dev;
+  }
+  const int sms = sm_count_current(), ctas = NT == 1 ? 2 : 1;  // of an SM
+  const size_t room = (size_t)(NT == 1 ? 113 : 226) * 1024;
+  const int rows = p.tokens * p.top_k, most = rows < p.experts ? rows : p.experts;  // experts that can have tokens
+
+  const size_t red = (size_t)4 * NT * 8 * 32 * 4;
+  p.stages = kMaxStages;
+  while (p.stages > 2 && smem_bytes(layout_up<FMT, NT>(), p.stages, red) > room) --p.stages;
+  const int64_t items = (int64_t)most * (p.ffn / kTile);
+  RB200_CUDA(launch_dependent(up, dim3((unsigned)(items < ctas * sms ? items : ctas * sms)), kThreads,
+                              smem_bytes(layout_up<FMT, NT>(), p.stages, red), stream, p, t1));
+
+  const size_t sums = (size_t)2 * p.tokens * kTile * 4;
+  p.stages = kMaxStages;
+  while (p.stages > 2 && smem_bytes(layout_down<FMT, NT>(), p.stages, sums) > room) --p.stages;
+  const int n_tiles = p.hidden / kTile, per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK);
+  p.cluster = ctas * sms / n_tiles;
+  if (p.cluster > 8) p.cluster = 8;
+  if (p.cluster > per) p.cluster = per;
+  if (p.cluster < 1) p.cluster = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_tiles * p.cluster), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes(layout_down<FMT, NT>(), p.stages, sums);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  RB200_CUDA(cudaLaunchKernelEx(&cfg, down, p, t2));
+  return 0;
+}
+
+template <int FMT>
+int launch_fmt(const Params& p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t stream) {
+  // an expert may have every token
+  if (p.tokens <= 8) return launch<FMT, 1>(p, t1, t2, stream);
+  if (p.tokens <= 16) return launch<FMT, 2>(p, t1, t2, stream);
+  return launch<FMT, 4>(p, t1, t2, stream);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+}  // namespace f4
+
+int fp4_moe_read_status(int* status_out) {
+  *status_out = 0;
+  int dev = -1;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= f4::kMaxDevices || !f4::g_launched[dev].load(std::memory_order_relaxed)) return 0;
+  int v = 0;
+  RB200_CUDA(cudaMemcpyFromSymbol(&v, f4::g_status, sizeof(int)));
+  if (v != 0) {
+    const int zero = 0;
+    RB200_CUDA(cudaMemcpyToSymbol(f4::g_status, &zero, sizeof(int)));
+  }
+  *status_out = v;
+  return 0;
+}
+
+}  // namespace rb200
+
+using namespace rb200;
+
+extern "C" {
+
+size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t ffn) {
+  return tokens > 0 && top_k > 0 && ffn > 0 ? (size_t)(tokens * top_k * ffn) * 2 : 0;
+}
+
+int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  RB200_CHECK(d != nullptr && d->struct_size == sizeof(rb200_moe_layer_fp4_desc), "rb200_moe_layer_fp4_desc has a wrong struct_size");
+  RB200_CHECK(d->format == f4::kMx || d->format == f4::kNv, "unknown 4-bit format %d", d->format);
+  RB200_CHECK(d->tokens >= 0 && d->tokens <= f4::kMaxTokens, "tokens=%lld outside [0, %d]", (long long)d->tokens, f4::kMaxTokens);
+  RB200_CHECK(d->num_experts >= 1 && d->num_experts <= f4::kMaxExperts, "num_experts=%lld outside [1, %d]", (long long)d->num_experts,
+              f4::kMaxExperts);
+  RB200_CHECK(d->top_k >= 1 && d->top_k <= f4::kMaxTopK && d->top_k <= d->num_experts, "top_k=%lld outside [1, min(%d, experts)]",
+              (long long)d->top_k, f4::kMaxTopK);
+  RB200_CHECK(d->hidden > 0 && d->hidden % 64 == 0 && d->ffn > 0 && d->ffn % 64 == 0 && d->hidden < (1 << 24) && d->ffn < (1 << 24) &&
+                  d->num_experts * 2 * d->ffn < (1ll << 31) && d->num_experts * d->hidden < (1ll << 31),
+              "hidden and ffn must be multiples of 64 (hidden=%lld, ffn=%lld)", (long long)d->hidden, (long long)d->ffn);
+  RB200_CHECK(d->format == f4::kNv || (!d->gate_up_tensor_scale && !d->down_tensor_scale), "the mx format has no tensor scale");
+  if (d->tokens == 0) return 0;
+  RB200_CHECK(d->x && d->logits && d->w_gate_up && d->gate_up_scales && d->w_down && d->down_scales && d->out && workspace,
+              "NULL argument");
+  RB200_CHECK(f4::aligned16(d->x) && f4::aligned16(d->w_gate_up) && f4::aligned16(d->gate_up_scales) && f4::aligned16(d->w_down) &&
+                  f4::aligned16(d->down_scales) && f4::aligned16(d->out) && f4::aligned16(workspace) &&
+                  (reinterpret_cast<uintptr_t>(d->logits) & 3u) == 0,
+              "tensors must be 16-byte aligned");
+  RB200_CHECK(workspace_bytes >= rb200_moe_layer_fp4_workspace_bytes(d->tokens, d->top_k, d->ffn),
+              "the workspace must hold rb200_moe_layer_fp4_workspace_bytes");
+  f4::Params p;
+  memset(&p, 0, sizeof(p));
+  p.x = static_cast<const __half*>(d->x);
+  p.logits = d->logits;
+  p.s1 = static_cast<const uint8_t*>(d->gate_up_scales);
+  p.s2 = static_cast<const uint8_t*>(d->down_scales);
+  p.ts1 = d->gate_up_tensor_scale;
+  p.ts2 = d->down_tensor_scale;
+  p.h = static_cast<__half*>(workspace);
+  p.out = static_cast<__half*>(d->out);
+  p.s1_expert = f4::scale_bytes(2 * d->ffn, d->hidden, d->format);
+  p.s2_expert = f4::scale_bytes(d->hidden, d->ffn, d->format);
+  p.tokens = (int)d->tokens;
+  p.experts = (int)d->num_experts;
+  p.top_k = (int)d->top_k;
+  p.renormalize = d->renormalize;
+  p.hidden = (int)d->hidden;
+  p.ffn = (int)d->ffn;
+  p.k_tiles1 = (int)f4::scale_k_tiles(d->hidden, d->format);
+  p.k_tiles2 = (int)f4::scale_k_tiles(d->ffn, d->format);
+  CUtensorMap t1, t2;
+  if (make_tensor_map_2d(&t1, d->w_gate_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d->hidden / 2,
+                         (unsigned long long)(d->num_experts * 2 * d->ffn), (unsigned long long)d->hidden / 2, 128, f4::kTile,
+                         CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tensor_map_2d(&t2, d->w_down, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d->ffn / 2,
+                         (unsigned long long)(d->num_experts * d->hidden), (unsigned long long)d->ffn / 2, 128, f4::kTile,
+                         CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+    return -1;
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < f4::kMaxDevices) f4::g_launched[dev].store(true, std::memory_order_relaxed);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return d->format == f4::kMx ? f4::launch_fmt<f4::kMx>(p, t1, t2, s) : f4::launch_fmt<f4::kNv>(p, t1, t2, s);
+}
+
+}  // extern "C"

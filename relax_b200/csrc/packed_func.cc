@@ -975,6 +975,51 @@ int pf_linear_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, 
   return rb200_linear_fp4(data_of(x), type, qw.k, &d, ws ? data_of(ws) : nullptr, ws ? (size_t)numel(ws) : 0, rb200_get_stream());
 }
 
+// (x, logits, w_gate_up, gate_up_scales, w_down, down_scales, top_k, format, gate_up_tensor_scale|null, down_tensor_scale|null,
+//  renormalize, workspace, out)
+int pf_moe_layer_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, void*) {
+  const char* fname = "relax_b200.moe_layer_fp4";
+  Args a{v, tc, n_args, fname};
+  PF_CHECK(n_args == 13, "%s expects 13 arguments, got %d", fname, n_args);
+  const DLTensor *x, *logits, *w1, *s1, *w2, *s2, *ts1, *ts2, *ws, *out;
+  int64_t top_k, renormalize;
+  Fp4Matrix up, down;
+  rb200_moe_layer_fp4_desc d;
+  memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  if (a.tensor(0, &x) || a.tensor(1, &logits) || a.tensor(2, &w1) || a.tensor(3, &s1) || a.tensor(4, &w2) || a.tensor(5, &s2) ||
+      a.integer(6, &top_k) || fp4_format(a, 7, &d.format) || a.tensor(8, &ts1, true) || a.tensor(9, &ts2, true) ||
+      a.integer(10, &renormalize) || a.tensor(11, &ws, true) || a.tensor(12, &out) || check_tensor(fname, "x", x, kDLFloat, 16) ||
+      check_tensor(fname, "logits", logits, kDLFloat, 32) || check_tensor(fname, "out", out, kDLFloat, 16) ||
+      fp4_matrix(fname, "w_gate_up", 3, d.format, w1, s1, ts1, &up) || fp4_matrix(fname, "w_down", 3, d.format, w2, s2, ts2, &down))
+    return -1;
+  PF_CHECK(x->ndim == 2 && logits->ndim == 2 && out->ndim == 2, "%s: x, logits and out must be 2-D", fname);
+  d.tokens = x->shape[0];
+  d.num_experts = up.batch;
+  d.top_k = top_k;
+  d.hidden = up.k;
+  d.ffn = down.k;
+  PF_CHECK(x->shape[1] == d.hidden && out->shape[0] == d.tokens && out->shape[1] == d.hidden, "%s: x and out must be [tokens, %lld]", fname,
+           (long long)d.hidden);
+  PF_CHECK(logits->shape[0] == d.tokens && logits->shape[1] == d.num_experts, "%s: logits must be [tokens, %lld]", fname,
+           (long long)d.num_experts);
+  PF_CHECK(down.batch == d.num_experts && up.rows == 2 * d.ffn && down.rows == d.hidden,
+           "%s: expected w_gate_up [E, 2 ffn, hidden / 2] and w_down [E, hidden, ffn / 2]", fname);
+  if (ws && check_tensor(fname, "workspace", ws, kDLUInt, 8)) return -1;
+  d.x = data_of(x);
+  d.logits = static_cast<const float*>(data_of(logits));
+  d.w_gate_up = up.codes;
+  d.gate_up_scales = up.scales;
+  d.gate_up_tensor_scale = up.ts;
+  d.w_down = down.codes;
+  d.down_scales = down.scales;
+  d.down_tensor_scale = down.ts;
+  d.out = data_of(out);
+  d.renormalize = renormalize != 0;
+  if (ret_tc) *ret_tc = RB200_ARG_NULL;
+  return rb200_moe_layer_fp4(&d, ws ? data_of(ws) : nullptr, ws ? (size_t)numel(ws) : 0, rb200_get_stream());
+}
+
 void register_builtin(const char* name, RB200PackedCFunc fn) {
   registry()[name] = new Entry{fn, nullptr, name};
 }
@@ -1004,6 +1049,7 @@ void ensure_builtins() {
   register_builtin("relax_b200.preprocess_fp4_scales", pf_preprocess_fp4_scales);
   register_builtin("relax_b200.gemm_fp4", pf_gemm_fp4);
   register_builtin("relax_b200.linear_fp4", pf_linear_fp4);
+  register_builtin("relax_b200.moe_layer_fp4", pf_moe_layer_fp4);
   register_builtin("runtime.get_cuda_stream", pf_get_stream);
   register_builtin("runtime.set_cuda_stream", pf_set_stream);
 }

@@ -39,6 +39,7 @@ struct Lib {
   decltype(&rb200_moe_gather) moe_gather;
   decltype(&rb200_moe_combine) moe_combine;
   decltype(&rb200_linear_fp4_workspace_bytes) linear_fp4_workspace_bytes;
+  decltype(&rb200_moe_layer_fp4_workspace_bytes) moe_layer_fp4_workspace_bytes;
 } lib;
 PyObject* error_class = nullptr;
 
@@ -741,6 +742,41 @@ PyObject* linear_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   GUARD_END
 }
 
+// moe_layer_fp4(x, logits, w_gate_up, gate_up_scales, w_down, down_scales, top_k, format, gate_up_tensor_scale, down_tensor_scale,
+//               renormalize, workspace, out)
+PyObject* moe_layer_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  GUARD_BEGIN
+  NEED_ARGS(13);
+  static Global fn("relax_b200.moe_layer_fp4");
+  const at::Tensor *x = as_tensor(a[0], "x"), *l = as_tensor(a[1], "logits"), *w2 = as_tensor(a[4], "w_down");
+  int64_t top_k;
+  Out out;
+  if (!x || !l || !w2 || !as_int(a[6], &top_k) || !out.take(a[12])) return nullptr;
+  if (x->dim() != 2 || w2->dim() != 3) return PyErr_SetString(PyExc_ValueError, "x must be [tokens, hidden], w_down [experts, hidden, ffn / 2]"), nullptr;
+  const at::Tensor xr = readable(*x);
+  at::Tensor lr = *l;
+  if (lr.scalar_type() != c10::ScalarType::Float || !lr.is_contiguous()) lr = lr.contiguous().to(c10::ScalarType::Float);
+  if (!out.given) out.t = empty_on(x->sizes(), c10::ScalarType::Half, *x);
+  at::Tensor ws;
+  if (a[11] == Py_None) {
+    ws = empty_on({static_cast<int64_t>(lib.moe_layer_fp4_workspace_bytes(x->size(0), top_k, w2->size(2) * 2))}, c10::ScalarType::Byte, *x);
+  } else {
+    const at::Tensor* p = as_tensor(a[11], "workspace");
+    if (!p) return nullptr;
+    ws = *p;
+  }
+  Frame f;
+  if (!f.tensor(xr) || !f.tensor(lr)) return nullptr;
+  for (int i = 2; i < 6; ++i)
+    if (!f.object(a[i])) return nullptr;
+  f.integer(top_k);
+  for (int i = 7; i < 11; ++i)
+    if (!f.object(a[i])) return nullptr;
+  if (!f.tensor(ws) || !f.tensor(out.t) || !f.call(fn.get())) return nullptr;
+  return out.give();
+  GUARD_END
+}
+
 // init(error_class, {symbol: address})
 PyObject* init(PyObject*, PyObject* args) {
   PyObject *cls, *table;
@@ -764,6 +800,7 @@ PyObject* init(PyObject*, PyObject* args) {
   TAKE(moe_gather, "rb200_moe_gather")
   TAKE(moe_combine, "rb200_moe_combine")
   TAKE(linear_fp4_workspace_bytes, "rb200_linear_fp4_workspace_bytes")
+  TAKE(moe_layer_fp4_workspace_bytes, "rb200_moe_layer_fp4_workspace_bytes")
 #undef TAKE
   Py_RETURN_NONE;
 }
@@ -773,7 +810,8 @@ PyMethodDef methods[] = {
     {"init", init, METH_VARARGS, nullptr},
     FAST(call),      FAST(check),     FAST(call_like), FAST(gemm_ft),    FAST(gemm_q4),    FAST(gemm_gptq),   FAST(gather_columns),
     FAST(moe_ft),    FAST(moe_q4),    FAST(group_fp16), FAST(moe_route),  FAST(moe_gather),  FAST(moe_combine),
-    FAST(encode_ft), FAST(encode_fp4), FAST(decode_fp4), FAST(preprocess_fp4_scales), FAST(gemm_fp4), FAST(linear_fp4), {nullptr, nullptr, 0, nullptr}};
+    FAST(encode_ft), FAST(encode_fp4), FAST(decode_fp4), FAST(preprocess_fp4_scales), FAST(gemm_fp4), FAST(linear_fp4),
+    FAST(moe_layer_fp4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

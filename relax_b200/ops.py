@@ -218,3 +218,23 @@ def linear_fp4(x, w, w_scales, fmt: str, x_tensor_scale=None, w_tensor_scale=Non
 def linear_fp4_workspace_bytes(m: int, k: int, fmt: str) -> int:
     from . import _lib
     return int(_lib.load().rb200_linear_fp4_workspace_bytes(m, k, {"mx": 0, "nv": 1}[fmt]))
+
+
+def moe_layer_fp4(x, logits, w_gate_up, gate_up_scales, w_down, down_scales, top_k: int, fmt: str, gate_up_tensor_scale=None,
+                  down_tensor_scale=None, renormalize: bool = False, workspace: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """An expert layer for at most 32 tokens over weights in 4-bit floats, in two kernels (``rb200_moe_layer_fp4``): what
+    :func:`moe_route`, :func:`moe_gather`, two grouped matmuls with ``silu(gate) * up`` between them and :func:`moe_combine`
+    do, for ``x`` fp16 [tokens, hidden] and router ``logits`` [tokens, experts].
+
+    ``w_gate_up`` codes [experts, 2 ffn, hidden/2] (gate rows first), ``w_down`` codes [experts, hidden, ffn/2], scales from
+    :func:`encode_fp4` or :func:`preprocess_fp4_scales`, tensor scales fp32 [experts] ("nv").  Gates are the softmax over all
+    experts, divided by their sum over the chosen ones with ``renormalize``.  ``workspace`` (uint8,
+    :func:`moe_layer_fp4_workspace_bytes`) and ``out`` make the call allocation-free."""
+    return native.moe_layer_fp4(x, logits, w_gate_up, gate_up_scales, w_down, down_scales, top_k, fmt, gate_up_tensor_scale,
+                                down_tensor_scale, renormalize, workspace, out)
+
+
+def moe_layer_fp4_workspace_bytes(tokens: int, top_k: int, ffn: int) -> int:
+    from . import _lib
+    return int(_lib.load().rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, ffn))

@@ -106,6 +106,40 @@ def test_linear_refusals():
     assert lin(m=0) == 0
 
 
+def _layer(**kw):
+    d = _lib.MoeLayerFp4Desc()
+    d.struct_size = ctypes.sizeof(_lib.MoeLayerFp4Desc)
+    for name in ("x", "logits", "w_gate_up", "gate_up_scales", "w_down", "down_scales", "out"):
+        setattr(d, name, 256)
+    d.tokens, d.num_experts, d.top_k, d.hidden, d.ffn = 2, 4, 2, 64, 128
+    for name, v in kw.items():
+        setattr(d, name, v)
+    return d
+
+
+@pytest.mark.parametrize("change, words", [
+    (dict(struct_size=8), "struct_size"), (dict(format=2), "format"), (dict(tokens=33), "tokens=33"), (dict(tokens=-1), "tokens=-1"),
+    (dict(num_experts=257), "num_experts=257"), (dict(num_experts=0), "num_experts=0"), (dict(top_k=5), "top_k=5"),
+    (dict(top_k=9, num_experts=16), "top_k=9"), (dict(top_k=0), "top_k=0"), (dict(hidden=96), "multiples of 64"),
+    (dict(ffn=32), "multiples of 64"), (dict(hidden=0), "multiples of 64"), (dict(gate_up_tensor_scale=256), "tensor scale"),
+    (dict(down_tensor_scale=256), "tensor scale"), (dict(x=None), "NULL"), (dict(logits=None), "NULL"), (dict(w_down=264), "aligned"),
+    (dict(out=264), "aligned"), (dict(logits=258), "aligned"),
+])
+def test_moe_refusals(change, words):
+    lib = _lib.load()
+    ws = ctypes.c_void_p(1024)
+    assert words in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer(**change)), ws, 1 << 20, None))
+
+
+def test_moe_workspace_refusals():
+    lib, ws = _lib.load(), ctypes.c_void_p(1024)
+    need = lib.rb200_moe_layer_fp4_workspace_bytes(2, 2, 128)
+    assert "NULL" in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer()), None, need, None))
+    assert "workspace" in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer()), ws, need - 1, None))
+    assert "aligned" in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer()), ctypes.c_void_p(1032), need, None))
+    assert lib.rb200_moe_layer_fp4(ctypes.byref(_layer(tokens=0)), ws, need, None) == 0
+
+
 def test_python_refusals():
     x = torch.zeros(4, 64).half()
     with pytest.raises(ValueError, match="mx"):
