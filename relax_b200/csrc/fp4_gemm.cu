@@ -13,6 +13,7 @@
 #include "fp4_encode.h"
 #include "fp4_gemm.h"
 #include "fp4_mma.cuh"
+#include "fp4_out.cuh"
 #include "tensormap.h"
 
 namespace rb200 {
@@ -37,16 +38,10 @@ constexpr int kWBytes = kTileN * 128;
 __device__ int g_status;
 
 struct Params {
+  Output o;
   const uint8_t* a_scales;
   const uint8_t* w_scales;
-  const float* a_ts;
-  const float* w_ts;
-  const void* bias;
-  const void* residual;
-  void* out;
-  int64_t ldo, ld_res;
-  int m, n, k, k_tiles;
-  int act, binop, unop;
+  int k, k_tiles;
   int nb, stages, tmem_cols, m_tiles, cluster, early;
 };
 
@@ -54,26 +49,6 @@ size_t stage_bytes(int fmt, int nb) {
   return (size_t)kWBytes + (size_t)nb * 128 + (size_t)stage_tiles(fmt) * 512 * (1 + (nb + 127) / 128);
 }
 size_t smem_bytes(int fmt, int nb, int stages) { return 1024 + stages * stage_bytes(fmt, nb) + (2 * kMaxStages + 2) * 8 + 32; }
-
-__device__ __forceinline__ float activation(float v, int act) {
-  switch (act) {
-    case RB200_ACT_RELU: return fmaxf(v, 0.0f);
-    case RB200_ACT_SILU: return v / (1.0f + __expf(-v));
-    case RB200_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    default: return v;
-  }
-}
-template <class T>
-__device__ __forceinline__ float finish(const Params& p, float v, float alpha, int m, int n) {
-  v *= alpha;
-  if (p.bias) v += widen(static_cast<const T*>(p.bias)[n]);
-  v = activation(v, p.act);
-  if (p.residual) {
-    const float r = widen(static_cast<const T*>(p.residual)[m * p.ld_res + n]);
-    v = p.binop == RB200_BIN_MULTIPLY ? v * r : v + r;
-  }
-  return p.unop == RB200_UN_RELU ? fmaxf(v, 0.0f) : v;
-}
 
 template <int FMT, class T>
 __global__ void __launch_bounds__(kThreads)
@@ -134,7 +109,7 @@ __global__ void __launch_bounds__(kThreads)
       tma_load(codes + (size_t)s * code_bytes + kWBytes, &tmap_a, c * 128, m0, &full[s]);
       for (int i = 0; i < a_tiles; ++i)
         // (a second tile of 128 rows that the batch does not reach: the first one again, its rows are never stored)
-        bulk_g2s(at + i * NT * 512, p.a_scales + ((int64_t)min((m0 >> 7) + i, (p.m - 1) >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c),
+        bulk_g2s(at + i * NT * 512, p.a_scales + ((int64_t)min((m0 >> 7) + i, (p.o.m - 1) >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c),
                  &full[s]);
     };
     const int first = min(stages, c1 - c0);  // stages filled before any is free again
@@ -224,7 +199,7 @@ __global__ void __launch_bounds__(kThreads)
     const int quad = warp & 3;
     const uint32_t lane_taddr = (uint32_t)(32 * quad) << 16;
     for (int c = 0; c < nb; c += 16) {
-      if (m0 + c >= p.m) break;
+      if (m0 + c >= p.o.m) break;
       float v[16];
       tc_ld16(lane_taddr | (tmem + c), v);
 #pragma unroll
@@ -235,11 +210,11 @@ __global__ void __launch_bounds__(kThreads)
   if (p.cluster > 1) cluster_sync();
   else __syncthreads();
   if (holder[1] == 0u) {
-    const float alpha = (p.a_ts ? *p.a_ts : 1.0f) * (p.w_ts ? *p.w_ts : 1.0f);
-    const int rows = min(nb, p.m - m0), lo = rows * rank / p.cluster, hi = rows * (rank + 1) / p.cluster;
+    const float alpha = out_scale(p.o);
+    const int rows = min(nb, p.o.m - m0), lo = rows * rank / p.cluster, hi = rows * (rank + 1) / p.cluster;
     const int n = n0 + lane * 4;
-    T* out = static_cast<T*>(p.out);
-    const bool wide = n + 4 <= p.n && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && p.ldo % 4 == 0;
+    T* out = static_cast<T*>(p.o.out);
+    const bool wide = n + 4 <= p.o.n && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && p.o.ldo % 4 == 0;
     for (int r = lo + warp; r < hi; r += kThreads / 32) {
       const uint32_t at = smem_u32(part + r * kTileN + lane * 4);
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -254,15 +229,15 @@ __global__ void __launch_bounds__(kThreads)
       const int m = m0 + r;
       __align__(16) T t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = n + i < p.n ? narrow<T>(finish<T>(p, f[i], alpha, m, n + i)) : narrow<T>(0.0f);
-      T* dst = out + m * p.ldo + n;
+      for (int i = 0; i < 4; ++i) t[i] = n + i < p.o.n ? narrow<T>(finish<T>(p.o, f[i], alpha, m, n + i)) : narrow<T>(0.0f);
+      T* dst = out + m * p.o.ldo + n;
       if (wide) {
         if (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
         else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (n + i < p.n) dst[i] = t[i];
+          if (n + i < p.o.n) dst[i] = t[i];
       }
     }
   }
@@ -287,7 +262,7 @@ int launch_typed(Params& p, const CUtensorMap& tw, const CUtensorMap& ta, cudaSt
     RB200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     configured_device = dev;
   }
-  const int n_tiles = (p.n + kTileN - 1) / kTileN, tiles = n_tiles * p.m_tiles, chunks = (p.k + kStageK - 1) / kStageK;
+  const int n_tiles = (p.o.n + kTileN - 1) / kTileN, tiles = n_tiles * p.m_tiles, chunks = (p.k + kStageK - 1) / kStageK;
   p.cluster = 1;
   while (p.cluster < 8 && tiles * p.cluster * 2 <= 2 * sm_count_current() && chunks >= 4 * p.cluster) p.cluster *= 2;
   p.stages = kMaxStages;
@@ -329,36 +304,30 @@ int fp4_gemm_read_status(int* status_out) {
   int dev = -1;
   RB200_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= f4::kMaxDevices || !f4::g_launched[dev].load(std::memory_order_relaxed)) return 0;
-  int v = 0;
+  int v = 0, pairs = 0;
   RB200_CUDA(cudaMemcpyFromSymbol(&v, f4::g_status, sizeof(int)));
   if (v != 0) {
     const int zero = 0;
     RB200_CUDA(cudaMemcpyToSymbol(f4::g_status, &zero, sizeof(int)));
   }
-  *status_out = v;
+  if (fp4_pair_read_status(&pairs) != 0) return -1;
+  *status_out = v != 0 ? v : pairs;
   return 0;
 }
 
 int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
   using namespace f4;
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < kMaxDevices) g_launched[dev].store(true, std::memory_order_relaxed);
+  if (d.m > 128) return fp4_pair_launch(d, stream);
   Params p;
   memset(&p, 0, sizeof(p));
+  p.o = output_of(d);
   p.a_scales = static_cast<const uint8_t*>(d.a_scales);
   p.w_scales = static_cast<const uint8_t*>(d.w_scales);
-  p.a_ts = d.a_tensor_scale;
-  p.w_ts = d.w_tensor_scale;
-  p.bias = d.bias;
-  p.residual = d.residual;
-  p.out = d.out;
-  p.ldo = d.ldo;
-  p.ld_res = d.n;
-  p.m = (int)d.m;
-  p.n = (int)d.n;
   p.k = (int)d.k;
   p.k_tiles = (int)scale_k_tiles(d.k, d.format);
-  p.act = d.activation;
-  p.binop = d.residual ? d.binary_op : RB200_BIN_NONE;
-  p.unop = d.unary_op;
   p.early = launch_overlap_enabled() ? 1 : 0;
   p.nb = d.m <= 256 ? (int)((d.m + 15) / 16 * 16) : 256;
   p.m_tiles = (int)((d.m + p.nb - 1) / p.nb);
@@ -370,9 +339,6 @@ int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
       make_tensor_map_2d(&ta, d.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.m,
                          (unsigned long long)d.k / 2, 128, (unsigned)p.nb, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
     return -1;
-  int dev = 0;
-  RB200_CUDA(cudaGetDevice(&dev));
-  if (dev >= 0 && dev < kMaxDevices) g_launched[dev].store(true, std::memory_order_relaxed);
   return d.format == kMx ? launch_fmt<kMx>(p, d.out_dtype, tw, ta, stream) : launch_fmt<kNv>(p, d.out_dtype, tw, ta, stream);
 }
 

@@ -1,0 +1,437 @@
+// Large batches of the 4-bit float product: pairs of CTAs on one 256 x 256 tile.
+//
+// The tile is out^T again: 256 rows of w, 128 in each CTA of the pair, by up to 256 rows of a, of which each CTA holds half
+// (tcgen05.mma, cta_group::2).  A stage is 256 k; everything it needs - codes, and scale tiles as rows of 128 words - comes
+// by tensor-map loads that count on rank 0's barrier, and rank 0's MMA thread copies the scales of both CTAs into tensor
+// memory.  What bounds a stage is the tensor cores (540 clocks at their nominal rate) and, close behind, what an SM takes
+// from L2: 38 KB at 64 bytes a clock are 600 clocks; tiles of 128 x 256 per SM without pairing would need 54 KB.
+// Accumulator and scales leave no room for a second accumulator, so the drain takes all 256 columns into registers (eight
+// warps, 128 columns each) and hands the tensor memory back before it applies the epilogue and stores: the MMAs of the next
+// tile wait for the reading only.
+#include <cstring>
+
+#include "fp4_gemm.h"
+#include "fp4_mma.cuh"
+#include "fp4_out.cuh"
+#include "tensormap.h"
+
+namespace rb200 {
+namespace f4 {
+namespace {
+
+using ug::elect_one;
+using ug::make_b_desc;
+using ug::tc_fence_after;
+using ug::tc_fence_before;
+
+constexpr int kThreads = 384;
+constexpr int kDrainWarps = 8;
+constexpr int kTileN = 128;  // rows of w in a CTA
+constexpr int kNb = 256;     // rows of a
+constexpr int kMaxStages = 6;
+constexpr int kStoreBytes = 2048;  // a warp's store: 32 columns by 32 (four-byte types: 16) rows
+
+__device__ int g_status;
+
+struct Params {
+  Output o;
+  int n_tiles, m_tiles, n_first, stages, early, tma_store, k, k_tiles;
+};
+
+template <int FMT>
+__host__ __device__ constexpr int stage_bytes() {
+  return kTileN * 128 + kNb / 2 * 128 + stage_tiles(FMT) * 512 * 3;
+}
+
+__device__ __forceinline__ void tmem_alloc2(uint32_t* holder, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// loads of either CTA, counted on rank 0's barrier
+__device__ __forceinline__ void tma_load2(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar0) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(bar0)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load3(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar0) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar0)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int c0, int c1, const void* src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1),
+               "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void stores_read() {  // all but the last LEFT stores have read shared memory
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ void commit2(uint64_t* bar) {  // arrives at both CTAs' barrier
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void copy_scales2(uint32_t taddr, uint64_t desc) {  // in both CTAs, each from its own shared memory
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int FMT>
+__device__ __forceinline__ void mma_scaled2(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                            uint32_t b_scales, uint32_t accumulate) {
+  if (FMT == kMx)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {  // 32 columns of this warp's lanes; tcgen05.wait::ld follows
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <int FMT, class T>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp4_pair_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                    const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_as,
+                    const __grid_constant__ CUtensorMap tmap_out) {
+  constexpr int NT = stage_tiles(FMT), kA = kTileN * 128, kWs = kA + kNb / 2 * 128, kAs = kWs + NT * 512;
+  constexpr int kWCol = kNb, kACol = kNb + 4 * NT;  // tensor memory columns of the scales
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int stages = p.stages;
+  uint8_t* store = smem + (size_t)stages * stage_bytes<FMT>();  // [drain warp][2][kStoreBytes]
+  uint64_t* full = reinterpret_cast<uint64_t*>(store + kDrainWarps * 2 * kStoreBytes);  // rank 0's are used
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* d_full = empty + kMaxStages;
+  uint64_t* d_empty = d_full + 1;  // rank 0's is used
+  uint32_t* holder = reinterpret_cast<uint32_t*>(d_empty + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank();
+  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(d_full, 1);
+    mbar_init(d_empty, 2 * kDrainWarps);
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc2(holder, 512u);
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before any remote arrival
+  tc_fence_after();
+  griddep_launch_dependents();
+  const uint32_t tmem = holder[0];
+  const int chunks = (p.k + kStageK - 1) / kStageK, items = p.n_tiles * p.m_tiles;
+  struct Item {
+    int n0, m0, width;  // this CTA's first row of w, the tile's first row of a, columns of the MMA
+  };
+  auto item_at = [&](int i) {
+    const int nt = p.n_first ? i % p.n_tiles : i / p.m_tiles, mt = p.n_first ? i / p.n_tiles : i % p.m_tiles;
+    Item it;
+    it.n0 = (2 * nt + rank) * kTileN;
+    it.m0 = mt * kNb;
+    it.width = min(kNb, (p.o.m - it.m0 + 31) / 32 * 32);
+    return it;
+  };
+
+  if (warp == 0) {
+    // ============================================================ loads
+    const bool leader = elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true, waited = false;
+    auto load_w = [&](const Item& it, int c, int s) {
+      uint8_t* at = smem + (size_t)s * stage_bytes<FMT>();
+      const uint32_t bar0 = at_rank(smem_u32(&full[s]), 0);
+      if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * (uint32_t)stage_bytes<FMT>());
+      tma_load2(at, &tmap_w, c * 128, it.n0, bar0);
+      tma_load3(at + kWs, &tmap_ws, 0, c * NT, it.n0 >> 7, bar0);
+    };
+    auto load_a = [&](const Item& it, int c, int s) {
+      uint8_t* at = smem + (size_t)s * stage_bytes<FMT>();
+      const uint32_t bar0 = at_rank(smem_u32(&full[s]), 0);
+      tma_load2(at + kA, &tmap_a, c * 128, it.m0 + rank * (it.width / 2), bar0);
+      tma_load3(at + kAs, &tmap_as, 0, c * NT, it.m0 >> 7, bar0);
+    };
+    if (!p.early) {
+      if (leader && pair < items) {
+        const Item it = item_at(pair);
+        for (int c = 0; c < min(stages, chunks); ++c) tma_prefetch(&tmap_w, c * 128, it.n0);
+      }
+      griddep_wait();
+      waited = true;
+    }
+    // before the wait only weights are read: as many stages as there are, in the first tile
+    int ahead = 0;
+    if (!waited) {
+      ahead = pair < items ? min(stages, chunks) : 0;
+      if (leader) {
+        const Item it = item_at(pair);
+        for (int c = 0; c < ahead; ++c) load_w(it, c, c);
+      }
+      __syncwarp();
+      griddep_wait();
+    }
+    for (int i = pair; ok && i < items; i += pairs) {
+      const Item it = item_at(i);
+      for (int c = 0; c < chunks; ++c) {
+        ok = mbar_wait_parked(&empty[s], ph, &g_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (leader) {
+          if (ahead == 0) load_w(it, c, s);
+          load_a(it, c, s);
+        }
+        __syncwarp();
+        if (ahead > 0) --ahead;
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    // every commit to this CTA's barriers has arrived, so every load has landed, before it may leave
+    for (int j = 0; ok && j < stages; ++j) {
+      ok = mbar_wait_parked(&empty[s], ph, &g_status);
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ============================================================ scales into tensor memory, MMAs
+    const bool leader = elect_one();
+    const uint64_t w_desc0 = make_b_desc(smem_u32(smem)), ws_desc0 = scale_desc(smem_u32(smem + kWs));
+    int s = 0;
+    uint32_t ph = 0, dph = 1;
+    bool ok = true;
+    for (int i = pair; ok && i < items; i += pairs, dph ^= 1u) {
+      const uint32_t idesc = mma_desc<FMT>(256, item_at(i).width);
+      const int a_tiles = item_at(i).width > 128 ? 2 : 1;
+      ok = mbar_wait_parked(d_empty, dph, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      for (int c = 0; c < chunks; ++c) {
+        ok = mbar_wait_parked(&full[s], ph, &g_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t off = (uint64_t)(s * (stage_bytes<FMT>() >> 4));
+          const uint64_t w_desc = w_desc0 + off, a_desc = w_desc + (uint64_t)(kA >> 4), sc = ws_desc0 + off;
+          const int mmas = min(kStageK, p.k - c * kStageK + kMmaK - 1) / kMmaK;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) copy_scales2(tmem + kWCol + 4 * t, sc + (uint64_t)(t * 32));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            copy_scales2(tmem + kACol + 8 * t, sc + (uint64_t)((NT + t) * 32));
+            if (a_tiles == 2) copy_scales2(tmem + kACol + 8 * t + 4, sc + (uint64_t)((2 * NT + t) * 32));
+          }
+#pragma unroll
+          for (int j = 0; j < kStageK / kMmaK; ++j) {
+            const int t = FMT == kMx ? j >> 1 : j;
+            if (j < mmas)
+              mma_scaled2<FMT>(tmem, w_desc + j * 2, a_desc + j * 2, FMT == kMx && (j & 1) ? upper_half(idesc) : idesc,
+                               tmem + kWCol + 4 * t, tmem + kACol + 8 * t, (c > 0 || j > 0) ? 1u : 0u);
+          }
+          commit2(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      if (ok && leader) commit2(d_full);
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ============================================================ drain
+    const int dw = warp - 4, quad = warp & 3, half = dw >> 2;
+    uint8_t* mine = store + dw * 2 * kStoreBytes;
+    const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(half * 128);
+    griddep_wait();
+    const float alpha = out_scale(p.o);
+    uint32_t ph = 0;
+    int buffer = 0;
+    for (int i = pair; i < items; i += pairs, ph ^= 1u) {
+      const Item it = item_at(i);
+      bool ok = mbar_wait_parked(d_full, ph, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const int rows = min(it.width, p.o.m - it.m0) - half * 128;  // of a, in this warp's columns
+      float v[128];
+      if (rows > 0) {
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(taddr + c, v + c);
+        ug::tc_wait_ld();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(at_rank(smem_u32(d_empty), 0));
+      const int n = it.n0 + quad * 32;
+      if (rows <= 0 || n >= p.o.n) continue;
+      const int m = it.m0 + half * 128;
+      constexpr int kRows = kStoreBytes / (32 * (int)sizeof(T));
+#pragma unroll
+      for (int c = 0; c < 128; c += kRows) {
+        if (c >= rows) break;
+        finish_column<T, kRows>(p.o, v + c, alpha, m + c, n + lane);
+        if (p.tma_store) {
+          T* st = reinterpret_cast<T*>(mine + buffer * kStoreBytes);
+          stores_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) st[r * 32 + lane] = narrow<T>(v[c + r]);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tma_store(&tmap_out, n, m + c, st);
+          buffer ^= 1;
+        } else if (n + lane < p.o.n) {
+          T* dst = static_cast<T*>(p.o.out) + (int64_t)(m + c) * p.o.ldo + n + lane;
+#pragma unroll
+          for (int r = 0; r < kRows; ++r)
+            if (c + r < rows) dst[r * p.o.ldo] = narrow<T>(v[c + r]);
+        }
+      }
+    }
+    stores_read<0>();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the other CTA may still have been reading this one's tiles, or arriving here
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem, 512u);
+  }
+}
+
+template <int FMT, class T>
+int launch_typed(Params& p, const CUtensorMap (&maps)[5], cudaStream_t stream) {
+  auto kern = fp4_pair_kernel<FMT, T>;
+  const size_t tail = (size_t)kDrainWarps * 2 * kStoreBytes + (2 * kMaxStages + 2) * 8 + 16 + 1024;
+  p.stages = kMaxStages;
+  while (p.stages > 2 && p.stages * (size_t)stage_bytes<FMT>() + tail > 227 * 1024) --p.stages;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = p.stages * (size_t)stage_bytes<FMT>() + tail;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    RB200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    configured_device = dev;
+  }
+  const int items = p.n_tiles * p.m_tiles, pairs = sm_count_current() / 2;
+  cfg.gridDim = dim3((unsigned)(2 * (items < pairs ? items : pairs)), 1, 1);
+  RB200_CUDA(cudaLaunchKernelEx(&cfg, kern, p, maps[0], maps[1], maps[2], maps[3], maps[4]));
+  return 0;
+}
+template <int FMT>
+int launch_fmt(Params& p, int dtype, const CUtensorMap (&maps)[5], cudaStream_t stream) {
+  switch (dtype) {
+    case kF16: return launch_typed<FMT, __half>(p, maps, stream);
+    case kBf16: return launch_typed<FMT, __nv_bfloat16>(p, maps, stream);
+    default: return launch_typed<FMT, float>(p, maps, stream);
+  }
+}
+
+// scales as rows of 128 words: [row tiles][k tiles][128], a stage's tiles of `row_tiles` x 128 rows a load
+int scale_map(CUtensorMap* map, const void* scales, int64_t rows, int64_t k, int fmt, unsigned row_tiles) {
+  const unsigned long long dims[3] = {128, (unsigned long long)scale_k_tiles(k, fmt), (unsigned long long)scale_row_tiles(rows)};
+  const unsigned long long strides[2] = {512, 512 * dims[1]};
+  const unsigned box[3] = {128, (unsigned)stage_tiles(fmt), row_tiles};
+  return make_tensor_map(map, scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+}  // namespace
+}  // namespace f4
+
+int fp4_pair_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
+  using namespace f4;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.o = output_of(d);
+  p.k = (int)d.k;
+  p.k_tiles = (int)scale_k_tiles(d.k, d.format);
+  p.early = launch_overlap_enabled() ? 1 : 0;
+  p.n_tiles = (int)((d.n + 2 * kTileN - 1) / (2 * kTileN));
+  p.m_tiles = (int)((d.m + kNb - 1) / kNb);
+  // Two tiles of a, the second one usually smaller: all the large ones first.  More: neighbours share a tile of w.
+  p.n_first = p.m_tiles <= 2;
+  const int width = d.out_dtype == kF32 ? 4 : 2;
+  p.tma_store = reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.ldo * width % 16 == 0;
+  CUtensorMap maps[5];
+  if (make_tensor_map_2d(&maps[0], d.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.n,
+                         (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tensor_map_2d(&maps[1], d.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.m,
+                         (unsigned long long)d.k / 2, 128, kNb / 2, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      scale_map(&maps[2], d.w_scales, d.n, d.k, d.format, 1) != 0 || scale_map(&maps[3], d.a_scales, d.m, d.k, d.format, 2) != 0)
+    return -1;
+  maps[4] = maps[0];
+  if (p.tma_store &&
+      make_tensor_map_2d(&maps[4], d.out,
+                         d.out_dtype == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                         : d.out_dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                         (unsigned long long)d.n, (unsigned long long)d.m, (unsigned long long)d.ldo * width, 32,
+                         (unsigned)(kStoreBytes / (32 * width)), CU_TENSOR_MAP_SWIZZLE_NONE) != 0)
+    return -1;
+  return d.format == kMx ? launch_fmt<kMx>(p, d.out_dtype, maps, stream) : launch_fmt<kNv>(p, d.out_dtype, maps, stream);
+}
+
+int fp4_pair_read_status(int* v) {
+  RB200_CUDA(cudaMemcpyFromSymbol(v, f4::g_status, sizeof(int)));
+  if (*v != 0) {
+    const int zero = 0;
+    RB200_CUDA(cudaMemcpyToSymbol(f4::g_status, &zero, sizeof(int)));
+  }
+  return 0;
+}
+
+}  // namespace rb200

@@ -188,7 +188,7 @@ def _check_product(got, a, w, alpha=1.0, tail=None):
 
 SHAPES = [(1, 1, 32), (1, 128, 64), (3, 130, 96), (8, 256, 256), (16, 64, 288), (17, 200, 320), (33, 127, 512), (64, 384, 1056),
           (100, 129, 2080), (129, 256, 800), (200, 100, 256), (257, 300, 544), (520, 257, 1024), (1, 4096, 4096), (40, 96, 8192),
-          (1000, 513, 96)]
+          (1000, 513, 96), (300, 9600, 64), (1300, 4100, 288), (385, 1024, 1536), (256, 128, 32)]
 
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
@@ -216,10 +216,10 @@ def test_gemm_every_code_and_scale(fmt):
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("m, n", [(5, 136), (70, 131)])
+@pytest.mark.parametrize("m, n", [(5, 136), (70, 131), (300, 264), (150, 131)])
 def test_gemm_epilogue(fmt, dtype, m, n):
     k, t = 256, TYPES[dtype]
-    g = _gen(m + n)
+    g = _gen(m + n if m < 100 else 5)
     (ac, asc, a), (wc, wsc, w) = _operand(g, fmt, m, k), _operand(g, fmt, n, k)
     scale = 1.0 / 64
     ta = torch.tensor([scale], device="cuda") if fmt == "nv" else None
