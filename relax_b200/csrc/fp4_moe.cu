@@ -36,16 +36,17 @@ constexpr int kMaxStages = 6;
 
 __device__ int g_status;
 
+// Rows are the (token, expert) pairs by expert; an entry is at most 8 NT rows of one expert.
 struct alignas(16) Routing {
   uint32_t mask[kMaxExperts];       // tokens of an expert
-  int active[kMaxRows];             // experts with tokens, in order
-  int row_begin[kMaxRows + 1];      // their rows
+  int entry_expert[kMaxRows];
+  int entry_row[kMaxRows + 1];
   uint8_t token_of_row[kMaxRows];
   float gate_of_row[kMaxRows];
   int expert_of[kMaxRows];          // by token and choice
   float gate_of[kMaxRows];
-  int warp_sum[2][kConsumers];
-  int experts;                      // number of active ones
+  int warp_sum[kConsumers];
+  int entries;
   int failed;
 };
 
@@ -70,114 +71,145 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return v == v ? ((b & 0x80000000u) ? ~b : b | 0x80000000u) : 0u;
 }
 
-// The routing by the eight consumer warps (256 threads; every thread of the CTA calls it).  The top_k largest logits of
-// a token (equal ones: lower expert first), gates softmax over all experts, or over the chosen ones.
-__device__ void route(const Params& p, Routing& r) {
+// U tokens (t, t + 8, ..) by a warp, side by side: what takes the time is the latency of each step.  PER experts a lane.
+template <int U, int PER>
+__device__ __forceinline__ void choose(const Params& p, Routing& r, int t) {
+  const int lane = threadIdx.x & 31;
+  float v[U][PER], top[U], sum[U], chosen[U], mine[U];
+  uint32_t key[U][PER];
+  int my_expert[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool token = t + u * kConsumers < p.tokens;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = i * 32 + lane;
+      v[u][i] = token && e < p.experts ? __ldcg(p.logits + (t + u * kConsumers) * p.experts + e) : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    top[u] = v[u][0];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      top[u] = fmaxf(top[u], v[u][i]);
+      key[u][i] = i * 32 + lane < p.experts ? max(order_key(v[u][i]), 1u) : 0u;  // 0: not there, or taken
+    }
+    chosen[u] = mine[u] = 0.0f;
+    my_expert[u] = 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    sum[u] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i * 32 + lane < p.experts) sum[u] += expf(v[u][i] - top[u]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+  for (int j = 0; j < p.top_k; ++j) {
+    uint32_t best[U], all[U];
+    int at[U], e[U];
+    float val[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      best[u] = key[u][0];
+      at[u] = lane;
+      val[u] = v[u][0];
+#pragma unroll
+      for (int i = 1; i < PER; ++i)
+        if (key[u][i] > best[u]) {
+          best[u] = key[u][i];
+          at[u] = i * 32 + lane;
+          val[u] = v[u][i];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) all[u] = __reduce_max_sync(0xffffffffu, best[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u] = (int)__reduce_min_sync(0xffffffffu, best[u] == all[u] ? (uint32_t)at[u] : 0xffffu);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = expf(__shfl_sync(0xffffffffu, val[u], e[u] & 31) - top[u]);
+      chosen[u] += w;
+      if (lane == j) {
+        mine[u] = w;
+        my_expert[u] = e[u];
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i * 32 + lane == e[u]) key[u][i] = 0u;
+    }
+  }
+  // (a NaN among the logits, or nothing but -inf: sum is NaN, and so is every gate)
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int token = t + u * kConsumers;
+    if (token < p.tokens && lane < p.top_k) {
+      r.expert_of[token * p.top_k + lane] = my_expert[u];
+      r.gate_of[token * p.top_k + lane] = p.renormalize && sum[u] == sum[u] ? mine[u] / chosen[u] : mine[u] / sum[u];
+      atomicOr(&r.mask[my_expert[u]], 1u << token);
+    }
+  }
+}
+
+// The routing, by every thread of the CTA: the top_k largest logits of a token (equal ones: lower expert first), gates
+// softmax over all experts or over the chosen ones; rows and entries of `most` rows in expert order.
+template <int U>
+__device__ void route(const Params& p, Routing& r, int most) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < kMaxExperts) r.mask[tid] = 0u;
   __syncthreads();
-  if (warp < kConsumers)
-    for (int t = warp; t < p.tokens; t += kConsumers) {
-      constexpr int kPer = kMaxExperts / 32;
-      const int per = (p.experts + 31) / 32;
-      float v[kPer];
-      uint32_t key[kPer];
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int e = i * 32 + lane;
-        v[i] = i < per && e < p.experts ? __ldcg(p.logits + t * p.experts + e) : -INFINITY;
-        top = fmaxf(top, v[i]);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int e = i * 32 + lane;
-        const bool there = i < per && e < p.experts;
-        if (there) sum += expf(v[i] - top);
-        key[i] = there ? max(order_key(v[i]), 1u) : 0u;  // 0: not there, or taken
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      float chosen = 0.0f, mine = 0.0f;
-      int my_expert = 0;
-      for (int j = 0; j < p.top_k; ++j) {
-        uint32_t best = 0u;
-        int at = 0;
-        float val = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (key[i] > best) {
-            best = key[i];
-            at = i;
-            val = v[i];
-          }
-        const uint32_t all = __reduce_max_sync(0xffffffffu, best);
-        const int e = (int)__reduce_min_sync(0xffffffffu, best == all ? (uint32_t)(at * 32 + lane) : 0xffffu);
-        const float l = __shfl_sync(0xffffffffu, val, e & 31), w = expf(l - top);
-        chosen += w;
-        if (lane == j) {
-          mine = w;
-          my_expert = e;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (i * 32 + lane == e) key[i] = 0u;
-      }
-      // (a NaN among the logits, or nothing but -inf: sum is NaN, and so is every gate)
-      if (lane < p.top_k) {
-        r.expert_of[t * p.top_k + lane] = my_expert;
-        r.gate_of[t * p.top_k + lane] = p.renormalize && sum == sum ? mine / chosen : mine / sum;
-        atomicOr(&r.mask[my_expert], 1u << t);
-      }
-    }
+  if (warp < kConsumers && warp < p.tokens) {
+    if (p.experts <= 32) choose<U, 1>(p, r, warp);
+    else if (p.experts <= 64) choose<U, 2>(p, r, warp);
+    else choose<U, kMaxExperts / 32>(p, r, warp);
+  }
   __syncthreads();
-  // experts with tokens and their rows, in expert order
   const uint32_t m = tid < kMaxExperts ? r.mask[tid] : 0u;
-  const int n = __popc(m);
-  const uint32_t ballot = __ballot_sync(0xffffffffu, n > 0);
-  int upto = n;
+  const int n = __popc(m), parts = (n + most - 1) / most;
+  int upto = n | parts << 16;  // rows and entries counted together
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
   }
-  if (warp < kConsumers && lane == 31) {
-    r.warp_sum[0][warp] = upto;
-    r.warp_sum[1][warp] = __popc(ballot);
-  }
+  if (warp < kConsumers && lane == 31) r.warp_sum[warp] = upto;
   __syncthreads();
   if (warp < kConsumers) {
-    int row = upto - n, a = __popc(ballot & ((1u << lane) - 1u));
-    for (int w = 0; w < warp; ++w) {
-      row += r.warp_sum[0][w];
-      a += r.warp_sum[1][w];
+    int before = upto - (n | parts << 16);
+    for (int w = 0; w < warp; ++w) before += r.warp_sum[w];
+    const int row = before & 0xffff, a = before >> 16;
+    for (int i = 0; i < parts; ++i) {
+      r.entry_expert[a + i] = tid;
+      r.entry_row[a + i] = row + i * most;
     }
-    if (n > 0) {
-      r.active[a] = tid;
-      r.row_begin[a] = row;
-      uint32_t left = m;
-      for (int i = 0; i < n; ++i, left &= left - 1u) {
-        const int t = __ffs((int)left) - 1;
-        float gate = 0.0f;
-        for (int j = 0; j < p.top_k; ++j)
-          if (r.expert_of[t * p.top_k + j] == tid) gate = r.gate_of[t * p.top_k + j];
-        r.token_of_row[row + i] = (uint8_t)t;
-        r.gate_of_row[row + i] = gate;
-      }
+    uint32_t left = m;
+    for (int i = 0; i < n; ++i, left &= left - 1u) {
+      const int t = __ffs((int)left) - 1;
+      float gate = 0.0f;
+      for (int j = 0; j < p.top_k; ++j)
+        if (r.expert_of[t * p.top_k + j] == tid) gate = r.gate_of[t * p.top_k + j];
+      r.token_of_row[row + i] = (uint8_t)t;
+      r.gate_of_row[row + i] = gate;
     }
     if (tid == kMaxExperts - 1) {
-      r.experts = a + (n > 0);
-      r.row_begin[a + (n > 0)] = row + n;
+      r.entries = a + parts;
+      r.entry_row[a + parts] = row + n;
     }
   }
   __syncthreads();
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// 16 bytes of global memory, or zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 // arrives at the barrier when this thread's copies so far have landed (the barrier counts these arrivals)
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
@@ -185,10 +217,15 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -196,71 +233,77 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Rows g and g + 8 of a 16-row block over the 32 k of a chunk: sums of the products with the x words of NT column tiles.
-// w0, w8: code words.  kMx: f0, f8 scales of the block; kNv: p0, p8 this lane's scales as f16x2.
+// The scales of rows g and g + 8 over 128 k, as the products take them.
+template <int FMT>
+struct Scales {
+  // kMx: fp32 scales of the four blocks of either row.  kNv: f16x2, this lane's scale of row g and of row g + 8, by chunk
+  float f0[4], f8[4];
+  uint32_t both[4];
+  __device__ __forceinline__ void take(const uint8_t* at, int t) {  // `at`: row g's word in the (first) tile
+    if (FMT == kMx) {
+      expand(*reinterpret_cast<const uint32_t*>(at), f0);
+      expand(*reinterpret_cast<const uint32_t*>(at + 8 * 16), f8);
+    } else {
+      // blocks 2i and 2i + 1 of chunk i; lanes t < 2 hold k of the first, the others of the second
+      const uint32_t sel = t < 2 ? 0x40u : 0x51u;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(at + q * 512) & 0x7f7f7f7fu;
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(at + q * 512 + 8 * 16) & 0x7f7f7f7fu;
+        both[2 * q] = from_e4m3x2(__byte_perm(a, b, sel));
+        both[2 * q + 1] = from_e4m3x2(__byte_perm(a, b, sel + 0x22u));
+      }
+    }
+  }
+  static __device__ __forceinline__ void expand(uint32_t w, float (&f)[4]) {
+    uint32_t lo, hi;  // bf16 has the exponents of e8m0
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.bf16x2.ue8m0x2 %0, a;\n\t"
+        "cvt.rn.bf16x2.ue8m0x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+    f[0] = __uint_as_float(lo << 16);
+    f[1] = __uint_as_float(lo & 0xffff0000u);
+    f[2] = __uint_as_float(hi << 16);
+    f[3] = __uint_as_float(hi & 0xffff0000u);
+  }
+};
+
+// Rows g and g + 8 of a 16-row block over the 32 k of chunk i: sums of the products with the x words of the column tiles.
 template <int FMT, int NT>
-__device__ __forceinline__ void chunk(float (&acc)[NT][4], uint32_t w0, uint32_t w8, float f0, float f8, uint32_t p0, uint32_t p8,
-                                      const uint4 (&x)[NT], int tiles) {
+__device__ __forceinline__ void chunk(float (&acc)[NT][4], uint32_t w0, uint32_t w8, const Scales<FMT>& s, int i, const uint4 (&x)[NT],
+                                      int tiles) {
   uint32_t a0[4], a8[4];
   from_codes8(w0, a0);
   from_codes8(w8, a8);
   if (FMT == kNv) {
+    const uint32_t p0 = __byte_perm(s.both[i], 0u, 0x1010), p8 = __byte_perm(s.both[i], 0u, 0x3232);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a0[i] = mul2(a0[i], p0);
-      a8[i] = mul2(a8[i], p8);
+    for (int q = 0; q < 4; ++q) {
+      a0[q] = mul2(a0[q], p0);
+      a8[q] = mul2(a8[q], p8);
     }
   }
-  const uint32_t lo[4] = {a0[0], a8[0], a0[1], a8[1]}, hi[4] = {a0[2], a8[2], a0[3], a8[3]};
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     if (j > 0 && j >= tiles) break;
     if (FMT == kNv) {
-      mma(acc[j], lo, x[j].x, x[j].y);
-      mma(acc[j], hi, x[j].z, x[j].w);
+      mma(acc[j], a0[0], a8[0], a0[1], a8[1], x[j].x, x[j].y);
+      mma(acc[j], a0[2], a8[2], a0[3], a8[3], x[j].z, x[j].w);
     } else {
-      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      mma(part, lo, x[j].x, x[j].y);
-      mma(part, hi, x[j].z, x[j].w);
-      acc[j][0] = fmaf(part[0], f0, acc[j][0]);
-      acc[j][1] = fmaf(part[1], f0, acc[j][1]);
-      acc[j][2] = fmaf(part[2], f8, acc[j][2]);
-      acc[j][3] = fmaf(part[3], f8, acc[j][3]);
+      float part[4];
+      mma_first(part, a0[0], a8[0], a0[1], a8[1], x[j].x, x[j].y);
+      mma(part, a0[2], a8[2], a0[3], a8[3], x[j].z, x[j].w);
+      acc[j][0] = fmaf(part[0], s.f0[i], acc[j][0]);
+      acc[j][1] = fmaf(part[1], s.f0[i], acc[j][1]);
+      acc[j][2] = fmaf(part[2], s.f8[i], acc[j][2]);
+      acc[j][3] = fmaf(part[3], s.f8[i], acc[j][3]);
     }
   }
 }
 
-// Four chunks (128 k) of 16 rows: `codes` a box of 128-byte rows, swizzled, c0 its first 16-byte column; `words` the scale
-// tiles (one of kMx, two of kNv) at this lane's row g, `words8` at row g + 8.
-template <int FMT, int NT>
-struct Quarter {
-  const uint8_t* row0;
-  const uint8_t* words0;
-  const uint8_t* words8;
-  uint32_t s0, s8;
-  int g, t;
-  __device__ __forceinline__ void scales(int i) {
-    if (FMT == kMx ? i == 0 : (i & 1) == 0) {
-      const int at = FMT == kMx ? 0 : (i >> 1) * 512;
-      s0 = *reinterpret_cast<const uint32_t*>(words0 + at);
-      s8 = *reinterpret_cast<const uint32_t*>(words8 + at);
-    }
-  }
-  __device__ __forceinline__ void step(int i, int column, float (&acc)[NT][4], const uint4 (&x)[NT], int tiles) {
-    scales(i);
-    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(row0 + ((column ^ g) << 4) + t * 4);
-    const uint32_t w8 = *reinterpret_cast<const uint32_t*>(row0 + 8 * 128 + ((column ^ g) << 4) + t * 4);
-    if (FMT == kMx) {
-      chunk<FMT, NT>(acc, w0, w8, e8m0_value((s0 >> (8 * i)) & 0xffu), e8m0_value((s8 >> (8 * i)) & 0xffu), 0u, 0u, x, tiles);
-    } else {
-      const int sh = 16 * (i & 1) + 8 * (t >> 1);
-      const uint32_t two = from_e4m3x2(((s0 >> sh) & 0x7fu) | ((s8 >> sh) & 0x7fu) << 8);
-      chunk<FMT, NT>(acc, w0, w8, 0.0f, 0.0f, __byte_perm(two, 0u, 0x1010), __byte_perm(two, 0u, 0x3232), x, tiles);
-    }
-  }
-};
-
-// shared memory: [codes of all stages][scales][x][barriers][routing ..]
+// Shared memory: [codes of all stages][scales][x][barriers][routing][sums], offsets from the aligned base.
 struct Layout {
   int code_bytes, scale_bytes, x_bytes;  // of a stage
 };
@@ -272,14 +315,10 @@ template <int FMT, int NT>
 __host__ __device__ constexpr Layout layout_down() {
   return {2 * kBox, 2 * stage_tiles(FMT) * 512, NT * 8 * 2 * kStageK * 2};
 }
+__host__ __device__ constexpr int stage_total(const Layout& l) { return l.code_bytes + l.scale_bytes + l.x_bytes; }
 
-// One kernel's ring of stages.
+// Position in the ring of stages.
 struct Ring {
-  uint8_t* codes;
-  uint8_t* scales;
-  uint8_t* x;
-  uint64_t* full;
-  uint64_t* empty;
   int stages, s;
   uint32_t ph;
   __device__ __forceinline__ void next() {
@@ -289,31 +328,23 @@ struct Ring {
     }
   }
 };
-__device__ __forceinline__ Ring make_ring(uint8_t* smem, const Layout& l, int stages) {
-  Ring r;
-  r.codes = smem;
-  r.scales = r.codes + stages * l.code_bytes;
-  r.x = r.scales + stages * l.scale_bytes;
-  r.full = reinterpret_cast<uint64_t*>(r.x + stages * l.x_bytes);
-  r.empty = r.full + kMaxStages;
-  r.stages = stages;
-  r.s = 0;
-  r.ph = 0u;
-  return r;
-}
-__device__ __forceinline__ void init_ring(const Ring& r) {
-  for (int i = 0; i < r.stages; ++i) {
-    mbar_init(&r.full[i], 1 + 32);       // the loads' bytes, a lane's copies of x each
-    mbar_init(&r.empty[i], kConsumers);
+__device__ __forceinline__ void init_ring(uint64_t* full, uint64_t* empty, int stages) {
+  for (int i = 0; i < stages; ++i) {
+    mbar_init(&full[i], 1 + 32);       // the loads' bytes, a lane's copies of x each
+    mbar_init(&empty[i], kConsumers);
   }
   mbar_fence_init();
 }
 // No load may be on its way when the CTA leaves: the last fill of every stage.
-__device__ __forceinline__ bool drain_ring(const Ring& r, int issued) {
-  bool ok = true;
-  for (int i = max(0, issued - r.stages); i < issued; ++i)
-    ok = mbar_wait_parked(&r.full[i % r.stages], (uint32_t)(i / r.stages) & 1u, &g_status) && ok;
-  return ok;
+__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, int issued) {
+  for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait_parked(&full[i % stages], (uint32_t)(i / stages) & 1u, &g_status);
+}
+// `tiles` consecutive scale tiles from `from` on, those past `last` replaced by the last one: it has the same rows' scales, and
+// what is past k is zero codes and zeros of x.
+__device__ __forceinline__ void load_scale_tiles(uint8_t* dst, const uint8_t* base, int from, int tiles, int last, uint64_t* bar) {
+  const int there = min(tiles, last + 1 - from);
+  bulk_g2s(dst, base + (int64_t)from * 512, (uint32_t)there * 512u, bar);
+  for (int i = there; i < tiles; ++i) bulk_g2s(dst + i * 512, base + (int64_t)last * 512, 512u, bar);
 }
 // 16-byte column of x in its row's 512 bytes, so that a quarter-warp's reads (two rows, four columns) meet no bank twice
 __device__ __forceinline__ int x_column(int row, int column) { return column ^ ((row & 1) << 2); }
@@ -321,94 +352,107 @@ __device__ __forceinline__ int x_column(int row, int column) { return column ^ (
 constexpr int kRoutingOffset = 2 * kMaxStages * 8;
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
-    moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
+__global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr Layout L = layout_up<FMT, NT>();
   constexpr int TILES = stage_tiles(FMT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  Ring ring = make_ring(smem, L, p.stages);
-  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(ring.full) + kRoutingOffset);
+  uint8_t* const scales = smem + p.stages * L.code_bytes;
+  uint8_t* const xs = scales + p.stages * L.scale_bytes;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(xs + p.stages * L.x_bytes);
+  uint64_t* const empty = full + kMaxStages;
+  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    init_ring(ring);
+    init_ring(full, empty, p.stages);
     r.failed = 0;
   }
   fence_proxy_async();
   griddep_wait();
   griddep_launch_dependents();
-  route(p, r);
+  route<NT == 1 ? 1 : 4>(p, r, NT * 8);
 
-  const int f_tiles = p.ffn / kTile, items = r.experts * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
+  const int f_tiles = p.ffn / kTile, items = r.entries * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
+  Ring ring = {p.stages, 0, 0u};
   if (warp == kConsumers) {
     // ============================================================ loads
     int issued = 0;
     bool ok = true;
     for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.active[a];
-      const int row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0;
+      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
+      const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
       const uint8_t* s_gate = p.s1 + e * p.s1_expert + (int64_t)(f0 >> 7) * p.k_tiles1 * 512;
       const uint8_t* s_up = p.s1 + e * p.s1_expert + (int64_t)((p.ffn + f0) >> 7) * p.k_tiles1 * 512;
       for (int c = 0; c < chunks; ++c) {
-        ok = mbar_wait_parked(&ring.empty[ring.s], ring.ph ^ 1u, &g_status);
+        ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint64_t* bar = &ring.full[ring.s];
+        uint64_t* bar = &full[ring.s];
         if (lane == 0) {
-          const uint32_t tiles = (uint32_t)min(TILES, p.k_tiles1 - c * TILES) * 512u;
-          uint8_t* w = ring.codes + ring.s * L.code_bytes;
-          uint8_t* sc = ring.scales + ring.s * L.scale_bytes;
-          mbar_arrive_expect_tx(bar, 2 * kBox + 2 * tiles);
+          uint8_t* w = smem + ring.s * L.code_bytes;
+          uint8_t* sc = scales + ring.s * L.scale_bytes;
+          mbar_arrive_expect_tx(bar, L.code_bytes + L.scale_bytes);
           tma_load(w, &tmap_w, c * 128, e * 2 * p.ffn + f0, bar);
           tma_load(w + kBox, &tmap_w, c * 128, e * 2 * p.ffn + p.ffn + f0, bar);
-          bulk_g2s(sc, s_gate + c * TILES * 512, tiles, bar);
-          bulk_g2s(sc + TILES * 512, s_up + c * TILES * 512, tiles, bar);
+          load_scale_tiles(sc, s_gate, c * TILES, TILES, p.k_tiles1 - 1, bar);
+          load_scale_tiles(sc + TILES * 512, s_up, c * TILES, TILES, p.k_tiles1 - 1, bar);
         }
         __syncwarp();
-        if (c * kStageK + lane * 8 < p.hidden)
-          for (int i = 0; i < rows; ++i)
-            cp_async16(ring.x + ring.s * L.x_bytes + i * (kStageK * 2) + x_column(i, lane) * 16,
-                       p.x + (int64_t)r.token_of_row[row0 + i] * p.hidden + c * kStageK + lane * 8);
+        const int k = c * kStageK + lane * 8;
+        const bool there = k < p.hidden;
+        const uint32_t dst = smem_u32(xs + ring.s * L.x_bytes);
+        for (int i = 0; i < rows; ++i)
+          cp_async16(dst + i * (kStageK * 2) + x_column(i, lane) * 16,
+                     p.x + (int64_t)r.token_of_row[row0 + i] * p.hidden + (there ? k : 0), there);
         cp_async_arrive(bar);
         ++issued;
         ring.next();
       }
     }
-    drain_ring(ring, issued);
+    drain_ring(full, p.stages, issued);
   } else {
     // ============================================================ products
     const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
     float* red = reinterpret_cast<float*>(&r + 1);  // [fb][value][lane]
+    const uint8_t* const w_at = smem + (fb * 16 + g) * 128 + t * 4;
+    const uint8_t* const x_at = xs + g * (kStageK * 2) + kh * 256 + t * 16;
+    const uint8_t* const s_at = scales + kh * (TILES / 2) * 512;
+    int off[4], xoff[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      off[i] = ((kh * 4 + i) ^ g) << 4;
+      xoff[i] = (i ^ (g & 1)) * 64;
+    }
     bool ok = true;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
-      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.active[a];
-      const int row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0, tiles = (rows + 7) / 8;
+      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
+      const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
       float gate[NT][4], up[NT][4];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) gate[j][i] = up[j][i] = 0.0f;
-      const int rg = (f0 & 127) + fb * 16 + g, ru = ((p.ffn + f0) & 127) + fb * 16 + g;  // rows in their scale tiles
+      // this lane's words in the scale tiles of its rows
+      const int sg = (int)scale_word((f0 & 127) + fb * 16 + g, 0, 1), su = TILES * 512 + (int)scale_word(((p.ffn + f0) & 127) + fb * 16 + g, 0, 1);
       for (int c = 0; c < chunks; ++c) {
-        if (ok) ok = mbar_wait_parked(&ring.full[ring.s], ring.ph, &g_status);
-        const uint8_t* w = ring.codes + ring.s * L.code_bytes + (fb * 16 + g) * 128;
-        const uint8_t* sc = ring.scales + ring.s * L.scale_bytes + kh * (TILES / 2) * 512;
-        Quarter<FMT, NT> qg = {w, sc + scale_word(rg, 0, 1), sc + scale_word(rg + 8, 0, 1), 0u, 0u, g, t};
-        Quarter<FMT, NT> qu = {w + kBox, sc + TILES * 512 + scale_word(ru, 0, 1), sc + TILES * 512 + scale_word(ru + 8, 0, 1), 0u, 0u, g, t};
-        const int left = (p.hidden - c * kStageK - kh * 128) / 32;  // chunks of 32 k there are
-        const uint8_t* xs = ring.x + ring.s * L.x_bytes + g * (kStageK * 2);
+        if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
+        const uint8_t* w = w_at + ring.s * L.code_bytes;
+        const uint8_t* x0 = x_at + ring.s * L.x_bytes;
+        Scales<FMT> qg, qu;
+        qg.take(s_at + ring.s * L.scale_bytes + sg, t);
+        qu.take(s_at + ring.s * L.scale_bytes + su, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (i >= left) break;
-          const int column = kh * 4 + i;
           uint4 x[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const uint4*>(xs + j * 8 * (kStageK * 2) + x_column(g, column * 4 + t) * 16);
-          qg.step(i, column, gate, x, tiles);
-          qu.step(i, column, up, x, tiles);
+          for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const uint4*>(x0 + xoff[i] + j * 8 * (kStageK * 2));
+          chunk<FMT, NT>(gate, *reinterpret_cast<const uint32_t*>(w + off[i]), *reinterpret_cast<const uint32_t*>(w + off[i] + 8 * 128), qg,
+                         i, x, tiles);
+          chunk<FMT, NT>(up, *reinterpret_cast<const uint32_t*>(w + off[i] + kBox),
+                         *reinterpret_cast<const uint32_t*>(w + off[i] + kBox + 8 * 128), qu, i, x, tiles);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+        if (lane == 0) mbar_arrive(&empty[ring.s]);
         ring.next();
       }
       // the halves of k meet; rows g, g + 8 of columns 2t, 2t + 1
@@ -443,43 +487,45 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 }
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
-    moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
+__global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr Layout L = layout_down<FMT, NT>();
   constexpr int TILES = stage_tiles(FMT), kUnitK = 2 * kStageK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  Ring ring = make_ring(smem, L, p.stages);
-  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(ring.full) + kRoutingOffset);
+  uint8_t* const scales = smem + p.stages * L.code_bytes;
+  uint8_t* const xs = scales + p.stages * L.scale_bytes;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(xs + p.stages * L.x_bytes);
+  uint64_t* const empty = full + kMaxStages;
+  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
   float* sums = reinterpret_cast<float*>(&r + 1);  // [half of k][token][64 columns]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.cluster) * kTile;
   if (tid == 0) {
-    init_ring(ring);
+    init_ring(full, empty, p.stages);
     r.failed = 0;
   }
   for (int i = tid; i < 2 * p.tokens * kTile; i += kThreads) sums[i] = 0.0f;
   fence_proxy_async();
   // The logits and the weights are older than the kernel before this one, which let this one start only after its own wait
   // (the logits are read past L1, which may hold what was there before them).
-  route(p, r);
+  route<NT == 1 ? 1 : 4>(p, r, NT * 8);
 
-  const int per = (p.ffn + kUnitK - 1) / kUnitK, units = r.experts * per;
+  const int per = (p.ffn + kUnitK - 1) / kUnitK, units = r.entries * per;
   const int u0 = (int)((int64_t)units * rank / p.cluster), u1 = (int)((int64_t)units * (rank + 1) / p.cluster);
+  Ring ring = {p.stages, 0, 0u};
   if (warp == kConsumers) {
     // ============================================================ loads
     int issued = 0;
     bool ok = true;
     auto load_w = [&](int u, int s) {
-      const int a = u / per, c = u - a * per, e = r.active[a];
-      const uint32_t tiles = (uint32_t)min(2 * TILES, p.k_tiles2 - c * 2 * TILES) * 512u;
-      uint8_t* w = ring.codes + s * L.code_bytes;
-      const bool two = c * kUnitK + kStageK < p.ffn;
-      mbar_arrive_expect_tx(&ring.full[s], (two ? 2 * kBox : kBox) + tiles);
-      tma_load(w, &tmap_w, c * 256, e * p.hidden + n0, &ring.full[s]);
-      if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + n0, &ring.full[s]);
-      bulk_g2s(ring.scales + s * L.scale_bytes, p.s2 + e * p.s2_expert + ((int64_t)(n0 >> 7) * p.k_tiles2 + c * 2 * TILES) * 512, tiles,
-               &ring.full[s]);
+      const int a = u / per, c = u - a * per, e = r.entry_expert[a];
+      uint8_t* w = smem + s * L.code_bytes;
+      const bool two = c * kUnitK + kStageK < p.ffn;  // (else the second box keeps what it had: its x is zeros)
+      mbar_arrive_expect_tx(&full[s], (two ? 2 * kBox : kBox) + L.scale_bytes);
+      tma_load(w, &tmap_w, c * 256, e * p.hidden + n0, &full[s]);
+      if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + n0, &full[s]);
+      load_scale_tiles(scales + s * L.scale_bytes, p.s2 + e * p.s2_expert + (int64_t)(n0 >> 7) * p.k_tiles2 * 512, c * 2 * TILES, 2 * TILES,
+                       p.k_tiles2 - 1, &full[s]);
     };
     const int first = min(p.stages, u1 - u0);
     if (lane == 0)
@@ -487,65 +533,72 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     griddep_wait();  // h is the kernel before's
     for (int u = u0; u < u1; ++u) {
       if (u - u0 >= first) {
-        ok = mbar_wait_parked(&ring.empty[ring.s], ring.ph ^ 1u, &g_status);
+        ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) load_w(u, ring.s);
       }
       __syncwarp();
-      const int a = u / per, c = u - a * per, row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0;
-      for (int i = 0; i < rows; ++i)
+      const int a = u / per, c = u - a * per, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
+      const uint32_t dst = smem_u32(xs + ring.s * L.x_bytes);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int k = c * kUnitK + half * kStageK + lane * 8;
-          if (k < p.ffn)
-            cp_async16(ring.x + ring.s * L.x_bytes + (half * NT * 8 + i) * (kStageK * 2) + x_column(i, lane) * 16,
-                       p.h + (int64_t)(row0 + i) * p.ffn + k);
-        }
-      cp_async_arrive(&ring.full[ring.s]);
+      for (int half = 0; half < 2; ++half) {
+        const int k = c * kUnitK + half * kStageK + lane * 8;
+        const bool there = k < p.ffn;
+        const __half* src = p.h + (int64_t)row0 * p.ffn + (there ? k : 0);
+        for (int i = 0; i < rows; ++i)
+          cp_async16(dst + (half * NT * 8 + i) * (kStageK * 2) + x_column(i, lane) * 16, src + (int64_t)i * p.ffn, there);
+      }
+      cp_async_arrive(&full[ring.s]);
       ++issued;
       ring.next();
     }
-    drain_ring(ring, issued);
+    drain_ring(full, p.stages, issued);
   } else {
     // ============================================================ products
     const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
+    const uint8_t* const w_at = smem + kh * kBox + (fb * 16 + g) * 128 + t * 4;
+    const uint8_t* const x_at = xs + (kh * NT * 8 + g) * (kStageK * 2) + t * 16;
+    const uint8_t* const s_at = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g, 0, 1);
+    int off[8], xoff[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) off[i] = (i ^ g) << 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xoff[i] = (i ^ (g & 1)) * 64;
     bool ok = true;
     float acc[NT][4];
-    const int rn = (n0 & 127) + fb * 16 + g;
     for (int u = u0; u < u1; ++u) {
       const int a = u / per, c = u - a * per;
-      const int row0 = r.row_begin[a], rows = r.row_begin[a + 1] - row0, tiles = (rows + 7) / 8;
+      const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
       if (u == u0 || c == 0) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
       }
-      if (ok) ok = mbar_wait_parked(&ring.full[ring.s], ring.ph, &g_status);
-      const uint8_t* w = ring.codes + ring.s * L.code_bytes + kh * kBox + (fb * 16 + g) * 128;
-      const uint8_t* xs = ring.x + ring.s * L.x_bytes + (kh * NT * 8 + g) * (kStageK * 2);
-      const int left = (p.ffn - c * kUnitK - kh * kStageK) / 32;
+      if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
+      const uint8_t* w = w_at + ring.s * L.code_bytes;
+      const uint8_t* x0 = x_at + ring.s * L.x_bytes;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const uint8_t* sc = ring.scales + ring.s * L.scale_bytes + (kh * TILES + q * (TILES / 2)) * 512;
-        Quarter<FMT, NT> qd = {w, sc + scale_word(rn, 0, 1), sc + scale_word(rn + 8, 0, 1), 0u, 0u, g, t};
+        Scales<FMT> qd;
+        qd.take(s_at + ring.s * L.scale_bytes + q * (TILES / 2) * 512, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int column = q * 4 + i;
-          if (column >= left) break;
           uint4 x[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const uint4*>(xs + j * 8 * (kStageK * 2) + x_column(g, column * 4 + t) * 16);
-          qd.step(i, column, acc, x, tiles);
+          for (int j = 0; j < NT; ++j)
+            x[j] = *reinterpret_cast<const uint4*>(x0 + xoff[i & 1] + q * 256 + (i >> 1) * 128 + j * 8 * (kStageK * 2));
+          chunk<FMT, NT>(acc, *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i]),
+                         *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i] + 8 * 128), qd, i, x, tiles);
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+      if (lane == 0) mbar_arrive(&empty[ring.s]);
       ring.next();
       if (u + 1 == u1 || c + 1 == per) {
-        // this expert's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane)
-        const float ts = p.ts2 ? p.ts2[r.active[a]] : 1.0f;
+        // this entry's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane)
+        const float ts = p.ts2 ? p.ts2[r.entry_expert[a]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -592,7 +645,7 @@ constexpr int kMaxDevices = 64;
 std::atomic<bool> g_launched[kMaxDevices];  // devices whose status word a wait may have set
 
 size_t smem_bytes(const Layout& l, int stages, size_t extra) {
-  return 1024 + (size_t)stages * (l.code_bytes + l.scale_bytes + l.x_bytes) + kRoutingOffset + sizeof(Routing) + extra;
+  return 1024 + (size_t)stages * stage_total(l) + kRoutingOffset + sizeof(Routing) + extra;
 }
 
 template <int FMT, int NT>
@@ -607,22 +660,22 @@ int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t 
     RB200_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     configured_device = dev;
   }
-  const int sms = sm_count_current(), ctas = NT == 1 ? 2 : 1;  // of an SM
-  const size_t room = (size_t)(NT == 1 ? 113 : 226) * 1024;
-  const int rows = p.tokens * p.top_k, most = rows < p.experts ? rows : p.experts;  // experts that can have tokens
+  const int ctas = 2 * sm_count_current();
+  const size_t room = (size_t)113 * 1024;  // two CTAs an SM
+  const int rows = p.tokens * p.top_k;
 
   const size_t red = (size_t)4 * NT * 8 * 32 * 4;
   p.stages = kMaxStages;
   while (p.stages > 2 && smem_bytes(layout_up<FMT, NT>(), p.stages, red) > room) --p.stages;
-  const int64_t items = (int64_t)most * (p.ffn / kTile);
-  RB200_CUDA(launch_dependent(up, dim3((unsigned)(items < ctas * sms ? items : ctas * sms)), kThreads,
+  const int64_t items = (int64_t)rows * (p.ffn / kTile);  // at most
+  RB200_CUDA(launch_dependent(up, dim3((unsigned)(items < ctas ? items : ctas)), kThreads,
                               smem_bytes(layout_up<FMT, NT>(), p.stages, red), stream, p, t1));
 
   const size_t sums = (size_t)2 * p.tokens * kTile * 4;
   p.stages = kMaxStages;
   while (p.stages > 2 && smem_bytes(layout_down<FMT, NT>(), p.stages, sums) > room) --p.stages;
   const int n_tiles = p.hidden / kTile, per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK);
-  p.cluster = ctas * sms / n_tiles;
+  p.cluster = ctas / n_tiles;
   if (p.cluster > 8) p.cluster = 8;
   if (p.cluster > per) p.cluster = per;
   if (p.cluster < 1) p.cluster = 1;
@@ -645,10 +698,7 @@ int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t 
 
 template <int FMT>
 int launch_fmt(const Params& p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t stream) {
-  // an expert may have every token
-  if (p.tokens <= 8) return launch<FMT, 1>(p, t1, t2, stream);
-  if (p.tokens <= 16) return launch<FMT, 2>(p, t1, t2, stream);
-  return launch<FMT, 4>(p, t1, t2, stream);
+  return p.tokens <= 8 ? launch<FMT, 1>(p, t1, t2, stream) : launch<FMT, 2>(p, t1, t2, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
