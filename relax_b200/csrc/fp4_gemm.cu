@@ -335,7 +335,7 @@ int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
   p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
   CUtensorMap tw, ta;
   if (make_tensor_map_2d(&tw, d.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.n,
-                         (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+                         (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0 ||
       make_tensor_map_2d(&ta, d.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.m,
                          (unsigned long long)d.k / 2, 128, (unsigned)p.nb, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
     return -1;

@@ -27,9 +27,11 @@ namespace rb200 {
 namespace f4 {
 namespace {
 
+using ug::elect_one;
+
 constexpr int kMaxTokens = 32, kMaxExperts = 256, kMaxTopK = 8, kMaxRows = kMaxTokens * kMaxTopK;
 constexpr int kConsumers = 8;  // warps: four blocks of 16 rows, two halves of k
-constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kThreads = (kConsumers + 2) * 32;  // and a warp for the weights' loads, one for x's
 constexpr int kTile = 64;      // rows of a weight box
 constexpr int kBox = kTile * 128;
 constexpr int kMaxStages = 6;
@@ -375,20 +377,20 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p,
   const int f_tiles = p.ffn / kTile, items = r.entries * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
   Ring ring = {p.stages, 0, 0u};
   if (warp == kConsumers) {
-    // ============================================================ loads
+    // ============================================================ weights
+    const bool leader = elect_one();
     int issued = 0;
     bool ok = true;
     for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
       const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
-      const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
       const uint8_t* s_gate = p.s1 + e * p.s1_expert + (int64_t)(f0 >> 7) * p.k_tiles1 * 512;
       const uint8_t* s_up = p.s1 + e * p.s1_expert + (int64_t)((p.ffn + f0) >> 7) * p.k_tiles1 * 512;
       for (int c = 0; c < chunks; ++c) {
         ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint64_t* bar = &full[ring.s];
-        if (lane == 0) {
+        if (leader) {
+          uint64_t* bar = &full[ring.s];
           uint8_t* w = smem + ring.s * L.code_bytes;
           uint8_t* sc = scales + ring.s * L.scale_bytes;
           mbar_arrive_expect_tx(bar, L.code_bytes + L.scale_bytes);
@@ -398,13 +400,31 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p,
           load_scale_tiles(sc + TILES * 512, s_up, c * TILES, TILES, p.k_tiles1 - 1, bar);
         }
         __syncwarp();
-        const int k = c * kStageK + lane * 8;
-        const bool there = k < p.hidden;
+        ++issued;
+        ring.next();
+      }
+    }
+    drain_ring(full, p.stages, issued);
+  } else if (warp == kConsumers + 1) {
+    // ============================================================ x
+    int issued = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const int a = item / f_tiles, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
+      const __half* src[NT * 8];
+#pragma unroll
+      for (int i = 0; i < NT * 8; ++i) src[i] = p.x + (int64_t)r.token_of_row[row0 + min(i, rows - 1)] * p.hidden + lane * 8;
+      for (int c = 0; c < chunks; ++c) {
+        ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int k = c * kStageK;
+        const bool there = k + lane * 8 < p.hidden;
         const uint32_t dst = smem_u32(xs + ring.s * L.x_bytes);
-        for (int i = 0; i < rows; ++i)
-          cp_async16(dst + i * (kStageK * 2) + x_column(i, lane) * 16,
-                     p.x + (int64_t)r.token_of_row[row0 + i] * p.hidden + (there ? k : 0), there);
-        cp_async_arrive(bar);
+#pragma unroll
+        for (int i = 0; i < NT * 8; ++i)
+          if (i < rows) cp_async16(dst + i * (kStageK * 2) + x_column(i, lane) * 16, there ? src[i] + k : p.x, there);
+        cp_async_arrive(&full[ring.s]);
         ++issued;
         ring.next();
       }
@@ -514,31 +534,37 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
   const int u0 = (int)((int64_t)units * rank / p.cluster), u1 = (int)((int64_t)units * (rank + 1) / p.cluster);
   Ring ring = {p.stages, 0, 0u};
   if (warp == kConsumers) {
-    // ============================================================ loads
+    // ============================================================ weights (older than the kernel before, too)
+    const bool leader = elect_one();
     int issued = 0;
-    bool ok = true;
-    auto load_w = [&](int u, int s) {
-      const int a = u / per, c = u - a * per, e = r.entry_expert[a];
-      uint8_t* w = smem + s * L.code_bytes;
-      const bool two = c * kUnitK + kStageK < p.ffn;  // (else the second box keeps what it had: its x is zeros)
-      mbar_arrive_expect_tx(&full[s], (two ? 2 * kBox : kBox) + L.scale_bytes);
-      tma_load(w, &tmap_w, c * 256, e * p.hidden + n0, &full[s]);
-      if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + n0, &full[s]);
-      load_scale_tiles(scales + s * L.scale_bytes, p.s2 + e * p.s2_expert + (int64_t)(n0 >> 7) * p.k_tiles2 * 512, c * 2 * TILES, 2 * TILES,
-                       p.k_tiles2 - 1, &full[s]);
-    };
-    const int first = min(p.stages, u1 - u0);
-    if (lane == 0)
-      for (int s = 0; s < first; ++s) load_w(u0 + s, s);
-    griddep_wait();  // h is the kernel before's
     for (int u = u0; u < u1; ++u) {
-      if (u - u0 >= first) {
-        ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) load_w(u, ring.s);
+      bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (leader) {
+        const int a = u / per, c = u - a * per, e = r.entry_expert[a];
+        uint64_t* bar = &full[ring.s];
+        uint8_t* w = smem + ring.s * L.code_bytes;
+        const bool two = c * kUnitK + kStageK < p.ffn;  // (else the second box keeps what it had: its x is zeros)
+        mbar_arrive_expect_tx(bar, (two ? 2 * kBox : kBox) + L.scale_bytes);
+        tma_load(w, &tmap_w, c * 256, e * p.hidden + n0, bar);
+        if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + n0, bar);
+        load_scale_tiles(scales + ring.s * L.scale_bytes, p.s2 + e * p.s2_expert + (int64_t)(n0 >> 7) * p.k_tiles2 * 512, c * 2 * TILES,
+                         2 * TILES, p.k_tiles2 - 1, bar);
       }
       __syncwarp();
+      ++issued;
+      ring.next();
+    }
+    drain_ring(full, p.stages, issued);
+  } else if (warp == kConsumers + 1) {
+    // ============================================================ h
+    griddep_wait();  // the kernel before's
+    int issued = 0;
+    for (int u = u0; u < u1; ++u) {
+      bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       const int a = u / per, c = u - a * per, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
       const uint32_t dst = smem_u32(xs + ring.s * L.x_bytes);
 #pragma unroll
@@ -546,8 +572,9 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
         const int k = c * kUnitK + half * kStageK + lane * 8;
         const bool there = k < p.ffn;
         const __half* src = p.h + (int64_t)row0 * p.ffn + (there ? k : 0);
-        for (int i = 0; i < rows; ++i)
-          cp_async16(dst + (half * NT * 8 + i) * (kStageK * 2) + x_column(i, lane) * 16, src + (int64_t)i * p.ffn, there);
+#pragma unroll
+        for (int i = 0; i < NT * 8; ++i)
+          if (i < rows) cp_async16(dst + (half * NT * 8 + i) * (kStageK * 2) + x_column(i, lane) * 16, src + (int64_t)i * p.ffn, there);
       }
       cp_async_arrive(&full[ring.s]);
       ++issued;
@@ -675,22 +702,37 @@ int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t 
   p.stages = kMaxStages;
   while (p.stages > 2 && smem_bytes(layout_down<FMT, NT>(), p.stages, sums) > room) --p.stages;
   const int n_tiles = p.hidden / kTile, per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK);
-  p.cluster = ctas / n_tiles;
-  if (p.cluster > 8) p.cluster = 8;
-  if (p.cluster > per) p.cluster = per;
-  if (p.cluster < 1) p.cluster = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(n_tiles * p.cluster), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem_bytes(layout_down<FMT, NT>(), p.stages, sums);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  // Clusters do not fill the SMs evenly, so how many of each size run at a time is asked for (once: the sums' share of
+  // shared memory at its largest, which changes no stage count).  Time goes with waves / size.
+  static thread_local int places_device = -1, places[9];
+  if (places_device != dev) {
+    cfg.numAttrs = 1;
+    cudaLaunchConfig_t ask = cfg;
+    ask.dynamicSmemBytes = room;
+    for (int c = 1; c <= 8; ++c) {
+      attr[0].val.clusterDim.x = (unsigned)c;
+      ask.gridDim = dim3((unsigned)(ctas / c * c), 1, 1);
+      RB200_CUDA(cudaOccupancyMaxActiveClusters(&places[c], down, &ask));
+    }
+    places_device = dev;
+  }
+  p.cluster = 1;
+  for (int c = 2; c <= 8 && c <= p.top_k * per; ++c) {  // (a token's experts are top_k different ones)
+    auto waves = [&](int size) { return places[size] < 1 ? 1 << 20 : (n_tiles + places[size] - 1) / places[size]; };
+    if (waves(c) * p.cluster < waves(p.cluster) * c) p.cluster = c;
+  }
+  cfg.gridDim = dim3((unsigned)(n_tiles * p.cluster), 1, 1);
+  attr[0].val.clusterDim.x = (unsigned)p.cluster;
   cfg.numAttrs = 2;
   RB200_CUDA(cudaLaunchKernelEx(&cfg, down, p, t2));
   return 0;
@@ -775,10 +817,10 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   CUtensorMap t1, t2;
   if (make_tensor_map_2d(&t1, d->w_gate_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d->hidden / 2,
                          (unsigned long long)(d->num_experts * 2 * d->ffn), (unsigned long long)d->hidden / 2, 128, f4::kTile,
-                         CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0 ||
       make_tensor_map_2d(&t2, d->w_down, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d->ffn / 2,
                          (unsigned long long)(d->num_experts * d->hidden), (unsigned long long)d->ffn / 2, 128, f4::kTile,
-                         CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0)
     return -1;
   int dev = 0;
   RB200_CUDA(cudaGetDevice(&dev));

@@ -31,7 +31,7 @@ namespace {
 // everything the encoding depends on.
 struct MapKey {
   const void* base;
-  int dtype, rank, swizzle;
+  int dtype, rank, swizzle, promotion;
   unsigned long long dims[5], strides[4];
   unsigned box[5];
   bool operator==(const MapKey& o) const { return memcmp(this, &o, sizeof(MapKey)) == 0; }
@@ -53,7 +53,7 @@ unsigned hash_key(const MapKey& k) {
 
 int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, int rank,
                     const unsigned long long* dims, const unsigned long long* strides_bytes,
-                    const unsigned* box, CUtensorMapSwizzle swizzle) {
+                    const unsigned* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   RB200_CHECK(rank >= 1 && rank <= 5, "tensor map rank %d out of range", rank);
   MapKey key;
   memset(&key, 0, sizeof(key));
@@ -61,6 +61,7 @@ int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtyp
   key.dtype = (int)dtype;
   key.rank = rank;
   key.swizzle = (int)swizzle;
+  key.promotion = (int)promotion;
   for (int i = 0; i < rank; ++i) {
     key.dims[i] = dims[i];
     key.box[i] = box[i];
@@ -87,7 +88,7 @@ int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtyp
     }
   }
   CUresult r = g_encode(out, dtype, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RB200_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
   slot.key = key;
@@ -99,10 +100,10 @@ int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtyp
 int make_tensor_map_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype,
                        unsigned long long dim0, unsigned long long dim1,
                        unsigned long long stride1_bytes, unsigned box0, unsigned box1,
-                       CUtensorMapSwizzle swizzle) {
+                       CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   const unsigned long long dims[2] = {dim0, dim1};
   const unsigned long long strides[1] = {stride1_bytes};
   const unsigned box[2] = {box0, box1};
-  return make_tensor_map(out, base, dtype, 2, dims, strides, box, swizzle);
+  return make_tensor_map(out, base, dtype, 2, dims, strides, box, swizzle, promotion);
 }
 }  // namespace rb200

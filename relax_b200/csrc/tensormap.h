@@ -11,9 +11,11 @@ namespace rb200 {
 int make_tensor_map_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype,
                        unsigned long long dim0, unsigned long long dim1,
                        unsigned long long stride1_bytes, unsigned box0, unsigned box1,
-                       CUtensorMapSwizzle swizzle);
+                       CUtensorMapSwizzle swizzle,
+                       CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 // General form: rank 1..5, dims[0] innermost, strides_bytes[i] = pitch of dims[i+1].
 int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, int rank,
                     const unsigned long long* dims, const unsigned long long* strides_bytes,
-                    const unsigned* box, CUtensorMapSwizzle swizzle);
+                    const unsigned* box, CUtensorMapSwizzle swizzle,
+                    CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }  // namespace rb200
