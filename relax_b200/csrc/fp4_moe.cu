@@ -29,8 +29,8 @@ namespace {
 
 using ug::elect_one;
 
-constexpr int kMaxTokens = 32, kMaxExperts = 256, kMaxTopK = 8, kMaxRows = kMaxTokens * kMaxTopK;
-constexpr int kConsumers = 8;  // warps: four blocks of 16 rows, two halves of k
+constexpr int kMaxTokens = 32, kMaxExperts = 256, kMaxTopK = 8;
+constexpr int kConsumers = 8;  // warps: four blocks of 16 rows, gate and up or two halves of k
 constexpr int kThreads = (kConsumers + 2) * 32;  // and a warp for the weights' loads, one for x's
 constexpr int kTile = 64;      // rows of a weight box
 constexpr int kBox = kTile * 128;
@@ -38,18 +38,20 @@ constexpr int kMaxStages = 6;
 
 __device__ int g_status;
 
-// Rows are the (token, expert) pairs by expert; an entry is at most 8 NT rows of one expert.
+// Rows are the (token, expert) pairs by expert; an entry is at most 8 NT rows of one expert.  NT = 1 has at most eight tokens.
+template <int NT>
 struct alignas(16) Routing {
-  uint32_t mask[kMaxExperts];       // tokens of an expert
-  int entry_expert[kMaxRows];
-  int entry_row[kMaxRows + 1];
-  uint8_t token_of_row[kMaxRows];
-  float gate_of_row[kMaxRows];
-  int expert_of[kMaxRows];          // by token and choice
-  float gate_of[kMaxRows];
+  static constexpr int kRows = (NT == 1 ? 8 : kMaxTokens) * kMaxTopK;
+  uint32_t mask[kMaxExperts];  // tokens of an expert
+  float gate_of_row[kRows];
+  float gate_of[kRows];        // by token and choice
   int warp_sum[kConsumers];
   int entries;
   int failed;
+  uint16_t entry_row[kRows + 2];
+  uint8_t entry_expert[kRows];
+  uint8_t token_of_row[kRows];
+  uint8_t expert_of[kRows];
 };
 
 struct Params {
@@ -74,8 +76,8 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 
 // U tokens (t, t + 8, ..) by a warp, side by side: what takes the time is the latency of each step.  PER experts a lane.
-template <int U, int PER>
-__device__ __forceinline__ void choose(const Params& p, Routing& r, int t) {
+template <int U, int PER, int NT>
+__device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, int t) {
   const int lane = threadIdx.x & 31;
   float v[U][PER], top[U], sum[U], chosen[U], mine[U];
   uint32_t key[U][PER];
@@ -154,7 +156,7 @@ __device__ __forceinline__ void choose(const Params& p, Routing& r, int t) {
   for (int u = 0; u < U; ++u) {
     const int token = t + u * kConsumers;
     if (token < p.tokens && lane < p.top_k) {
-      r.expert_of[token * p.top_k + lane] = my_expert[u];
+      r.expert_of[token * p.top_k + lane] = (uint8_t)my_expert[u];
       r.gate_of[token * p.top_k + lane] = p.renormalize && sum[u] == sum[u] ? mine[u] / chosen[u] : mine[u] / sum[u];
       atomicOr(&r.mask[my_expert[u]], 1u << token);
     }
@@ -162,9 +164,10 @@ __device__ __forceinline__ void choose(const Params& p, Routing& r, int t) {
 }
 
 // The routing, by every thread of the CTA: the top_k largest logits of a token (equal ones: lower expert first), gates
-// softmax over all experts or over the chosen ones; rows and entries of `most` rows in expert order.
-template <int U>
-__device__ void route(const Params& p, Routing& r, int most) {
+// softmax over all experts or over the chosen ones; rows and entries in expert order.
+template <int NT>
+__device__ void route(const Params& p, Routing<NT>& r) {
+  constexpr int U = NT == 1 ? 1 : kMaxTokens / kConsumers, most = NT * 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < kMaxExperts) r.mask[tid] = 0u;
   __syncthreads();
@@ -189,8 +192,8 @@ __device__ void route(const Params& p, Routing& r, int most) {
     for (int w = 0; w < warp; ++w) before += r.warp_sum[w];
     const int row = before & 0xffff, a = before >> 16;
     for (int i = 0; i < parts; ++i) {
-      r.entry_expert[a + i] = tid;
-      r.entry_row[a + i] = row + i * most;
+      r.entry_expert[a + i] = (uint8_t)tid;
+      r.entry_row[a + i] = (uint16_t)(row + i * most);
     }
     uint32_t left = m;
     for (int i = 0; i < n; ++i, left &= left - 1u) {
@@ -203,7 +206,7 @@ __device__ void route(const Params& p, Routing& r, int most) {
     }
     if (tid == kMaxExperts - 1) {
       r.entries = a + parts;
-      r.entry_row[a + parts] = row + n;
+      r.entry_row[a + parts] = (uint16_t)(row + n);
     }
   }
   __syncthreads();
@@ -305,6 +308,35 @@ __device__ __forceinline__ void chunk(float (&acc)[NT][4], uint32_t w0, uint32_t
   }
 }
 
+// A warp's share of a stage: 16 rows over 256 k, eight chunks of 32.  `w` row g of the block in a box of 128-byte rows, swizzled,
+// at this lane's word; `x` row g of the stage's x at this lane's 16 bytes; `sc` row g's word in the first scale tile.
+template <int FMT, int NT>
+struct Walk {
+  int off[8], xoff[2];
+  __device__ __forceinline__ explicit Walk(int g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) off[i] = (i ^ g) << 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xoff[i] = (i ^ (g & 1)) * 64;
+  }
+  __device__ __forceinline__ void stage(float (&acc)[NT][4], const uint8_t* w, const uint8_t* x0, const uint8_t* sc, int t, int tiles) const {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      Scales<FMT> s;
+      s.take(sc + q * (stage_tiles(FMT) / 2) * 512, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 x[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          x[j] = *reinterpret_cast<const uint4*>(x0 + xoff[i & 1] + q * 256 + (i >> 1) * 128 + j * 8 * (kStageK * 2));
+        chunk<FMT, NT>(acc, *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i]),
+                       *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i] + 8 * 128), s, i, x, tiles);
+      }
+    }
+  }
+};
+
 // Shared memory: [codes of all stages][scales][x][barriers][routing][sums], offsets from the aligned base.
 struct Layout {
   int code_bytes, scale_bytes, x_bytes;  // of a stage
@@ -352,9 +384,10 @@ __device__ __forceinline__ void load_scale_tiles(uint8_t* dst, const uint8_t* ba
 __device__ __forceinline__ int x_column(int row, int column) { return column ^ ((row & 1) << 2); }
 
 constexpr int kRoutingOffset = 2 * kMaxStages * 8;
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr Layout L = layout_up<FMT, NT>();
   constexpr int TILES = stage_tiles(FMT);
   extern __shared__ uint8_t smem_raw[];
@@ -363,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p,
   uint8_t* const xs = scales + p.stages * L.scale_bytes;
   uint64_t* const full = reinterpret_cast<uint64_t*>(xs + p.stages * L.x_bytes);
   uint64_t* const empty = full + kMaxStages;
-  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
+  Routing<NT>& r = *reinterpret_cast<Routing<NT>*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     init_ring(full, empty, p.stages);
@@ -372,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p,
   fence_proxy_async();
   griddep_wait();
   griddep_launch_dependents();
-  route<NT == 1 ? 1 : 4>(p, r, NT * 8);
+  route<NT>(p, r);
 
   const int f_tiles = p.ffn / kTile, items = r.entries * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
   Ring ring = {p.stages, 0, 0u};
@@ -431,70 +464,46 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p,
     }
     drain_ring(full, p.stages, issued);
   } else {
-    // ============================================================ products
-    const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
+    // ============================================================ products: warps 0 to 3 gate rows, 4 to 7 up rows
+    const int fb = warp & 3, is_up = warp >> 2, g = lane >> 2, t = lane & 3;
     float* red = reinterpret_cast<float*>(&r + 1);  // [fb][value][lane]
-    const uint8_t* const w_at = smem + (fb * 16 + g) * 128 + t * 4;
-    const uint8_t* const x_at = xs + g * (kStageK * 2) + kh * 256 + t * 16;
-    const uint8_t* const s_at = scales + kh * (TILES / 2) * 512;
-    int off[4], xoff[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      off[i] = ((kh * 4 + i) ^ g) << 4;
-      xoff[i] = (i ^ (g & 1)) * 64;
-    }
+    const Walk<FMT, NT> walk(g);
+    const uint8_t* const w_at = smem + is_up * kBox + (fb * 16 + g) * 128 + t * 4;
+    const uint8_t* const x_at = xs + g * (kStageK * 2) + t * 16;
     bool ok = true;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
       const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
       const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
-      float gate[NT][4], up[NT][4];
+      float acc[NT][4];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gate[j][i] = up[j][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
       // this lane's words in the scale tiles of its rows
-      const int sg = (int)scale_word((f0 & 127) + fb * 16 + g, 0, 1), su = TILES * 512 + (int)scale_word(((p.ffn + f0) & 127) + fb * 16 + g, 0, 1);
+      const uint8_t* const s_at = scales + is_up * TILES * 512 + (int)scale_word(((is_up ? p.ffn + f0 : f0) & 127) + fb * 16 + g, 0, 1);
       for (int c = 0; c < chunks; ++c) {
         if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
-        const uint8_t* w = w_at + ring.s * L.code_bytes;
-        const uint8_t* x0 = x_at + ring.s * L.x_bytes;
-        Scales<FMT> qg, qu;
-        qg.take(s_at + ring.s * L.scale_bytes + sg, t);
-        qu.take(s_at + ring.s * L.scale_bytes + su, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 x[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const uint4*>(x0 + xoff[i] + j * 8 * (kStageK * 2));
-          chunk<FMT, NT>(gate, *reinterpret_cast<const uint32_t*>(w + off[i]), *reinterpret_cast<const uint32_t*>(w + off[i] + 8 * 128), qg,
-                         i, x, tiles);
-          chunk<FMT, NT>(up, *reinterpret_cast<const uint32_t*>(w + off[i] + kBox),
-                         *reinterpret_cast<const uint32_t*>(w + off[i] + kBox + 8 * 128), qu, i, x, tiles);
-        }
+        walk.stage(acc, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s_at + ring.s * L.scale_bytes, t, tiles);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[ring.s]);
         ring.next();
       }
-      // the halves of k meet; rows g, g + 8 of columns 2t, 2t + 1
+      // gate and up meet; rows g, g + 8 of columns 2t, 2t + 1
       if (!ok) r.failed = 1;
-      if (kh == 1) {
+      if (is_up) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            red[((fb * NT + j) * 8 + i) * 32 + lane] = gate[j][i];
-            red[((fb * NT + j) * 8 + 4 + i) * 32 + lane] = up[j][i];
-          }
+          for (int i = 0; i < 4; ++i) red[((fb * NT + j) * 4 + i) * 32 + lane] = acc[j][i];
       }
       consumers_sync();
-      if (kh == 0 && r.failed == 0) {
+      if (!is_up && r.failed == 0) {
         const float ts = p.ts1 ? p.ts1[e] : 1.0f;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float gv = (gate[j][i] + red[((fb * NT + j) * 8 + i) * 32 + lane]) * ts;
-            const float uv = (up[j][i] + red[((fb * NT + j) * 8 + 4 + i) * 32 + lane]) * ts;
+            const float gv = acc[j][i] * ts, uv = red[((fb * NT + j) * 4 + i) * 32 + lane] * ts;
             const int row = j * 8 + 2 * t + (i & 1), f = f0 + fb * 16 + g + (i >> 1) * 8;
             // (h is rounded to fp16: it is the next product's operand, 2^-11 of itself at most, the error of its sum is
             // below that of the output's own rounding)
@@ -507,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_up_kernel(const Params p,
 }
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr Layout L = layout_down<FMT, NT>();
   constexpr int TILES = stage_tiles(FMT), kUnitK = 2 * kStageK;
   extern __shared__ uint8_t smem_raw[];
@@ -516,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
   uint8_t* const xs = scales + p.stages * L.scale_bytes;
   uint64_t* const full = reinterpret_cast<uint64_t*>(xs + p.stages * L.x_bytes);
   uint64_t* const empty = full + kMaxStages;
-  Routing& r = *reinterpret_cast<Routing*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
+  Routing<NT>& r = *reinterpret_cast<Routing<NT>*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
   float* sums = reinterpret_cast<float*>(&r + 1);  // [half of k][token][64 columns]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.cluster) * kTile;
@@ -528,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
   fence_proxy_async();
   // The logits and the weights are older than the kernel before this one, which let this one start only after its own wait
   // (the logits are read past L1, which may hold what was there before them).
-  route<NT == 1 ? 1 : 4>(p, r, NT * 8);
+  route<NT>(p, r);
 
   const int per = (p.ffn + kUnitK - 1) / kUnitK, units = r.entries * per;
   const int u0 = (int)((int64_t)units * rank / p.cluster), u1 = (int)((int64_t)units * (rank + 1) / p.cluster);
@@ -587,11 +596,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
     const uint8_t* const w_at = smem + kh * kBox + (fb * 16 + g) * 128 + t * 4;
     const uint8_t* const x_at = xs + (kh * NT * 8 + g) * (kStageK * 2) + t * 16;
     const uint8_t* const s_at = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g, 0, 1);
-    int off[8], xoff[2];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) off[i] = (i ^ g) << 4;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) xoff[i] = (i ^ (g & 1)) * 64;
+    const Walk<FMT, NT> walk(g);
     bool ok = true;
     float acc[NT][4];
     for (int u = u0; u < u1; ++u) {
@@ -604,22 +609,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
           for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
       }
       if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
-      const uint8_t* w = w_at + ring.s * L.code_bytes;
-      const uint8_t* x0 = x_at + ring.s * L.x_bytes;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        Scales<FMT> qd;
-        qd.take(s_at + ring.s * L.scale_bytes + q * (TILES / 2) * 512, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 x[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            x[j] = *reinterpret_cast<const uint4*>(x0 + xoff[i & 1] + q * 256 + (i >> 1) * 128 + j * 8 * (kStageK * 2));
-          chunk<FMT, NT>(acc, *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i]),
-                         *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i] + 8 * 128), qd, i, x, tiles);
-        }
-      }
+      walk.stage(acc, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s_at + ring.s * L.scale_bytes, t, tiles);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[ring.s]);
       ring.next();
@@ -671,8 +661,9 @@ __global__ void __launch_bounds__(kThreads, 2) moe_fp4_down_kernel(const Params 
 constexpr int kMaxDevices = 64;
 std::atomic<bool> g_launched[kMaxDevices];  // devices whose status word a wait may have set
 
+template <int NT>
 size_t smem_bytes(const Layout& l, int stages, size_t extra) {
-  return 1024 + (size_t)stages * stage_total(l) + kRoutingOffset + sizeof(Routing) + extra;
+  return 1024 + (size_t)stages * stage_total(l) + kRoutingOffset + sizeof(Routing<NT>) + extra;
 }
 
 template <int FMT, int NT>
@@ -687,24 +678,24 @@ int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t 
     RB200_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     configured_device = dev;
   }
-  const int ctas = 2 * sm_count_current();
-  const size_t room = (size_t)113 * 1024;  // two CTAs an SM
+  const int ctas = ctas_per_sm(NT) * sm_count_current();
+  const size_t room = (size_t)(NT == 1 ? 75 : 113) * 1024;  // so that they fit an SM's 228 KB, 1 KB more each
   const int rows = p.tokens * p.top_k;
 
-  const size_t red = (size_t)4 * NT * 8 * 32 * 4;
+  const size_t red = (size_t)4 * NT * 4 * 32 * 4;
   p.stages = kMaxStages;
-  while (p.stages > 2 && smem_bytes(layout_up<FMT, NT>(), p.stages, red) > room) --p.stages;
+  while (p.stages > 2 && smem_bytes<NT>(layout_up<FMT, NT>(), p.stages, red) > room) --p.stages;
   const int64_t items = (int64_t)rows * (p.ffn / kTile);  // at most
   RB200_CUDA(launch_dependent(up, dim3((unsigned)(items < ctas ? items : ctas)), kThreads,
-                              smem_bytes(layout_up<FMT, NT>(), p.stages, red), stream, p, t1));
+                              smem_bytes<NT>(layout_up<FMT, NT>(), p.stages, red), stream, p, t1));
 
   const size_t sums = (size_t)2 * p.tokens * kTile * 4;
   p.stages = kMaxStages;
-  while (p.stages > 2 && smem_bytes(layout_down<FMT, NT>(), p.stages, sums) > room) --p.stages;
+  while (p.stages > 2 && smem_bytes<NT>(layout_down<FMT, NT>(), p.stages, sums) > room) --p.stages;
   const int n_tiles = p.hidden / kTile, per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes(layout_down<FMT, NT>(), p.stages, sums);
+  cfg.dynamicSmemBytes = smem_bytes<NT>(layout_down<FMT, NT>(), p.stages, sums);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
