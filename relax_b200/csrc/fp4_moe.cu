@@ -32,7 +32,7 @@ using ug::elect_one;
 constexpr int kMaxTokens = 32, kMaxExperts = 256, kMaxTopK = 8;
 constexpr int kConsumers = 8;  // warps: four blocks of 16 rows, gate and up or two halves of k
 constexpr int kThreads = (kConsumers + 2) * 32;  // and a warp for the weights' loads, one for x's
-constexpr int kTile = 64;      // rows of a weight box
+constexpr int kTile = 64;      // rows of a weight box: four 16-row blocks, inside one tile of scales
 constexpr int kBox = kTile * 128;
 constexpr int kMaxStages = 6;
 
@@ -48,6 +48,7 @@ struct alignas(16) Routing {
   int warp_sum[kConsumers];
   int entries;
   int failed;
+  uint16_t first_row[kMaxExperts];  // of an expert
   uint16_t entry_row[kRows + 2];
   uint8_t entry_expert[kRows];
   uint8_t token_of_row[kRows];
@@ -75,112 +76,92 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return v == v ? ((b & 0x80000000u) ? ~b : b | 0x80000000u) : 0u;
 }
 
-// U tokens (t, t + 8, ..) by a warp, side by side: what takes the time is the latency of each step.  PER experts a lane.
-template <int U, int PER, int NT>
+// order_key's inverse (NaN for 0)
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return k == 0u ? __uint_as_float(0x7fffffffu) : __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
+
+// A token by a warp, PER experts a lane.  Loops stay loops: the kernel's instructions are not in the caches when it starts, so
+// what is executed once costs its fetch (29 tokens, 64 experts: 6.6 us unrolled over four tokens, the rounds alone 3).
+template <int PER, int NT>
 __device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, int t) {
   const int lane = threadIdx.x & 31;
-  float v[U][PER], top[U], sum[U], chosen[U], mine[U];
-  uint32_t key[U][PER];
-  int my_expert[U];
+  uint32_t key[PER];  // 0: not there, or taken
+  bool nan = false;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const bool token = t + u * kConsumers < p.tokens;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = i * 32 + lane;
-      v[u][i] = token && e < p.experts ? __ldcg(p.logits + (t + u * kConsumers) * p.experts + e) : -INFINITY;
-    }
+  for (int i = 0; i < PER; ++i) {
+    const int e = i * 32 + lane;
+    const bool there = e < p.experts;
+    const float v = (there ? __ldcg(p.logits + t * p.experts + e) : 0.0f) + 0.0f;  // (-0 is +0 then)
+    nan = nan || v != v;
+    key[i] = there ? max(order_key(v), 1u) : 0u;
   }
+  uint32_t top = 0u;
+  float sum = 0.0f, mine = 0.0f;
+  int my_expert = 0;
+#pragma unroll 1
+  for (int j = 0; j < p.top_k; ++j) {
+    uint32_t best = key[0];
+    int at = lane;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    top[u] = v[u][0];
+    for (int i = 1; i < PER; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i * 32 + lane;
+      }
+    const uint32_t all = __reduce_max_sync(0xffffffffu, best);
+    const int e = (int)__reduce_min_sync(0xffffffffu, best == all ? (uint32_t)at : 0xffffu);
+    if (j == 0) {
+      top = all;
+      if (!p.renormalize) {  // the sum over all experts
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      top[u] = fmaxf(top[u], v[u][i]);
-      key[u][i] = i * 32 + lane < p.experts ? max(order_key(v[u][i]), 1u) : 0u;  // 0: not there, or taken
+        for (int i = 0; i < PER; ++i)
+          if (key[i] != 0u) sum += expf(key_value(key[i]) - key_value(top));
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
     }
-    chosen[u] = mine[u] = 0.0f;
-    my_expert[u] = 0;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int u = 0; u < U; ++u) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    sum[u] = 0.0f;
+    if (lane == j) {
+      mine = expf(key_value(all) - key_value(top));
+      my_expert = e;
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (i * 32 + lane < p.experts) sum[u] += expf(v[u][i] - top[u]);
+      if (i * 32 + lane == e) key[i] = 0u;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
-  for (int j = 0; j < p.top_k; ++j) {
-    uint32_t best[U], all[U];
-    int at[U], e[U];
-    float val[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      best[u] = key[u][0];
-      at[u] = lane;
-      val[u] = v[u][0];
-#pragma unroll
-      for (int i = 1; i < PER; ++i)
-        if (key[u][i] > best[u]) {
-          best[u] = key[u][i];
-          at[u] = i * 32 + lane;
-          val[u] = v[u][i];
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) all[u] = __reduce_max_sync(0xffffffffu, best[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) e[u] = (int)__reduce_min_sync(0xffffffffu, best[u] == all[u] ? (uint32_t)at[u] : 0xffffu);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float w = expf(__shfl_sync(0xffffffffu, val[u], e[u] & 31) - top[u]);
-      chosen[u] += w;
-      if (lane == j) {
-        mine[u] = w;
-        my_expert[u] = e[u];
-      }
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i * 32 + lane == e[u]) key[u][i] = 0u;
-    }
+  if (p.renormalize) {  // the sum over the chosen ones, in their order
+    sum = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < p.top_k; ++j) sum += __shfl_sync(0xffffffffu, mine, j);
   }
-  // (a NaN among the logits, or nothing but -inf: sum is NaN, and so is every gate)
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int token = t + u * kConsumers;
-    if (token < p.tokens && lane < p.top_k) {
-      r.expert_of[token * p.top_k + lane] = (uint8_t)my_expert[u];
-      r.gate_of[token * p.top_k + lane] = p.renormalize && sum[u] == sum[u] ? mine[u] / chosen[u] : mine[u] / sum[u];
-      atomicOr(&r.mask[my_expert[u]], 1u << token);
-    }
+  // (an infinite maximum: its difference to itself is NaN)
+  nan = __any_sync(0xffffffffu, nan);
+  if (lane < p.top_k) {
+    r.expert_of[t * p.top_k + lane] = (uint8_t)my_expert;
+    r.gate_of[t * p.top_k + lane] = nan ? __uint_as_float(0x7fffffffu) : mine / sum;
+    atomicOr(&r.mask[my_expert], 1u << t);
   }
 }
 
 // The routing, by every thread of the CTA: the top_k largest logits of a token (equal ones: lower expert first), gates
-// softmax over all experts or over the chosen ones; rows and entries in expert order.
+// softmax over all experts or over the chosen ones; rows and entries in expert order.  The entries are there when it
+// returns, the rows' tokens and gates after rows_sync, in which the weights' warp takes no part.
 template <int NT>
-__device__ void route(const Params& p, Routing<NT>& r) {
-  constexpr int U = NT == 1 ? 1 : kMaxTokens / kConsumers, most = NT * 8;
+__device__ __forceinline__ void route(const Params& p, Routing<NT>& r) {
+  constexpr int most = NT * 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < kMaxExperts) r.mask[tid] = 0u;
   __syncthreads();
-  if (warp < kConsumers && warp < p.tokens) {
-    if (p.experts <= 32) choose<U, 1>(p, r, warp);
-    else if (p.experts <= 64) choose<U, 2>(p, r, warp);
-    else choose<U, kMaxExperts / 32>(p, r, warp);
+#pragma unroll 1
+  for (int t = warp; t < p.tokens; t += kThreads / 32) {
+    if (p.experts <= 32) choose<1>(p, r, t);
+    else if (p.experts <= 64) choose<2>(p, r, t);
+    else choose<kMaxExperts / 32>(p, r, t);
   }
   __syncthreads();
-  const uint32_t m = tid < kMaxExperts ? r.mask[tid] : 0u;
-  const int n = __popc(m), parts = (n + most - 1) / most;
+  const int n = tid < kMaxExperts ? __popc(r.mask[tid]) : 0, parts = (n + most - 1) / most;
   int upto = n | parts << 16;  // rows and entries counted together
-#pragma unroll
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
@@ -189,20 +170,14 @@ __device__ void route(const Params& p, Routing<NT>& r) {
   __syncthreads();
   if (warp < kConsumers) {
     int before = upto - (n | parts << 16);
+#pragma unroll 1
     for (int w = 0; w < warp; ++w) before += r.warp_sum[w];
     const int row = before & 0xffff, a = before >> 16;
+    r.first_row[tid] = (uint16_t)row;
+#pragma unroll 1
     for (int i = 0; i < parts; ++i) {
       r.entry_expert[a + i] = (uint8_t)tid;
       r.entry_row[a + i] = (uint16_t)(row + i * most);
-    }
-    uint32_t left = m;
-    for (int i = 0; i < n; ++i, left &= left - 1u) {
-      const int t = __ffs((int)left) - 1;
-      float gate = 0.0f;
-      for (int j = 0; j < p.top_k; ++j)
-        if (r.expert_of[t * p.top_k + j] == tid) gate = r.gate_of[t * p.top_k + j];
-      r.token_of_row[row + i] = (uint8_t)t;
-      r.gate_of_row[row + i] = gate;
     }
     if (tid == kMaxExperts - 1) {
       r.entries = a + parts;
@@ -210,6 +185,15 @@ __device__ void route(const Params& p, Routing<NT>& r) {
     }
   }
   __syncthreads();
+  if (tid < p.tokens * p.top_k) {
+    const int e = r.expert_of[tid], t = tid / p.top_k, row = r.first_row[e] + __popc(r.mask[e] & ((1u << t) - 1u));
+    r.token_of_row[row] = (uint8_t)t;
+    r.gate_of_row[row] = r.gate_of[tid];
+  }
+}
+__device__ __forceinline__ void rows_sync() {
+  if ((threadIdx.x >> 5) == kConsumers) asm volatile("bar.arrive 2, %0;" ::"n"(kThreads) : "memory");
+  else asm volatile("bar.sync 2, %0;" ::"n"(kThreads) : "memory");
 }
 
 // 16 bytes of global memory, or zeros
@@ -232,29 +216,31 @@ __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+// Four 8 x 16-byte matrices: lane i names row i % 8 of matrix i / 8, and lane (g, t) gets word t of row g of each.
+__device__ __forceinline__ void load_matrices(uint32_t (&v)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(at)
+               : "memory");
 }
 
 // The scales of rows g and g + 8 over 128 k, as the products take them.
 template <int FMT>
 struct Scales {
-  // kMx: fp32 scales of the four blocks of either row.  kNv: f16x2, this lane's scale of row g and of row g + 8, by chunk
+  // kMx: fp32 scales of the four blocks of either row.  kNv: this lane's scales of row g (low half) and of row g + 8, by chunk
   float f0[4], f8[4];
   uint32_t both[4];
-  __device__ __forceinline__ void take(const uint8_t* at, int t) {  // `at`: row g's word in the (first) tile
+  __device__ __forceinline__ void take(const uint8_t* at0, const uint8_t* at8, int t) {  // their words in the (first) tile
     if (FMT == kMx) {
-      expand(*reinterpret_cast<const uint32_t*>(at), f0);
-      expand(*reinterpret_cast<const uint32_t*>(at + 8 * 16), f8);
+      expand(*reinterpret_cast<const uint32_t*>(at0), f0);
+      expand(*reinterpret_cast<const uint32_t*>(at8), f8);
     } else {
       // blocks 2i and 2i + 1 of chunk i; lanes t < 2 hold k of the first, the others of the second
       const uint32_t sel = t < 2 ? 0x40u : 0x51u;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const uint32_t a = *reinterpret_cast<const uint32_t*>(at + q * 512) & 0x7f7f7f7fu;
-        const uint32_t b = *reinterpret_cast<const uint32_t*>(at + q * 512 + 8 * 16) & 0x7f7f7f7fu;
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(at0 + q * 512) & 0x7f7f7f7fu;
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(at8 + q * 512) & 0x7f7f7f7fu;
         both[2 * q] = from_e4m3x2(__byte_perm(a, b, sel));
         both[2 * q + 1] = from_e4m3x2(__byte_perm(a, b, sel + 0x22u));
       }
@@ -283,11 +269,13 @@ __device__ __forceinline__ void chunk(float (&acc)[NT][4], uint32_t w0, uint32_t
   from_codes8(w0, a0);
   from_codes8(w8, a8);
   if (FMT == kNv) {
-    const uint32_t p0 = __byte_perm(s.both[i], 0u, 0x1010), p8 = __byte_perm(s.both[i], 0u, 0x3232);
+    const __half2 both = *reinterpret_cast<const __half2*>(&s.both[i]);
+    const __half2 p0 = __low2half2(both), p8 = __high2half2(both);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      a0[q] = mul2(a0[q], p0);
-      a8[q] = mul2(a8[q], p8);
+      __half2 v0 = __hmul2(*reinterpret_cast<const __half2*>(&a0[q]), p0), v8 = __hmul2(*reinterpret_cast<const __half2*>(&a8[q]), p8);
+      a0[q] = *reinterpret_cast<const uint32_t*>(&v0);
+      a8[q] = *reinterpret_cast<const uint32_t*>(&v8);
     }
   }
 #pragma unroll
@@ -308,30 +296,39 @@ __device__ __forceinline__ void chunk(float (&acc)[NT][4], uint32_t w0, uint32_t
   }
 }
 
-// A warp's share of a stage: 16 rows over 256 k, eight chunks of 32.  `w` row g of the block in a box of 128-byte rows, swizzled,
-// at this lane's word; `x` row g of the stage's x at this lane's 16 bytes; `sc` row g's word in the first scale tile.
+// A warp's share of a stage: 16 rows over 256 k, eight chunks of 32.  `w` the block's first row in a box of 128-byte rows,
+// swizzled; `x` row g of the stage's x at this lane's 16 bytes; `s0`, `s8` rows g's and g + 8's words in the first scale tile.
+// kNv adds the chunks to two accumulators in turn: one MMA after the other into one is a chain of 20 clocks a link.
 template <int FMT, int NT>
 struct Walk {
-  int off[8], xoff[2];
-  __device__ __forceinline__ explicit Walk(int g) {
+  static constexpr int kSums = FMT == kNv ? 2 : 1;
+  uint32_t off[4];
+  int xoff[2];
+  __device__ __forceinline__ explicit Walk(int lane) {
+    const int r = lane & 7, m = lane >> 3;  // rows r, r + 8 of chunk 2j, then of chunk 2j + 1
 #pragma unroll
-    for (int i = 0; i < 8; ++i) off[i] = (i ^ g) << 4;
+    for (int j = 0; j < 4; ++j) off[j] = (uint32_t)(((m & 1) * 8 + r) * 128 + (((2 * j + (m >> 1)) ^ r) << 4));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) xoff[i] = (i ^ (g & 1)) * 64;
+    for (int i = 0; i < 2; ++i) xoff[i] = (i ^ ((lane >> 2) & 1)) * 64;
   }
-  __device__ __forceinline__ void stage(float (&acc)[NT][4], const uint8_t* w, const uint8_t* x0, const uint8_t* sc, int t, int tiles) const {
+  __device__ __forceinline__ void stage(float (&acc)[kSums][NT][4], uint32_t w, const uint8_t* x0, const uint8_t* s0, const uint8_t* s8, int t,
+                                        int tiles) const {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       Scales<FMT> s;
-      s.take(sc + q * (stage_tiles(FMT) / 2) * 512, t);
+      s.take(s0 + q * (stage_tiles(FMT) / 2) * 512, s8 + q * (stage_tiles(FMT) / 2) * 512, t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint4 x[NT];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[4];
+        load_matrices(v, w + off[q * 2 + h]);
+        uint4 x[2][NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          x[j] = *reinterpret_cast<const uint4*>(x0 + xoff[i & 1] + q * 256 + (i >> 1) * 128 + j * 8 * (kStageK * 2));
-        chunk<FMT, NT>(acc, *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i]),
-                       *reinterpret_cast<const uint32_t*>(w + off[q * 4 + i] + 8 * 128), s, i, x, tiles);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            x[i][j] = *reinterpret_cast<const uint4*>(x0 + xoff[i] + q * 256 + h * 128 + j * 8 * (kStageK * 2));
+        chunk<FMT, NT>(acc[0], v[0], v[1], s, 2 * h, x[0], tiles);
+        chunk<FMT, NT>(acc[kSums - 1], v[2], v[3], s, 2 * h + 1, x[1], tiles);
       }
     }
   }
@@ -341,13 +338,10 @@ struct Walk {
 struct Layout {
   int code_bytes, scale_bytes, x_bytes;  // of a stage
 };
-template <int FMT, int NT>
-__host__ __device__ constexpr Layout layout_up() {
-  return {2 * kBox, 2 * stage_tiles(FMT) * 512, NT * 8 * kStageK * 2};
-}
-template <int FMT, int NT>
-__host__ __device__ constexpr Layout layout_down() {
-  return {2 * kBox, 2 * stage_tiles(FMT) * 512, NT * 8 * 2 * kStageK * 2};
+// up: boxes of gate and of up, with their scale tiles; down: two boxes of consecutive k, theirs
+template <int FMT, int NT, bool UP>
+__host__ __device__ constexpr Layout layout() {
+  return {2 * kBox, 2 * stage_tiles(FMT) * 512, NT * 8 * (UP ? 1 : 2) * kStageK * 2};
 }
 __host__ __device__ constexpr int stage_total(const Layout& l) { return l.code_bytes + l.scale_bytes + l.x_bytes; }
 
@@ -383,13 +377,40 @@ __device__ __forceinline__ void load_scale_tiles(uint8_t* dst, const uint8_t* ba
 // 16-byte column of x in its row's 512 bytes, so that a quarter-warp's reads (two rows, four columns) meet no bank twice
 __device__ __forceinline__ int x_column(int row, int column) { return column ^ ((row & 1) << 2); }
 
+// Rows src + i * pitch elements (or, with tokens, src + token * pitch) of 256 k into a stage's x, 16 bytes a lane.
+__device__ __forceinline__ void copy_rows(uint32_t dst, const __half* src, int64_t pitch, const uint8_t* tokens, int rows, bool there) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 2
+  for (int i = 0; i < rows; ++i)
+    cp_async16(dst + i * (kStageK * 2) + x_column(i, lane) * 16, src + (tokens ? tokens[i] : i) * pitch, there);
+}
+
+template <int S, int NT>
+__device__ __forceinline__ void zero(float (&sum)[S][NT][4]) {
+#pragma unroll
+  for (int q = 0; q < S; ++q)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[q][j][i] = 0.0f;
+}
+template <int S, int NT>
+__device__ __forceinline__ void join(float (&sum)[S][NT][4]) {  // all into the first
+#pragma unroll
+  for (int q = 1; q < S; ++q)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[0][j][i] += sum[q][j][i];
+}
+
 constexpr int kRoutingOffset = 2 * kMaxStages * 8;
-__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int kCtasPerSm = 2;
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
-  constexpr Layout L = layout_up<FMT, NT>();
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr int TILES = stage_tiles(FMT);
+  constexpr Layout L = layout<FMT, NT, true>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* const scales = smem + p.stages * L.code_bytes;
@@ -399,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(c
   Routing<NT>& r = *reinterpret_cast<Routing<NT>*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
+    tma_prefetch_map(&tmap_w);
     init_ring(full, empty, p.stages);
     r.failed = 0;
   }
@@ -406,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(c
   griddep_wait();
   griddep_launch_dependents();
   route<NT>(p, r);
+  rows_sync();
 
   const int f_tiles = p.ffn / kTile, items = r.entries * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
   Ring ring = {p.stages, 0, 0u};
@@ -444,19 +467,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(c
     bool ok = true;
     for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
       const int a = item / f_tiles, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
-      const __half* src[NT * 8];
-#pragma unroll
-      for (int i = 0; i < NT * 8; ++i) src[i] = p.x + (int64_t)r.token_of_row[row0 + min(i, rows - 1)] * p.hidden + lane * 8;
       for (int c = 0; c < chunks; ++c) {
         ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int k = c * kStageK;
-        const bool there = k + lane * 8 < p.hidden;
-        const uint32_t dst = smem_u32(xs + ring.s * L.x_bytes);
-#pragma unroll
-        for (int i = 0; i < NT * 8; ++i)
-          if (i < rows) cp_async16(dst + i * (kStageK * 2) + x_column(i, lane) * 16, there ? src[i] + k : p.x, there);
+        const int k = c * kStageK + lane * 8;
+        const bool there = k < p.hidden;
+        copy_rows(smem_u32(xs + ring.s * L.x_bytes), p.x + (there ? k : 0), p.hidden, r.token_of_row + row0, rows, there);
         cp_async_arrive(&full[ring.s]);
         ++issued;
         ring.next();
@@ -467,27 +484,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(c
     // ============================================================ products: warps 0 to 3 gate rows, 4 to 7 up rows
     const int fb = warp & 3, is_up = warp >> 2, g = lane >> 2, t = lane & 3;
     float* red = reinterpret_cast<float*>(&r + 1);  // [fb][value][lane]
-    const Walk<FMT, NT> walk(g);
-    const uint8_t* const w_at = smem + is_up * kBox + (fb * 16 + g) * 128 + t * 4;
+    const Walk<FMT, NT> walk(lane);
+    constexpr int kSums = Walk<FMT, NT>::kSums;
+    const uint32_t w_at = smem_u32(smem) + is_up * kBox + fb * 16 * 128;
     const uint8_t* const x_at = xs + g * (kStageK * 2) + t * 16;
     bool ok = true;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
       const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
       const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
-      float acc[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+      float sum[kSums][NT][4];
+      zero(sum);
       // this lane's words in the scale tiles of its rows
-      const uint8_t* const s_at = scales + is_up * TILES * 512 + (int)scale_word(((is_up ? p.ffn + f0 : f0) & 127) + fb * 16 + g, 0, 1);
+      const uint8_t* const s0 = scales + is_up * TILES * 512 + (int)scale_word(((is_up ? p.ffn + f0 : f0) & 127) + fb * 16 + g, 0, 1);
+      const uint8_t* const s8 = scales + is_up * TILES * 512 + (int)scale_word(((is_up ? p.ffn + f0 : f0) & 127) + fb * 16 + g + 8, 0, 1);
       for (int c = 0; c < chunks; ++c) {
         if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
-        walk.stage(acc, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s_at + ring.s * L.scale_bytes, t, tiles);
+        walk.stage(sum, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s0 + ring.s * L.scale_bytes, s8 + ring.s * L.scale_bytes, t,
+                   tiles);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[ring.s]);
         ring.next();
       }
+      float(&acc)[NT][4] = sum[0];
+      join(sum);
       // gate and up meet; rows g, g + 8 of columns 2t, 2t + 1
       if (!ok) r.failed = 1;
       if (is_up) {
@@ -516,9 +535,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_up_kernel(c
 }
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
-  constexpr Layout L = layout_down<FMT, NT>();
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr int TILES = stage_tiles(FMT), kUnitK = 2 * kStageK;
+  constexpr Layout L = layout<FMT, NT, false>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* const scales = smem + p.stages * L.code_bytes;
@@ -530,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.cluster) * kTile;
   if (tid == 0) {
+    tma_prefetch_map(&tmap_w);
     init_ring(full, empty, p.stages);
     r.failed = 0;
   }
@@ -538,6 +558,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel
   // The logits and the weights are older than the kernel before this one, which let this one start only after its own wait
   // (the logits are read past L1, which may hold what was there before them).
   route<NT>(p, r);
+  rows_sync();
 
   const int per = (p.ffn + kUnitK - 1) / kUnitK, units = r.entries * per;
   const int u0 = (int)((int64_t)units * rank / p.cluster), u1 = (int)((int64_t)units * (rank + 1) / p.cluster);
@@ -575,15 +596,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const int a = u / per, c = u - a * per, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
-      const uint32_t dst = smem_u32(xs + ring.s * L.x_bytes);
-#pragma unroll
+#pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int k = c * kUnitK + half * kStageK + lane * 8;
         const bool there = k < p.ffn;
-        const __half* src = p.h + (int64_t)row0 * p.ffn + (there ? k : 0);
-#pragma unroll
-        for (int i = 0; i < NT * 8; ++i)
-          if (i < rows) cp_async16(dst + (half * NT * 8 + i) * (kStageK * 2) + x_column(i, lane) * 16, src + (int64_t)i * p.ffn, there);
+        copy_rows(smem_u32(xs + ring.s * L.x_bytes) + half * (NT * 8 * kStageK * 2), p.h + (int64_t)row0 * p.ffn + (there ? k : 0), p.ffn,
+                  nullptr, rows, there);
       }
       cp_async_arrive(&full[ring.s]);
       ++issued;
@@ -593,28 +611,28 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel
   } else {
     // ============================================================ products
     const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
-    const uint8_t* const w_at = smem + kh * kBox + (fb * 16 + g) * 128 + t * 4;
+    const uint32_t w_at = smem_u32(smem) + kh * kBox + fb * 16 * 128;
     const uint8_t* const x_at = xs + (kh * NT * 8 + g) * (kStageK * 2) + t * 16;
-    const uint8_t* const s_at = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g, 0, 1);
-    const Walk<FMT, NT> walk(g);
+    const uint8_t* const s0 = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g, 0, 1);
+    const uint8_t* const s8 = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g + 8, 0, 1);
+    const Walk<FMT, NT> walk(lane);
+    constexpr int kSums = Walk<FMT, NT>::kSums;
     bool ok = true;
-    float acc[NT][4];
+    float sum[kSums][NT][4];
+    float(&acc)[NT][4] = sum[0];
     for (int u = u0; u < u1; ++u) {
       const int a = u / per, c = u - a * per;
       const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
-      if (u == u0 || c == 0) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-      }
+      if (u == u0 || c == 0) zero(sum);
       if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
-      walk.stage(acc, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s_at + ring.s * L.scale_bytes, t, tiles);
+      walk.stage(sum, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s0 + ring.s * L.scale_bytes, s8 + ring.s * L.scale_bytes, t,
+                 tiles);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[ring.s]);
       ring.next();
       if (u + 1 == u1 || c + 1 == per) {
-        // this entry's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane)
+        join(sum);
+        // this entry's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane at a time)
         const float ts = p.ts2 ? p.ts2[r.entry_expert[a]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -638,20 +656,20 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) moe_fp4_down_kernel
   cluster_sync();
   if (r.failed == 0) {
     // four columns of a token a thread
-    const int quads = p.tokens * (kTile / 4);
-    for (int i = rank * kThreads + tid; i < quads; i += p.cluster * kThreads) {
+    constexpr int quads = kTile / 4;
+    for (int i = rank * kThreads + tid; i < p.tokens * quads; i += p.cluster * kThreads) {
+      const int token = i / quads, column = (i - token * quads) * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int q = 0; q < p.cluster; ++q)
         for (int half = 0; half < 2; ++half) {
-          const float4 o = ld_cluster4(at_rank(smem_u32(sums + half * p.tokens * kTile + i * 4), q));
+          const float4 o = ld_cluster4(at_rank(smem_u32(sums + (half * p.tokens + token) * kTile + column), q));
           v.x += o.x;
           v.y += o.y;
           v.z += o.z;
           v.w += o.w;
         }
       const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
-      const int token = i / (kTile / 4), n = n0 + (i % (kTile / 4)) * 4;
-      *reinterpret_cast<uint2*>(p.out + (int64_t)token * p.hidden + n) =
+      *reinterpret_cast<uint2*>(p.out + (int64_t)token * p.hidden + n0 + column) =
           make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
   }
@@ -666,36 +684,26 @@ size_t smem_bytes(const Layout& l, int stages, size_t extra) {
   return 1024 + (size_t)stages * stage_total(l) + kRoutingOffset + sizeof(Routing<NT>) + extra;
 }
 
+struct Weights {
+  const void* up;
+  const void* down;
+};
+
+int weight_map(CUtensorMap* map, const void* w, int64_t rows, int64_t k) {
+  return make_tensor_map_2d(map, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)k / 2, (unsigned long long)rows,
+                            (unsigned long long)k / 2, 128, kTile, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
 template <int FMT, int NT>
-int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t stream) {
+int launch(Params p, const Weights& w, cudaStream_t stream) {
   auto up = moe_fp4_up_kernel<FMT, NT>;
   auto down = moe_fp4_down_kernel<FMT, NT>;
-  static thread_local int configured_device = -1;
-  int dev = 0;
-  RB200_CUDA(cudaGetDevice(&dev));
-  if (configured_device != dev) {
-    RB200_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    RB200_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    configured_device = dev;
-  }
-  const int ctas = ctas_per_sm(NT) * sm_count_current();
-  const size_t room = (size_t)(NT == 1 ? 75 : 113) * 1024;  // so that they fit an SM's 228 KB, 1 KB more each
-  const int rows = p.tokens * p.top_k;
-
-  const size_t red = (size_t)4 * NT * 4 * 32 * 4;
-  p.stages = kMaxStages;
-  while (p.stages > 2 && smem_bytes<NT>(layout_up<FMT, NT>(), p.stages, red) > room) --p.stages;
-  const int64_t items = (int64_t)rows * (p.ffn / kTile);  // at most
-  RB200_CUDA(launch_dependent(up, dim3((unsigned)(items < ctas ? items : ctas)), kThreads,
-                              smem_bytes<NT>(layout_up<FMT, NT>(), p.stages, red), stream, p, t1));
-
-  const size_t sums = (size_t)2 * p.tokens * kTile * 4;
-  p.stages = kMaxStages;
-  while (p.stages > 2 && smem_bytes<NT>(layout_down<FMT, NT>(), p.stages, sums) > room) --p.stages;
-  const int n_tiles = p.hidden / kTile, per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK);
+  const int sms = sm_count_current(), ctas = kCtasPerSm * sms;
+  const size_t room = (size_t)113 * 1024;  // so that two fit an SM's 228 KB, 1 KB more each
+  const size_t red = (size_t)4 * NT * 4 * 32 * 4, sums = (size_t)2 * p.tokens * kTile * 4;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes<NT>(layout_down<FMT, NT>(), p.stages, sums);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -703,35 +711,53 @@ int launch(Params p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  // Clusters do not fill the SMs evenly, so how many of each size run at a time is asked for (once: the sums' share of
-  // shared memory at its largest, which changes no stage count).  Time goes with waves / size.
-  static thread_local int places_device = -1, places[9];
-  if (places_device != dev) {
-    cfg.numAttrs = 1;
+  static thread_local int configured_device = -1, places[9];
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    RB200_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    RB200_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    // clusters do not fill the SMs evenly: how many of each size run at a time
     cudaLaunchConfig_t ask = cfg;
+    ask.numAttrs = 1;
     ask.dynamicSmemBytes = room;
     for (int c = 1; c <= 8; ++c) {
       attr[0].val.clusterDim.x = (unsigned)c;
       ask.gridDim = dim3((unsigned)(ctas / c * c), 1, 1);
       RB200_CUDA(cudaOccupancyMaxActiveClusters(&places[c], down, &ask));
     }
-    places_device = dev;
+    configured_device = dev;
   }
+
+  Layout l = layout<FMT, NT, true>();
+  p.stages = kMaxStages;
+  while (p.stages > 2 && smem_bytes<NT>(l, p.stages, red) > room) --p.stages;
+  CUtensorMap map;
+  if (weight_map(&map, w.up, (int64_t)p.experts * 2 * p.ffn, p.hidden) != 0) return -1;
+  const int64_t most = (int64_t)p.tokens * p.top_k * (p.ffn / kTile);
+  RB200_CUDA(launch_dependent(up, dim3((unsigned)(most < ctas ? most : ctas)), kThreads, smem_bytes<NT>(l, p.stages, red), stream, p, map));
+
+  // down: as large a cluster as leaves room for all of them at a time (a token's experts are top_k different ones).  An eighth
+  // less than the query says: 103 clusters of four and 32 of eight, which it had room for, ran one after the others.
+  const int per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK), n_tiles = p.hidden / kTile;
   p.cluster = 1;
-  for (int c = 2; c <= 8 && c <= p.top_k * per; ++c) {  // (a token's experts are top_k different ones)
-    auto waves = [&](int size) { return places[size] < 1 ? 1 << 20 : (n_tiles + places[size] - 1) / places[size]; };
-    if (waves(c) * p.cluster < waves(p.cluster) * c) p.cluster = c;
-  }
+  for (int c = 2; c <= 8 && c <= p.top_k * per; ++c)
+    if (n_tiles <= places[c] - places[c] / 8) p.cluster = c;
+  l = layout<FMT, NT, false>();
+  p.stages = kMaxStages;
+  while (p.stages > 2 && smem_bytes<NT>(l, p.stages, sums) > room) --p.stages;
+  if (weight_map(&map, w.down, (int64_t)p.experts * p.hidden, p.ffn) != 0) return -1;
   cfg.gridDim = dim3((unsigned)(n_tiles * p.cluster), 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes<NT>(l, p.stages, sums);
   attr[0].val.clusterDim.x = (unsigned)p.cluster;
   cfg.numAttrs = 2;
-  RB200_CUDA(cudaLaunchKernelEx(&cfg, down, p, t2));
+  RB200_CUDA(cudaLaunchKernelEx(&cfg, down, p, map));
   return 0;
 }
 
 template <int FMT>
-int launch_fmt(const Params& p, const CUtensorMap& t1, const CUtensorMap& t2, cudaStream_t stream) {
-  return p.tokens <= 8 ? launch<FMT, 1>(p, t1, t2, stream) : launch<FMT, 2>(p, t1, t2, stream);
+int launch_fmt(const Params& p, const Weights& w, cudaStream_t stream) {
+  return p.tokens <= 8 ? launch<FMT, 1>(p, w, stream) : launch<FMT, 2>(p, w, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -805,19 +831,12 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   p.ffn = (int)d->ffn;
   p.k_tiles1 = (int)f4::scale_k_tiles(d->hidden, d->format);
   p.k_tiles2 = (int)f4::scale_k_tiles(d->ffn, d->format);
-  CUtensorMap t1, t2;
-  if (make_tensor_map_2d(&t1, d->w_gate_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d->hidden / 2,
-                         (unsigned long long)(d->num_experts * 2 * d->ffn), (unsigned long long)d->hidden / 2, 128, f4::kTile,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0 ||
-      make_tensor_map_2d(&t2, d->w_down, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d->ffn / 2,
-                         (unsigned long long)(d->num_experts * d->hidden), (unsigned long long)d->ffn / 2, 128, f4::kTile,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0)
-    return -1;
+  const f4::Weights w = {d->w_gate_up, d->w_down};
   int dev = 0;
   RB200_CUDA(cudaGetDevice(&dev));
   if (dev >= 0 && dev < f4::kMaxDevices) f4::g_launched[dev].store(true, std::memory_order_relaxed);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return d->format == f4::kMx ? f4::launch_fmt<f4::kMx>(p, t1, t2, s) : f4::launch_fmt<f4::kNv>(p, t1, t2, s);
+  return d->format == f4::kMx ? f4::launch_fmt<f4::kMx>(p, w, s) : f4::launch_fmt<f4::kNv>(p, w, s);
 }
 
 }  // extern "C"

@@ -73,6 +73,9 @@ CASES = [  # tokens, hidden, ffn, experts, top_k
     (1, 64, 64, 1, 1), (1, 128, 64, 2, 1), (1, 256, 128, 4, 2), (2, 320, 192, 3, 3), (3, 64, 1088, 8, 2), (5, 576, 64, 5, 4),
     (7, 448, 320, 33, 6), (8, 512, 512, 8, 2), (8, 192, 832, 256, 8), (9, 256, 256, 4, 2), (13, 640, 384, 16, 8), (16, 128, 128, 2, 2),
     (17, 256, 192, 3, 1), (29, 384, 448, 64, 6), (32, 256, 320, 1, 1), (32, 512, 256, 8, 8), (1, 4096, 256, 2, 2), (2, 128, 4160, 3, 2),
+    # boxes of 64, 56, 48, 40 and 32 rows, whose rows lie in two scale tiles or past the matrix
+    (1, 128, 8256, 2, 1), (1, 192, 6976, 2, 1), (1, 64, 5568, 3, 2), (1, 128, 3648, 4, 3), (8, 4160, 128, 3, 3), (9, 2880, 192, 4, 2),
+    (4, 3584, 64, 2, 2), (20, 4096, 64, 2, 1), (1, 7168, 64, 2, 1),
 ]
 
 
@@ -106,6 +109,7 @@ def test_equal_logits_go_to_the_lower_expert():
     logits[2, 39] = 3.0
     logits[3] = float("-inf")
     logits[3, 33], logits[3, 2] = -1.0, -1.0
+    logits[0, 0::2] = -0.0
     got = ops.moe_layer_fp4(x, logits, *w, 3, "mx", *t)
     ref_logits = logits.double().cpu().numpy()
     _check(got, *_layer(x.double().cpu().numpy(), ref_logits, 3, False, *v))
