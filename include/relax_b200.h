@@ -394,7 +394,7 @@ RB200_API int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb
  * x and out fp16 [tokens, hidden], logits fp32 [tokens, num_experts]; w_gate_up codes [num_experts, 2 ffn, hidden / 2], gate
  * rows first; w_down codes [num_experts, hidden, ffn / 2]; scales of each expert in tiles, experts after one another;
  * tensor scales [num_experts] (nv only; NULL: 1).  hidden and ffn multiples of 64, num_experts <= 256, top_k <= 8.
- * workspace: rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, ffn) bytes, of the call's own until it has run.
+ * workspace: rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, hidden, ffn) bytes, of the call's own until it has run.
  * The weights, scales and logits must not be written between this call and its end.
  * Takes the place of rb200_moe_route, rb200_moe_gather, two grouped matmuls and rb200_moe_combine.
  */
@@ -414,7 +414,7 @@ typedef struct rb200_moe_layer_fp4_desc {
   int32_t renormalize;
   int32_t reserved;
 } rb200_moe_layer_fp4_desc;
-RB200_API size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t ffn);
+RB200_API size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn);
 RB200_API int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ low-latency all-reduce */

@@ -13,9 +13,9 @@
 // Weights come by tensor-map loads in 128-byte rows, swizzled; a lane's code words are then free of bank conflicts.  A
 // warp's lane (g, t) holds, of the 32 k of a chunk, k 8t .. 8t + 7 of rows g and g + 8: the MMAs' k slots are a permutation
 // of k, the same one for x, whose eight values are one 16-byte word.
-// `down` cuts the (expert, k) sequence of 64 output columns over the CTAs of a cluster; each adds gate times its sums in
-// shared memory, every word by one thread in the order of the sequence, and the cluster's parts are added in rank order:
-// nothing depends on timing.
+// `down` cuts the sequence of (64 output columns, entry, 512 k) evenly over the CTAs.  Each adds gate times its sums in shared
+// memory, every word by one thread at a time in the order of the sequence; what it has of a column tile that is not its own
+// alone goes to the workspace, and the last CTA to come adds the parts up in the order of the CTAs: nothing depends on timing.
 #include <atomic>
 #include <cstring>
 
@@ -35,6 +35,7 @@ constexpr int kThreads = (kConsumers + 2) * 32;  // and a warp for the weights' 
 constexpr int kTile = 64;      // rows of a weight box: four 16-row blocks, inside one tile of scales
 constexpr int kBox = kTile * 128;
 constexpr int kMaxStages = 6;
+constexpr int kMaxCtas = 512;  // that the workspace has room for
 
 __device__ int g_status;
 
@@ -48,6 +49,7 @@ struct alignas(16) Routing {
   int warp_sum[kConsumers];
   int entries;
   int failed;
+  uint32_t ticket;
   uint16_t first_row[kMaxExperts];  // of an expert
   uint16_t entry_row[kRows + 2];
   uint8_t entry_expert[kRows];
@@ -67,7 +69,9 @@ struct Params {
   int64_t s1_expert, s2_expert;  // bytes of an expert's scales
   int tokens, experts, top_k, renormalize;
   int hidden, ffn, k_tiles1, k_tiles2;
-  int stages, cluster;
+  int stages;
+  float* parts;       // down: two tiles [tokens][64] a CTA
+  uint32_t* tickets;  // down: a tile's parts that are there
 };
 
 // order of floats as unsigned numbers, NaN lowest
@@ -84,7 +88,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // A token by a warp, PER experts a lane.  Loops stay loops: the kernel's instructions are not in the caches when it starts, so
 // what is executed once costs its fetch (29 tokens, 64 experts: 6.6 us unrolled over four tokens, the rounds alone 3).
 template <int PER, int NT>
-__device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, int t) {
+__device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, const float* logits, int t) {
   const int lane = threadIdx.x & 31;
   uint32_t key[PER];  // 0: not there, or taken
   bool nan = false;
@@ -92,13 +96,14 @@ __device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, int t) {
   for (int i = 0; i < PER; ++i) {
     const int e = i * 32 + lane;
     const bool there = e < p.experts;
-    const float v = (there ? __ldcg(p.logits + t * p.experts + e) : 0.0f) + 0.0f;  // (-0 is +0 then)
+    const float v = (there ? logits[t * p.experts + e] : 0.0f) + 0.0f;  // (-0 is +0 then)
     nan = nan || v != v;
     key[i] = there ? max(order_key(v), 1u) : 0u;
   }
-  uint32_t top = 0u;
-  float sum = 0.0f, mine = 0.0f;
+  uint32_t first[PER], my_key = 0u;
   int my_expert = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) first[i] = key[i];
 #pragma unroll 1
   for (int j = 0; j < p.top_k; ++j) {
     uint32_t best = key[0];
@@ -110,30 +115,29 @@ __device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, int t) {
         at = i * 32 + lane;
       }
     const uint32_t all = __reduce_max_sync(0xffffffffu, best);
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == all ? (uint32_t)at : 0xffffu);
-    if (j == 0) {
-      top = all;
-      if (!p.renormalize) {  // the sum over all experts
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (key[i] != 0u) sum += expf(key_value(key[i]) - key_value(top));
-#pragma unroll 1
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      }
-    }
+    int e;
+    if (PER == 1) e = __ffs((int)__ballot_sync(0xffffffffu, best == all)) - 1;
+    else e = (int)__reduce_min_sync(0xffffffffu, best == all ? (uint32_t)at : 0xffffu);
     if (lane == j) {
-      mine = expf(key_value(all) - key_value(top));
+      my_key = all;
       my_expert = e;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (i * 32 + lane == e) key[i] = 0u;
   }
-  if (p.renormalize) {  // the sum over the chosen ones, in their order
-    sum = 0.0f;
-#pragma unroll 1
-    for (int j = 0; j < p.top_k; ++j) sum += __shfl_sync(0xffffffffu, mine, j);
+  const float top = key_value(__shfl_sync(0xffffffffu, my_key, 0));
+  const float mine = lane < p.top_k ? expf(key_value(my_key) - top) : 0.0f;
+  float sum = 0.0f;
+  if (p.renormalize) {  // over the chosen ones, else over all experts
+    sum = mine;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (first[i] != 0u) sum += expf(key_value(first[i]) - top);
   }
+#pragma unroll 1
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   // (an infinite maximum: its difference to itself is NaN)
   nan = __any_sync(0xffffffffu, nan);
   if (lane < p.top_k) {
@@ -146,18 +150,22 @@ __device__ __forceinline__ void choose(const Params& p, Routing<NT>& r, int t) {
 // The routing, by every thread of the CTA: the top_k largest logits of a token (equal ones: lower expert first), gates
 // softmax over all experts or over the chosen ones; rows and entries in expert order.  The entries are there when it
 // returns, the rows' tokens and gates after rows_sync, in which the weights' warp takes no part.
+// `scratch`: tokens x experts floats, where loads go later.
 template <int NT>
-__device__ __forceinline__ void route(const Params& p, Routing<NT>& r) {
+__device__ __forceinline__ void route(const Params& p, Routing<NT>& r, float* scratch) {
   constexpr int most = NT * 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < kMaxExperts) r.mask[tid] = 0u;
+#pragma unroll 1
+  for (int i = tid; i < p.tokens * p.experts; i += kThreads) scratch[i] = __ldcg(p.logits + i);
   __syncthreads();
 #pragma unroll 1
   for (int t = warp; t < p.tokens; t += kThreads / 32) {
-    if (p.experts <= 32) choose<1>(p, r, t);
-    else if (p.experts <= 64) choose<2>(p, r, t);
-    else choose<kMaxExperts / 32>(p, r, t);
+    if (p.experts <= 32) choose<1>(p, r, scratch, t);
+    else if (p.experts <= 64) choose<2>(p, r, scratch, t);
+    else choose<kMaxExperts / 32>(p, r, scratch, t);
   }
+  fence_proxy_async();  // bulk copies write the scratch next
   __syncthreads();
   const int n = tid < kMaxExperts ? __popc(r.mask[tid]) : 0, parts = (n + most - 1) / most;
   int upto = n | parts << 16;  // rows and entries counted together
@@ -427,7 +435,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
   fence_proxy_async();
   griddep_wait();
   griddep_launch_dependents();
-  route<NT>(p, r);
+  if (blockIdx.x == 0)
+    for (int i = tid; i < p.hidden / kTile; i += kThreads) p.tickets[i] = 0u;
+  route<NT>(p, r, reinterpret_cast<float*>(smem));
   rows_sync();
 
   const int f_tiles = p.ffn / kTile, items = r.entries * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
@@ -534,6 +544,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
   }
 }
 
+// The sequence of units (64 output columns, entry, 512 k) cut evenly over the CTAs.
+struct Share {
+  int total, ctas, per_tile;  // units, CTAs with some, units of 64 columns
+  __device__ __forceinline__ int begin(int cta) const { return (int)((int64_t)total * cta / ctas); }
+  __device__ __forceinline__ int owner(int unit) const { return (int)(((int64_t)(unit + 1) * ctas - 1) / total); }
+};
+// A unit's place, kept by counting: the divisions took as long as a unit's products.
+struct Place {
+  int tile, a, c, per, entries;
+  __device__ __forceinline__ Place(int unit, int per_, int entries_) : per(per_), entries(entries_) {
+    tile = unit / (per * entries);
+    const int v = unit - tile * (per * entries);
+    a = v / per;
+    c = v - a * per;
+  }
+  __device__ __forceinline__ bool last_of_entry() const { return c + 1 == per; }
+  __device__ __forceinline__ bool last_of_tile() const { return last_of_entry() && a + 1 == entries; }
+  __device__ __forceinline__ void next() {
+    if (++c == per) {
+      c = 0;
+      if (++a == entries) {
+        a = 0;
+        ++tile;
+      }
+    }
+  }
+};
+
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr int TILES = stage_tiles(FMT), kUnitK = 2 * kStageK;
@@ -547,7 +585,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
   Routing<NT>& r = *reinterpret_cast<Routing<NT>*>(reinterpret_cast<uint8_t*>(full) + kRoutingOffset);
   float* sums = reinterpret_cast<float*>(&r + 1);  // [half of k][token][64 columns]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)cluster_rank(), n0 = (int)(blockIdx.x / p.cluster) * kTile;
   if (tid == 0) {
     tma_prefetch_map(&tmap_w);
     init_ring(full, empty, p.stages);
@@ -557,29 +594,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
   fence_proxy_async();
   // The logits and the weights are older than the kernel before this one, which let this one start only after its own wait
   // (the logits are read past L1, which may hold what was there before them).
-  route<NT>(p, r);
+  route<NT>(p, r, reinterpret_cast<float*>(smem));
   rows_sync();
 
-  const int per = (p.ffn + kUnitK - 1) / kUnitK, units = r.entries * per;
-  const int u0 = (int)((int64_t)units * rank / p.cluster), u1 = (int)((int64_t)units * (rank + 1) / p.cluster);
+  const int per = (p.ffn + kUnitK - 1) / kUnitK;
+  Share share;
+  share.per_tile = r.entries * per;
+  share.total = p.hidden / kTile * share.per_tile;
+  share.ctas = min((int)gridDim.x, share.total);
+  const bool any = (int)blockIdx.x < share.ctas;
+  const int u0 = any ? share.begin(blockIdx.x) : 0, u1 = any ? share.begin(blockIdx.x + 1) : 0;
   Ring ring = {p.stages, 0, 0u};
   if (warp == kConsumers) {
     // ============================================================ weights (older than the kernel before, too)
     const bool leader = elect_one();
     int issued = 0;
-    for (int u = u0; u < u1; ++u) {
+    Place at(u0, per, r.entries);
+    for (int u = u0; u < u1; ++u, at.next()) {
       bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (leader) {
-        const int a = u / per, c = u - a * per, e = r.entry_expert[a];
+        const int tile = at.tile, c = at.c, e = r.entry_expert[at.a];
         uint64_t* bar = &full[ring.s];
         uint8_t* w = smem + ring.s * L.code_bytes;
         const bool two = c * kUnitK + kStageK < p.ffn;  // (else the second box keeps what it had: its x is zeros)
         mbar_arrive_expect_tx(bar, (two ? 2 * kBox : kBox) + L.scale_bytes);
-        tma_load(w, &tmap_w, c * 256, e * p.hidden + n0, bar);
-        if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + n0, bar);
-        load_scale_tiles(scales + ring.s * L.scale_bytes, p.s2 + e * p.s2_expert + (int64_t)(n0 >> 7) * p.k_tiles2 * 512, c * 2 * TILES,
+        tma_load(w, &tmap_w, c * 256, e * p.hidden + tile * kTile, bar);
+        if (two) tma_load(w + kBox, &tmap_w, c * 256 + 128, e * p.hidden + tile * kTile, bar);
+        load_scale_tiles(scales + ring.s * L.scale_bytes, p.s2 + e * p.s2_expert + (int64_t)(tile >> 1) * p.k_tiles2 * 512, c * 2 * TILES,
                          2 * TILES, p.k_tiles2 - 1, bar);
       }
       __syncwarp();
@@ -590,12 +633,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
   } else if (warp == kConsumers + 1) {
     // ============================================================ h
     griddep_wait();  // the kernel before's
+    griddep_launch_dependents();
     int issued = 0;
-    for (int u = u0; u < u1; ++u) {
+    Place at(u0, per, r.entries);
+    for (int u = u0; u < u1; ++u, at.next()) {
       bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const int a = u / per, c = u - a * per, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
+      const int c = at.c, row0 = r.entry_row[at.a], rows = r.entry_row[at.a + 1] - row0;
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int k = c * kUnitK + half * kStageK + lane * 8;
@@ -610,70 +655,107 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
     drain_ring(full, p.stages, issued);
   } else {
     // ============================================================ products
+    griddep_wait();  // for what is written below
     const int fb = warp & 3, kh = warp >> 2, g = lane >> 2, t = lane & 3;
     const uint32_t w_at = smem_u32(smem) + kh * kBox + fb * 16 * 128;
     const uint8_t* const x_at = xs + (kh * NT * 8 + g) * (kStageK * 2) + t * 16;
-    const uint8_t* const s0 = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g, 0, 1);
-    const uint8_t* const s8 = scales + kh * TILES * 512 + (int)scale_word((n0 & 127) + fb * 16 + g + 8, 0, 1);
+    const int s_row = (int)scale_word(fb * 16 + g, 0, 1), s_row8 = (int)scale_word(fb * 16 + g + 8, 0, 1);
     const Walk<FMT, NT> walk(lane);
     constexpr int kSums = Walk<FMT, NT>::kSums;
     bool ok = true;
     float sum[kSums][NT][4];
     float(&acc)[NT][4] = sum[0];
-    for (int u = u0; u < u1; ++u) {
-      const int a = u / per, c = u - a * per;
-      const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
-      if (u == u0 || c == 0) zero(sum);
+    int tile_first = u0;  // this CTA's first unit of the tile at hand
+    Place at(u0, per, r.entries);
+    int row0 = 0, rows = 0, tiles = 0;
+    for (int u = u0; u < u1; ++u, at.next()) {
+      const int tile = at.tile;
+      if (u == u0 || at.c == 0) {
+        zero(sum);
+        row0 = r.entry_row[at.a];
+        rows = r.entry_row[at.a + 1] - row0;
+        tiles = (rows + 7) / 8;
+      }
       if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
-      walk.stage(sum, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s0 + ring.s * L.scale_bytes, s8 + ring.s * L.scale_bytes, t,
-                 tiles);
+      const uint8_t* sc = scales + ring.s * L.scale_bytes + kh * TILES * 512 + (tile & 1) * 8;  // rows 64 .. 127 of a scale tile: words 2, 3
+      walk.stage(sum, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, sc + s_row, sc + s_row8, t, tiles);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[ring.s]);
       ring.next();
-      if (u + 1 == u1 || c + 1 == per) {
+      const bool tile_ends = u + 1 == u1 || at.last_of_tile();
+      if (tile_ends || at.last_of_entry()) {
         join(sum);
         // this entry's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane at a time)
-        const float ts = p.ts2 ? p.ts2[r.entry_expert[a]] : 1.0f;
+        const float ts = p.ts2 ? p.ts2[r.entry_expert[at.a]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = j * 8 + 2 * t + (i & 1);
             if (row < rows) {
-              float* at = sums + ((kh * p.tokens + r.token_of_row[row0 + row]) * kTile + fb * 16 + g + (i >> 1) * 8);
-              *at = fmaf(r.gate_of_row[row0 + row] * ts, acc[j][i], *at);
+              float* word = sums + ((kh * p.tokens + r.token_of_row[row0 + row]) * kTile + fb * 16 + g + (i >> 1) * 8);
+              *word = fmaf(r.gate_of_row[row0 + row] * ts, acc[j][i], *word);
             }
           }
         __syncwarp();
       }
-    }
-    if (!ok)
-      for (int q = 0; q < p.cluster; ++q) st_cluster(at_rank(smem_u32(&r.failed), q), 1u);
-  }
-  griddep_wait();
-  griddep_launch_dependents();
-  __syncthreads();
-  cluster_sync();
-  if (r.failed == 0) {
-    // four columns of a token a thread
-    constexpr int quads = kTile / 4;
-    for (int i = rank * kThreads + tid; i < p.tokens * quads; i += p.cluster * kThreads) {
-      const int token = i / quads, column = (i - token * quads) * 4;
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int q = 0; q < p.cluster; ++q)
-        for (int half = 0; half < 2; ++half) {
-          const float4 o = ld_cluster4(at_rank(smem_u32(sums + (half * p.tokens + token) * kTile + column), q));
-          v.x += o.x;
-          v.y += o.y;
-          v.z += o.z;
-          v.w += o.w;
+      if (tile_ends) {
+        if (!ok) r.failed = 1;
+        consumers_sync();
+        // The tile as far as this CTA has it: written as it is if that is all of it, else put with the parts of other CTAs; who
+        // comes last adds them up, in the order of the CTAs.
+        constexpr int quads = kTile / 4;
+        const int first = share.owner(tile * share.per_tile), last = share.owner((tile + 1) * share.per_tile - 1);
+        const bool whole = first == last;
+        const int size = p.tokens * kTile;
+        float* mine = p.parts + (int64_t)(blockIdx.x * 2 + (tile_first == u0 ? 0 : 1)) * size;
+        bool write = whole && r.failed == 0;
+        if (!whole) {
+          for (int i = tid; i < size / 4; i += kConsumers * 32) {
+            const float4 x = reinterpret_cast<const float4*>(sums)[i], y = reinterpret_cast<const float4*>(sums + size)[i];
+            __stcg(reinterpret_cast<float4*>(mine) + i, make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w));
+          }
+          __threadfence();
+          consumers_sync();
+          if (tid == 0) r.ticket = atomicAdd(p.tickets + tile, 1u | (r.failed ? 0x10000u : 0u));
+          consumers_sync();
+          // (every part is there, and none of a CTA whose wait ran out)
+          write = r.ticket == (uint32_t)(last - first) && r.failed == 0;
+          __threadfence();
         }
-      const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
-      *reinterpret_cast<uint2*>(p.out + (int64_t)token * p.hidden + n0 + column) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        if (write) {
+          for (int i = tid; i < size / 4; i += kConsumers * 32) {
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            auto add = [&](const float4& q) {
+              o.x += q.x;
+              o.y += q.y;
+              o.z += q.z;
+              o.w += q.w;
+            };
+            if (whole) {
+              add(reinterpret_cast<const float4*>(sums)[i]);
+              add(reinterpret_cast<const float4*>(sums + size)[i]);
+            } else {
+#pragma unroll 4
+              for (int q = first; q <= last; ++q) {
+                const int slot = share.begin(q) / share.per_tile == tile ? 0 : 1;
+                add(__ldcg(reinterpret_cast<const float4*>(p.parts + (int64_t)(q * 2 + slot) * size) + i));
+              }
+            }
+            const __half2 lo = __floats2half2_rn(o.x, o.y), hi = __floats2half2_rn(o.z, o.w);
+            *reinterpret_cast<uint2*>(p.out + (int64_t)(i / quads) * p.hidden + tile * kTile + (i % quads) * 4) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+          }
+        }
+        tile_first = u + 1;
+        if (u + 1 < u1) {
+          consumers_sync();
+          for (int i = tid; i < 2 * size; i += kConsumers * 32) sums[i] = 0.0f;
+          consumers_sync();
+        }
+      }
     }
   }
-  cluster_sync();  // others may still be reading this CTA's sums
 }
 
 constexpr int kMaxDevices = 64;
@@ -699,33 +781,15 @@ template <int FMT, int NT>
 int launch(Params p, const Weights& w, cudaStream_t stream) {
   auto up = moe_fp4_up_kernel<FMT, NT>;
   auto down = moe_fp4_down_kernel<FMT, NT>;
-  const int sms = sm_count_current(), ctas = kCtasPerSm * sms;
+  const int most_ctas = kCtasPerSm * sm_count_current(), ctas = most_ctas < kMaxCtas ? most_ctas : kMaxCtas;
   const size_t room = (size_t)113 * 1024;  // so that two fit an SM's 228 KB, 1 KB more each
   const size_t red = (size_t)4 * NT * 4 * 32 * 4, sums = (size_t)2 * p.tokens * kTile * 4;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  static thread_local int configured_device = -1, places[9];
+  static thread_local int configured_device = -1;
   int dev = 0;
   RB200_CUDA(cudaGetDevice(&dev));
   if (configured_device != dev) {
     RB200_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     RB200_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    // clusters do not fill the SMs evenly: how many of each size run at a time
-    cudaLaunchConfig_t ask = cfg;
-    ask.numAttrs = 1;
-    ask.dynamicSmemBytes = room;
-    for (int c = 1; c <= 8; ++c) {
-      attr[0].val.clusterDim.x = (unsigned)c;
-      ask.gridDim = dim3((unsigned)(ctas / c * c), 1, 1);
-      RB200_CUDA(cudaOccupancyMaxActiveClusters(&places[c], down, &ask));
-    }
     configured_device = dev;
   }
 
@@ -737,27 +801,29 @@ int launch(Params p, const Weights& w, cudaStream_t stream) {
   const int64_t most = (int64_t)p.tokens * p.top_k * (p.ffn / kTile);
   RB200_CUDA(launch_dependent(up, dim3((unsigned)(most < ctas ? most : ctas)), kThreads, smem_bytes<NT>(l, p.stages, red), stream, p, map));
 
-  // down: as large a cluster as leaves room for all of them at a time (a token's experts are top_k different ones).  An eighth
-  // less than the query says: 103 clusters of four and 32 of eight, which it had room for, ran one after the others.
-  const int per = (p.ffn + 2 * kStageK - 1) / (2 * kStageK), n_tiles = p.hidden / kTile;
-  p.cluster = 1;
-  for (int c = 2; c <= 8 && c <= p.top_k * per; ++c)
-    if (n_tiles <= places[c] - places[c] / 8) p.cluster = c;
   l = layout<FMT, NT, false>();
   p.stages = kMaxStages;
   while (p.stages > 2 && smem_bytes<NT>(l, p.stages, sums) > room) --p.stages;
   if (weight_map(&map, w.down, (int64_t)p.experts * p.hidden, p.ffn) != 0) return -1;
-  cfg.gridDim = dim3((unsigned)(n_tiles * p.cluster), 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes<NT>(l, p.stages, sums);
-  attr[0].val.clusterDim.x = (unsigned)p.cluster;
-  cfg.numAttrs = 2;
-  RB200_CUDA(cudaLaunchKernelEx(&cfg, down, p, map));
+  RB200_CUDA(launch_dependent(down, dim3((unsigned)ctas), kThreads, smem_bytes<NT>(l, p.stages, sums), stream, p, map));
   return 0;
 }
 
 template <int FMT>
 int launch_fmt(const Params& p, const Weights& w, cudaStream_t stream) {
   return p.tokens <= 8 ? launch<FMT, 1>(p, w, stream) : launch<FMT, 2>(p, w, stream);
+}
+
+// [h | parts | tickets]
+struct Workspace {
+  size_t parts, tickets, bytes;
+};
+Workspace workspace_of(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn) {
+  Workspace w;
+  w.parts = (size_t)((tokens * top_k * ffn * 2 + 255) / 256 * 256);
+  w.tickets = w.parts + (size_t)kMaxCtas * 2 * tokens * kTile * 4;
+  w.bytes = w.tickets + (size_t)((hidden + kTile - 1) / kTile) * 4;
+  return w;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -786,8 +852,9 @@ using namespace rb200;
 
 extern "C" {
 
-size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t ffn) {
-  return tokens > 0 && top_k > 0 && ffn > 0 ? (size_t)(tokens * top_k * ffn) * 2 : 0;
+size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn) {
+  if (tokens <= 0 || top_k <= 0 || hidden <= 0 || ffn <= 0) return 0;
+  return f4::workspace_of(tokens, top_k, hidden, ffn).bytes;
 }
 
 int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -801,6 +868,8 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   RB200_CHECK(d->hidden > 0 && d->hidden % 64 == 0 && d->ffn > 0 && d->ffn % 64 == 0 && d->hidden < (1 << 24) && d->ffn < (1 << 24) &&
                   d->num_experts * 2 * d->ffn < (1ll << 31) && d->num_experts * d->hidden < (1ll << 31),
               "hidden and ffn must be multiples of 64 (hidden=%lld, ffn=%lld)", (long long)d->hidden, (long long)d->ffn);
+  RB200_CHECK(d->hidden / 64 * d->tokens * d->top_k * ((d->ffn + 511) / 512) < (1ll << 30) && d->ffn / 64 * d->tokens * d->top_k < (1ll << 30),
+              "the layer is too large (hidden=%lld, ffn=%lld)", (long long)d->hidden, (long long)d->ffn);
   RB200_CHECK(d->format == f4::kNv || (!d->gate_up_tensor_scale && !d->down_tensor_scale), "the mx format has no tensor scale");
   if (d->tokens == 0) return 0;
   RB200_CHECK(d->x && d->logits && d->w_gate_up && d->gate_up_scales && d->w_down && d->down_scales && d->out && workspace,
@@ -809,7 +878,7 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
                   f4::aligned16(d->down_scales) && f4::aligned16(d->out) && f4::aligned16(workspace) &&
                   (reinterpret_cast<uintptr_t>(d->logits) & 3u) == 0,
               "tensors must be 16-byte aligned");
-  RB200_CHECK(workspace_bytes >= rb200_moe_layer_fp4_workspace_bytes(d->tokens, d->top_k, d->ffn),
+  RB200_CHECK(workspace_bytes >= rb200_moe_layer_fp4_workspace_bytes(d->tokens, d->top_k, d->hidden, d->ffn),
               "the workspace must hold rb200_moe_layer_fp4_workspace_bytes");
   f4::Params p;
   memset(&p, 0, sizeof(p));
@@ -819,7 +888,10 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   p.s2 = static_cast<const uint8_t*>(d->down_scales);
   p.ts1 = d->gate_up_tensor_scale;
   p.ts2 = d->down_tensor_scale;
+  const f4::Workspace ws = f4::workspace_of(d->tokens, d->top_k, d->hidden, d->ffn);
   p.h = static_cast<__half*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.parts);
+  p.tickets = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + ws.tickets);
   p.out = static_cast<__half*>(d->out);
   p.s1_expert = f4::scale_bytes(2 * d->ffn, d->hidden, d->format);
   p.s2_expert = f4::scale_bytes(d->hidden, d->ffn, d->format);

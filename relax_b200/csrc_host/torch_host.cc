@@ -759,7 +759,7 @@ PyObject* moe_layer_fp4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (!out.given) out.t = empty_on(x->sizes(), c10::ScalarType::Half, *x);
   at::Tensor ws;
   if (a[11] == Py_None) {
-    ws = empty_on({static_cast<int64_t>(lib.moe_layer_fp4_workspace_bytes(x->size(0), top_k, w2->size(2) * 2))}, c10::ScalarType::Byte, *x);
+    ws = empty_on({static_cast<int64_t>(lib.moe_layer_fp4_workspace_bytes(x->size(0), top_k, x->size(1), w2->size(2) * 2))}, c10::ScalarType::Byte, *x);
   } else {
     const at::Tensor* p = as_tensor(a[11], "workspace");
     if (!p) return nullptr;

@@ -235,6 +235,6 @@ def moe_layer_fp4(x, logits, w_gate_up, gate_up_scales, w_down, down_scales, top
                                 down_tensor_scale, renormalize, workspace, out)
 
 
-def moe_layer_fp4_workspace_bytes(tokens: int, top_k: int, ffn: int) -> int:
+def moe_layer_fp4_workspace_bytes(tokens: int, top_k: int, hidden: int, ffn: int) -> int:
     from . import _lib
-    return int(_lib.load().rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, ffn))
+    return int(_lib.load().rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, hidden, ffn))

@@ -133,7 +133,7 @@ def test_moe_refusals(change, words):
 
 def test_moe_workspace_refusals():
     lib, ws = _lib.load(), ctypes.c_void_p(1024)
-    need = lib.rb200_moe_layer_fp4_workspace_bytes(2, 2, 128)
+    need = lib.rb200_moe_layer_fp4_workspace_bytes(2, 2, 64, 128)
     assert "NULL" in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer()), None, need, None))
     assert "workspace" in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer()), ws, need - 1, None))
     assert "aligned" in _error(lib.rb200_moe_layer_fp4(ctypes.byref(_layer()), ctypes.c_void_p(1032), need, None))

@@ -157,7 +157,7 @@ def test_strides_types_outputs_and_empty_batches():
     wide = torch.zeros(5, 300, device="cuda").half()
     wide[:, 3:259] = x
     assert torch.equal(ops.moe_layer_fp4(wide[:, 3:259], logits.double(), *w, 2, "mx"), want)
-    ws = torch.empty(ops.moe_layer_fp4_workspace_bytes(5, 2, 192), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(ops.moe_layer_fp4_workspace_bytes(5, 2, 256, 192), dtype=torch.uint8, device="cuda")
     out = torch.zeros(6, 256, device="cuda").half()
     assert torch.equal(ops.moe_layer_fp4(x, logits, *w, 2, "mx", workspace=ws, out=out[:5]), want)
     assert not out[5].any()
