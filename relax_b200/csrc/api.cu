@@ -283,6 +283,10 @@ int rb200_check_async_error(void* stream, int* status_out) {
   if (noalloc_read_status(&v2) != 0 || encode_read_status(&v3) != 0 || fp4_gemm_read_status(&v4) != 0 ||
       fp4_moe_read_status(&v5) != 0)
     return -1;
+  if (v5 != 0) {  // hand-over words of an expert layer whose wait gave up
+    RB200_CUDA(cudaDeviceSynchronize());
+    if (handover_reset() != 0) return -1;
+  }
   if (st == 0) st = v2 != 0 ? v2 : v3 != 0 ? v3 : v4 != 0 ? v4 : v5;
   if (status_out) *status_out = st;
   return 0;

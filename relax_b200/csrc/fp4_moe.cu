@@ -21,6 +21,7 @@
 
 #include "../../include/relax_b200.h"
 #include "fp4_mma.cuh"
+#include "handover.h"
 #include "tensormap.h"
 
 namespace rb200 {
@@ -72,6 +73,8 @@ struct Params {
   int stages;
   float* parts;       // down: two tiles [tokens][64] a CTA
   uint32_t* tickets;  // down: a tile's parts that are there
+  uint32_t* words;    // up: hand-over words, or nullptr
+  uint64_t wait_ns;   // bound of the wait for them
 };
 
 // order of floats as unsigned numbers, NaN lowest
@@ -415,6 +418,92 @@ __device__ __forceinline__ void join(float (&sum)[S][NT][4]) {  // all into the 
 constexpr int kRoutingOffset = 2 * kMaxStages * 8;
 constexpr int kCtasPerSm = 2;
 
+// A sequence of units cut evenly over the CTAs.
+struct Share {
+  int total, ctas;  // units, CTAs with some
+  __device__ __forceinline__ int begin(int cta) const { return (int)((int64_t)total * cta / ctas); }
+  __device__ __forceinline__ int owner(int unit) const { return (int)(((int64_t)(unit + 1) * ctas - 1) / total); }
+};
+// A unit's place, (tile, a, c) for `down`, (a, tile, c) for `up`, kept by counting: the divisions took as long as a unit's
+// products.
+template <bool UP>
+struct Place {
+  int tile, a, c, per, inner;  // chunks of an inner item, items of an outer one
+  __device__ __forceinline__ Place(int unit, int per_, int inner_) : per(per_), inner(inner_) {
+    const int outer = unit / (per * inner), v = unit - outer * (per * inner), in = v / per;
+    tile = UP ? in : outer;
+    a = UP ? outer : in;
+    c = v - in * per;
+  }
+  __device__ __forceinline__ bool last_of_entry() const { return c + 1 == per; }
+  __device__ __forceinline__ bool last_of_tile() const { return last_of_entry() && a + 1 == inner; }
+  __device__ __forceinline__ void next() {
+    if (++c == per) {
+      c = 0;
+      int& in = UP ? tile : a;
+      if (++in == inner) {
+        in = 0;
+        ++(UP ? a : tile);
+      }
+    }
+  }
+};
+
+// Hand-over words (handover.h): a warp's sums of a part of a 64-row tile.  A word is its own flag, vacant (all bits set) at rest.
+constexpr uint32_t kVacant = 0xffffffffu;
+template <int NT>
+__host__ __device__ constexpr int part_words() {
+  return kConsumers * NT * 4 * 32;
+}
+template <int NT>
+__device__ __forceinline__ uint4* part_of(uint32_t* words, int cta, int j) {
+  return reinterpret_cast<uint4*>(words + (int64_t)cta * part_words<NT>()) + ((threadIdx.x >> 5) * NT + j) * 32 + (threadIdx.x & 31);
+}
+template <int NT>
+__device__ __forceinline__ void publish(uint32_t* words, int cta, const float (&acc)[NT][4]) {
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __float_as_uint(acc[j][i]);
+      if (v[i] == kVacant) v[i] = 0x7fffffffu;
+    }
+    asm volatile("st.volatile.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(part_of<NT>(words, cta, j)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3])
+                 : "memory");
+  }
+}
+// acc += the part of `cta`, whose words are left vacant; false when the wait for them ran out
+template <int NT>
+__device__ __forceinline__ bool absorb(uint32_t* words, int cta, float (&acc)[NT][4], uint64_t limit_ns) {
+#pragma unroll 1
+  for (int j = 0; j < NT; ++j) {
+    uint4* at = part_of<NT>(words, cta, j);
+    uint32_t v[4];
+    uint64_t began = 0;
+    for (;;) {
+      asm volatile("ld.volatile.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(at) : "memory");
+      if (v[0] != kVacant && v[1] != kVacant && v[2] != kVacant && v[3] != kVacant) break;
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (began == 0) began = now;
+      if (now - began > limit_ns) {
+        atomicExch(&g_status, kStatusWaitTimeout);
+        return false;
+      }
+    }
+    asm volatile("st.volatile.global.v4.u32 [%0], {%1, %1, %1, %1};" ::"l"(at), "r"(kVacant) : "memory");
+#pragma unroll
+    for (int q = 0; q < NT; ++q)  // (registers have no index)
+      if (q == j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[q][i] += __uint_as_float(v[i]);
+      }
+  }
+  return true;
+}
+
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr int TILES = stage_tiles(FMT);
@@ -440,54 +529,56 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
   route<NT>(p, r, reinterpret_cast<float*>(smem));
   rows_sync();
 
+  // (entry, 64 f, 256 k) units.  With words to hand over parts in, the CTAs get equal shares: whoever has an item's first k adds
+  // what the CTAs behind it did of it, which they do first; else whole items.
   const int f_tiles = p.ffn / kTile, items = r.entries * f_tiles, chunks = (p.hidden + kStageK - 1) / kStageK;
+  Share share;
+  share.total = p.words ? items * chunks : items;
+  share.ctas = min((int)gridDim.x, p.words ? max(share.total / 2, 1) : items);
+  const bool any = (int)blockIdx.x < share.ctas;
+  const int unit = p.words ? 1 : chunks;
+  const int u0 = any ? share.begin(blockIdx.x) * unit : 0, u1 = any ? share.begin(blockIdx.x + 1) * unit : 0;
   Ring ring = {p.stages, 0, 0u};
   if (warp == kConsumers) {
     // ============================================================ weights
     const bool leader = elect_one();
     int issued = 0;
-    bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
-      const uint8_t* s_gate = p.s1 + e * p.s1_expert + (int64_t)(f0 >> 7) * p.k_tiles1 * 512;
-      const uint8_t* s_up = p.s1 + e * p.s1_expert + (int64_t)((p.ffn + f0) >> 7) * p.k_tiles1 * 512;
-      for (int c = 0; c < chunks; ++c) {
-        ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (leader) {
-          uint64_t* bar = &full[ring.s];
-          uint8_t* w = smem + ring.s * L.code_bytes;
-          uint8_t* sc = scales + ring.s * L.scale_bytes;
-          mbar_arrive_expect_tx(bar, L.code_bytes + L.scale_bytes);
-          tma_load(w, &tmap_w, c * 128, e * 2 * p.ffn + f0, bar);
-          tma_load(w + kBox, &tmap_w, c * 128, e * 2 * p.ffn + p.ffn + f0, bar);
-          load_scale_tiles(sc, s_gate, c * TILES, TILES, p.k_tiles1 - 1, bar);
-          load_scale_tiles(sc + TILES * 512, s_up, c * TILES, TILES, p.k_tiles1 - 1, bar);
-        }
-        __syncwarp();
-        ++issued;
-        ring.next();
+    Place<true> at(u0, chunks, f_tiles);
+    for (int u = u0; u < u1; ++u, at.next()) {
+      bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (leader) {
+        const int c = at.c, f0 = at.tile * kTile, e = r.entry_expert[at.a];
+        const uint8_t* s_e = p.s1 + e * p.s1_expert;
+        uint64_t* bar = &full[ring.s];
+        uint8_t* w = smem + ring.s * L.code_bytes;
+        uint8_t* sc = scales + ring.s * L.scale_bytes;
+        mbar_arrive_expect_tx(bar, L.code_bytes + L.scale_bytes);
+        tma_load(w, &tmap_w, c * 128, e * 2 * p.ffn + f0, bar);
+        tma_load(w + kBox, &tmap_w, c * 128, e * 2 * p.ffn + p.ffn + f0, bar);
+        load_scale_tiles(sc, s_e + (int64_t)(f0 >> 7) * p.k_tiles1 * 512, c * TILES, TILES, p.k_tiles1 - 1, bar);
+        load_scale_tiles(sc + TILES * 512, s_e + (int64_t)((p.ffn + f0) >> 7) * p.k_tiles1 * 512, c * TILES, TILES, p.k_tiles1 - 1, bar);
       }
+      __syncwarp();
+      ++issued;
+      ring.next();
     }
     drain_ring(full, p.stages, issued);
   } else if (warp == kConsumers + 1) {
     // ============================================================ x
     int issued = 0;
-    bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int a = item / f_tiles, row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0;
-      for (int c = 0; c < chunks; ++c) {
-        ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const int k = c * kStageK + lane * 8;
-        const bool there = k < p.hidden;
-        copy_rows(smem_u32(xs + ring.s * L.x_bytes), p.x + (there ? k : 0), p.hidden, r.token_of_row + row0, rows, there);
-        cp_async_arrive(&full[ring.s]);
-        ++issued;
-        ring.next();
-      }
+    Place<true> at(u0, chunks, f_tiles);
+    for (int u = u0; u < u1; ++u, at.next()) {
+      bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const int row0 = r.entry_row[at.a], rows = r.entry_row[at.a + 1] - row0, k = at.c * kStageK + lane * 8;
+      const bool there = k < p.hidden;
+      copy_rows(smem_u32(xs + ring.s * L.x_bytes), p.x + (there ? k : 0), p.hidden, r.token_of_row + row0, rows, there);
+      cp_async_arrive(&full[ring.s]);
+      ++issued;
+      ring.next();
     }
     drain_ring(full, p.stages, issued);
   } else {
@@ -499,15 +590,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
     const uint32_t w_at = smem_u32(smem) + is_up * kBox + fb * 16 * 128;
     const uint8_t* const x_at = xs + g * (kStageK * 2) + t * 16;
     bool ok = true;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-      const int a = item / f_tiles, f0 = (item - a * f_tiles) * kTile, e = r.entry_expert[a];
-      const int row0 = r.entry_row[a], rows = r.entry_row[a + 1] - row0, tiles = (rows + 7) / 8;
+    Place<true> at(u0, chunks, f_tiles);
+    for (int u = u0; u < u1;) {
+      const int f0 = at.tile * kTile, e = r.entry_expert[at.a], first = at.c, n = min(chunks - first, u1 - u);
+      const int row0 = r.entry_row[at.a], rows = r.entry_row[at.a + 1] - row0, tiles = (rows + 7) / 8;
       float sum[kSums][NT][4];
       zero(sum);
       // this lane's words in the scale tiles of its rows
       const uint8_t* const s0 = scales + is_up * TILES * 512 + (int)scale_word(((is_up ? p.ffn + f0 : f0) & 127) + fb * 16 + g, 0, 1);
       const uint8_t* const s8 = scales + is_up * TILES * 512 + (int)scale_word(((is_up ? p.ffn + f0 : f0) & 127) + fb * 16 + g + 8, 0, 1);
-      for (int c = 0; c < chunks; ++c) {
+      for (int i = 0; i < n; ++i, at.next()) {
         if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
         walk.stage(sum, w_at + ring.s * L.code_bytes, x_at + ring.s * L.x_bytes, s0 + ring.s * L.scale_bytes, s8 + ring.s * L.scale_bytes, t,
                    tiles);
@@ -515,8 +607,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
         if (lane == 0) mbar_arrive(&empty[ring.s]);
         ring.next();
       }
+      u += n;
       float(&acc)[NT][4] = sum[0];
       join(sum);
+      if (first > 0) {
+        if (ok) publish<NT>(p.words, blockIdx.x, acc);
+        continue;
+      }
+      if (n < chunks) {
+        const int last = share.owner(u - n + chunks - 1);
+        for (int q = blockIdx.x + 1; ok && q <= last; ++q) ok = absorb<NT>(p.words, q, acc, p.wait_ns);
+      }
       // gate and up meet; rows g, g + 8 of columns 2t, 2t + 1
       if (!ok) r.failed = 1;
       if (is_up) {
@@ -544,34 +645,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
   }
 }
 
-// The sequence of units (64 output columns, entry, 512 k) cut evenly over the CTAs.
-struct Share {
-  int total, ctas, per_tile;  // units, CTAs with some, units of 64 columns
-  __device__ __forceinline__ int begin(int cta) const { return (int)((int64_t)total * cta / ctas); }
-  __device__ __forceinline__ int owner(int unit) const { return (int)(((int64_t)(unit + 1) * ctas - 1) / total); }
-};
-// A unit's place, kept by counting: the divisions took as long as a unit's products.
-struct Place {
-  int tile, a, c, per, entries;
-  __device__ __forceinline__ Place(int unit, int per_, int entries_) : per(per_), entries(entries_) {
-    tile = unit / (per * entries);
-    const int v = unit - tile * (per * entries);
-    a = v / per;
-    c = v - a * per;
-  }
-  __device__ __forceinline__ bool last_of_entry() const { return c + 1 == per; }
-  __device__ __forceinline__ bool last_of_tile() const { return last_of_entry() && a + 1 == entries; }
-  __device__ __forceinline__ void next() {
-    if (++c == per) {
-      c = 0;
-      if (++a == entries) {
-        a = 0;
-        ++tile;
-      }
-    }
-  }
-};
-
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w) {
   constexpr int TILES = stage_tiles(FMT), kUnitK = 2 * kStageK;
@@ -598,9 +671,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
   rows_sync();
 
   const int per = (p.ffn + kUnitK - 1) / kUnitK;
+  const int per_tile = r.entries * per;
   Share share;
-  share.per_tile = r.entries * per;
-  share.total = p.hidden / kTile * share.per_tile;
+  share.total = p.hidden / kTile * per_tile;
   share.ctas = min((int)gridDim.x, share.total);
   const bool any = (int)blockIdx.x < share.ctas;
   const int u0 = any ? share.begin(blockIdx.x) : 0, u1 = any ? share.begin(blockIdx.x + 1) : 0;
@@ -609,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
     // ============================================================ weights (older than the kernel before, too)
     const bool leader = elect_one();
     int issued = 0;
-    Place at(u0, per, r.entries);
+    Place<false> at(u0, per, r.entries);
     for (int u = u0; u < u1; ++u, at.next()) {
       bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
       ok = __all_sync(0xffffffffu, ok);
@@ -635,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
     griddep_wait();  // the kernel before's
     griddep_launch_dependents();
     int issued = 0;
-    Place at(u0, per, r.entries);
+    Place<false> at(u0, per, r.entries);
     for (int u = u0; u < u1; ++u, at.next()) {
       bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
       ok = __all_sync(0xffffffffu, ok);
@@ -666,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
     float sum[kSums][NT][4];
     float(&acc)[NT][4] = sum[0];
     int tile_first = u0;  // this CTA's first unit of the tile at hand
-    Place at(u0, per, r.entries);
+    Place<false> at(u0, per, r.entries);
     int row0 = 0, rows = 0, tiles = 0;
     for (int u = u0; u < u1; ++u, at.next()) {
       const int tile = at.tile;
@@ -705,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
         // The tile as far as this CTA has it: written as it is if that is all of it, else put with the parts of other CTAs; who
         // comes last adds them up, in the order of the CTAs.
         constexpr int quads = kTile / 4;
-        const int first = share.owner(tile * share.per_tile), last = share.owner((tile + 1) * share.per_tile - 1);
+        const int first = share.owner(tile * per_tile), last = share.owner((tile + 1) * per_tile - 1);
         const bool whole = first == last;
         const int size = p.tokens * kTile;
         float* mine = p.parts + (int64_t)(blockIdx.x * 2 + (tile_first == u0 ? 0 : 1)) * size;
@@ -738,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
             } else {
 #pragma unroll 4
               for (int q = first; q <= last; ++q) {
-                const int slot = share.begin(q) / share.per_tile == tile ? 0 : 1;
+                const int slot = share.begin(q) / per_tile == tile ? 0 : 1;
                 add(__ldcg(reinterpret_cast<const float4*>(p.parts + (int64_t)(q * 2 + slot) * size) + i));
               }
             }
@@ -798,8 +871,9 @@ int launch(Params p, const Weights& w, cudaStream_t stream) {
   while (p.stages > 2 && smem_bytes<NT>(l, p.stages, red) > room) --p.stages;
   CUtensorMap map;
   if (weight_map(&map, w.up, (int64_t)p.experts * 2 * p.ffn, p.hidden) != 0) return -1;
-  const int64_t most = (int64_t)p.tokens * p.top_k * (p.ffn / kTile);
-  RB200_CUDA(launch_dependent(up, dim3((unsigned)(most < ctas ? most : ctas)), kThreads, smem_bytes<NT>(l, p.stages, red), stream, p, map));
+  p.words = handover_words(stream, sm_count_current(), (size_t)ctas * part_words<NT>() * sizeof(uint32_t));
+  p.wait_ns = (wait_limit_ms() ? (uint64_t)wait_limit_ms() : 2000ull) * 1000000ull;
+  RB200_CUDA(launch_dependent(up, dim3((unsigned)ctas), kThreads, smem_bytes<NT>(l, p.stages, red), stream, p, map));
 
   l = layout<FMT, NT, false>();
   p.stages = kMaxStages;
@@ -868,7 +942,7 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   RB200_CHECK(d->hidden > 0 && d->hidden % 64 == 0 && d->ffn > 0 && d->ffn % 64 == 0 && d->hidden < (1 << 24) && d->ffn < (1 << 24) &&
                   d->num_experts * 2 * d->ffn < (1ll << 31) && d->num_experts * d->hidden < (1ll << 31),
               "hidden and ffn must be multiples of 64 (hidden=%lld, ffn=%lld)", (long long)d->hidden, (long long)d->ffn);
-  RB200_CHECK(d->hidden / 64 * d->tokens * d->top_k * ((d->ffn + 511) / 512) < (1ll << 30) && d->ffn / 64 * d->tokens * d->top_k < (1ll << 30),
+  RB200_CHECK(d->hidden / 64 * d->tokens * d->top_k * ((d->ffn + 511) / 512) < (1ll << 30) && d->ffn / 64 * d->tokens * d->top_k * ((d->hidden + 255) / 256) < (1ll << 30),
               "the layer is too large (hidden=%lld, ffn=%lld)", (long long)d->hidden, (long long)d->ffn);
   RB200_CHECK(d->format == f4::kNv || (!d->gate_up_tensor_scale && !d->down_tensor_scale), "the mx format has no tensor scale");
   if (d->tokens == 0) return 0;
