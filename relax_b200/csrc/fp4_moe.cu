@@ -160,7 +160,15 @@ __device__ __forceinline__ void route(const Params& p, Routing<NT>& r, float* sc
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < kMaxExperts) r.mask[tid] = 0u;
 #pragma unroll 1
-  for (int i = tid; i < p.tokens * p.experts; i += kThreads) scratch[i] = __ldcg(p.logits + i);
+  for (int i = tid; i < p.tokens * p.experts; i += 8 * kThreads) {  // (eight loads on their way: one after the other is a microsecond each)
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j * kThreads < p.tokens * p.experts) v[j] = __ldcg(p.logits + i + j * kThreads);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j * kThreads < p.tokens * p.experts) scratch[i + j * kThreads] = v[j];
+  }
   __syncthreads();
 #pragma unroll 1
   for (int t = warp; t < p.tokens; t += kThreads / 32) {
@@ -674,7 +682,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
   const int per_tile = r.entries * per;
   Share share;
   share.total = p.hidden / kTile * per_tile;
-  share.ctas = min((int)gridDim.x, share.total);
+  share.ctas = (int)gridDim.x;
+  // as many CTAs a column tile where that is nearly all of them: every CTA then has a part of one tile only
+  const int each = share.ctas / (p.hidden / kTile);
+  if (each * (p.hidden / kTile) * 16 >= share.ctas * 15) share.ctas = each * (p.hidden / kTile);
+  share.ctas = min(share.ctas, share.total);
   const bool any = (int)blockIdx.x < share.ctas;
   const int u0 = any ? share.begin(blockIdx.x) : 0, u1 = any ? share.begin(blockIdx.x + 1) : 0;
   Ring ring = {p.stages, 0, 0u};
@@ -740,14 +752,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
     float(&acc)[NT][4] = sum[0];
     int tile_first = u0;  // this CTA's first unit of the tile at hand
     Place<false> at(u0, per, r.entries);
-    int row0 = 0, rows = 0, tiles = 0;
+    int rows = 0, tiles = 0, token[NT][2];
+    float gate[NT][2];
     for (int u = u0; u < u1; ++u, at.next()) {
       const int tile = at.tile;
       if (u == u0 || at.c == 0) {
         zero(sum);
-        row0 = r.entry_row[at.a];
+        const int row0 = r.entry_row[at.a];
         rows = r.entry_row[at.a + 1] - row0;
         tiles = (rows + 7) / 8;
+        const float ts = p.ts2 ? p.ts2[r.entry_expert[at.a]] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {  // of this lane's columns of the sums
+            const int row = row0 + min(j * 8 + 2 * t + q, rows - 1);
+            token[j][q] = r.token_of_row[row];
+            gate[j][q] = r.gate_of_row[row] * ts;
+          }
       }
       if (ok) ok = mbar_wait_parked(&full[ring.s], ring.ph, &g_status);
       const uint8_t* sc = scales + ring.s * L.scale_bytes + kh * TILES * 512 + (tile & 1) * 8;  // rows 64 .. 127 of a scale tile: words 2, 3
@@ -759,17 +781,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
       if (tile_ends || at.last_of_entry()) {
         join(sum);
         // this entry's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane at a time)
-        const float ts = p.ts2 ? p.ts2[r.entry_expert[at.a]] : 1.0f;
+        float* word[NT][2];
+        float had[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = j * 8 + 2 * t + (i & 1);
-            if (row < rows) {
-              float* word = sums + ((kh * p.tokens + r.token_of_row[row0 + row]) * kTile + fb * 16 + g + (i >> 1) * 8);
-              *word = fmaf(r.gate_of_row[row0 + row] * ts, acc[j][i], *word);
-            }
+          for (int q = 0; q < 2; ++q) {
+            word[j][q] = sums + (kh * p.tokens + token[j][q]) * kTile + fb * 16 + g;
+            had[j][q] = word[j][q][0];
+            had[j][2 + q] = word[j][q][8];
           }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (j * 8 + 2 * t + q < rows) {
+              word[j][q][0] = fmaf(gate[j][q], acc[j][q], had[j][q]);
+              word[j][q][8] = fmaf(gate[j][q], acc[j][2 + q], had[j][2 + q]);
+            }
         __syncwarp();
       }
       if (tile_ends) {
