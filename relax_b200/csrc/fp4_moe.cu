@@ -40,10 +40,10 @@ constexpr int kMaxCtas = 512;  // that the workspace has room for
 
 __device__ int g_status;
 
-// Rows are the (token, expert) pairs by expert; an entry is at most 8 NT rows of one expert.  NT = 1 has at most eight tokens.
+// Rows are the (token, expert) pairs by expert; an entry is at most 8 NT rows of one expert.
 template <int NT>
 struct alignas(16) Routing {
-  static constexpr int kRows = (NT == 1 ? 8 : kMaxTokens) * kMaxTopK;
+  static constexpr int kRows = kMaxTokens * kMaxTopK;
   uint32_t mask[kMaxExperts];  // tokens of an expert
   float gate_of_row[kRows];
   float gate_of[kRows];        // by token and choice
@@ -914,7 +914,10 @@ int launch(Params p, const Weights& w, cudaStream_t stream) {
 
 template <int FMT>
 int launch_fmt(const Params& p, const Weights& w, cudaStream_t stream) {
-  return p.tokens <= 8 ? launch<FMT, 1>(p, w, stream) : launch<FMT, 2>(p, w, stream);
+  // Entries of eight rows, or of sixteen where experts have more than four on average: weights of an expert with more rows than
+  // an entry are read again (by then from L2), rows that are not there take shared memory from the stages (29 tokens,
+  // 64 experts of top 6: 100 us with sixteen, 79 with eight).
+  return p.tokens <= 8 || p.tokens * p.top_k <= 4 * p.experts ? launch<FMT, 1>(p, w, stream) : launch<FMT, 2>(p, w, stream);
 }
 
 // [h | parts | tickets]
