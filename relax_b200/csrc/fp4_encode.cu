@@ -6,7 +6,7 @@
 // over the blocks of a row; a block whose s is 0 has codes 0, one with an infinity or a NaN the NaN scale and codes 0, and
 // where ts is not a positive finite number every block has the NaN scale.
 //
-// One pass over x: a lane takes 16 consecutive k, a warp 512.  kMx is exact in fp32 as it stands (division by a power of
+// One pass over x: a lane takes 16 consecutive k, a warp 512, two rows on their way.  kMx is exact in fp32 as it stands (division by a power of
 // two).  kNv divides by s * ts, which fp32 cannot hold: x is multiplied by 1 / (s ts) taken once 2^-21 too small and once too
 // large, and where the two codes differ - x lies next to the border between them - x and the border are compared in 64
 // bits, where border * s * ts is exact (3 + 4 + 24 bits).  The scale itself is rounded from a 64-bit quotient: see
@@ -19,40 +19,64 @@ namespace {
 using namespace f4;
 
 constexpr int kWarps = 8;
+constexpr int kRowsPerCta = 32;  // a CTA's rows, of 512 k
 
+// 16 consecutive elements as they lie in memory, their values, and the bits of their largest magnitude as fp32 (a NaN's are
+// above infinity's)
 template <class T>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16]);
-template <>
-__device__ __forceinline__ void load16<__half>(const __half* p, float (&v)[16]) {
-  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+struct Sixteen {
+  static constexpr int kVectors = sizeof(T);  // of 16 bytes
+  uint4 raw[kVectors];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    for (int i = 0; i < kVectors; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ uint32_t word(int i) const {
+    const uint4& q = raw[i >> 2];
+    return (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+  }
+  __device__ __forceinline__ float2 two(int i) const;  // elements 2i, 2i + 1
+  __device__ __forceinline__ uint32_t top() const;
+};
+template <>
+__device__ __forceinline__ float2 Sixteen<__half>::two(int i) const {
+  const uint32_t w = word(i);
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 template <>
-__device__ __forceinline__ void load16<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[16]) {
-  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+__device__ __forceinline__ float2 Sixteen<__nv_bfloat16>::two(int i) const {
+  return make_float2(__uint_as_float(word(i) << 16), __uint_as_float(word(i) & 0xffff0000u));
 }
 template <>
-__device__ __forceinline__ void load16<float>(const float* p, float (&v)[16]) {
+__device__ __forceinline__ float2 Sixteen<float>::two(int i) const {
+  return make_float2(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+}
+// (magnitudes of either 16-bit type order as integers, two at a time)
+template <class T>
+__device__ __forceinline__ uint32_t top_pair(const Sixteen<T>& v) {
+  uint32_t m = v.word(0) & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 f = reinterpret_cast<const float4*>(p)[i];
-    v[4 * i] = f.x;
-    v[4 * i + 1] = f.y;
-    v[4 * i + 2] = f.z;
-    v[4 * i + 3] = f.w;
-  }
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, v.word(i) & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
+}
+template <>
+__device__ __forceinline__ uint32_t Sixteen<__half>::top() const {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top_pair(*this))));
+}
+template <>
+__device__ __forceinline__ uint32_t Sixteen<__nv_bfloat16>::top() const {
+  return top_pair(*this) << 16;
+}
+template <>
+__device__ __forceinline__ uint32_t Sixteen<float>::top() const {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, word(i) & 0x7fffffffu);
+  return m;
 }
 
 // RNE_e4m3 of amax / (6 ts), r = that quotient in 64 bits (off by a few 2^-53).  The borders between e4m3 values have five
@@ -79,18 +103,30 @@ __device__ __noinline__ uint32_t code_by_borders(double ax, double unit) {
   return c;
 }
 
+// eight values times f -> codes
+template <class T>
+__device__ __forceinline__ uint32_t scaled_codes(const Sixteen<T>& v, int half, float f) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 q = v.two(4 * half + i);
+    // both products in one instruction
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(q.x), "+f"(q.y)
+        : "f"(f));
+    y[2 * i] = q.x;
+    y[2 * i + 1] = q.y;
+  }
+  return to_codes8(y);
+}
+
 // codes of 16 elements
-template <int FMT>
-__device__ __forceinline__ void codes16(const float (&v)[16], uint32_t byte, float ts, uint32_t (&out)[2]) {
+template <int FMT, class T>
+__device__ __forceinline__ void codes16(const Sixteen<T>& v, uint32_t byte, float ts, uint32_t (&out)[2]) {
   if (FMT == kMx) {
     const float inv = __uint_as_float((254u - byte) << 23);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i] * inv;
-      out[h] = to_codes8(y);
-    }
+    out[0] = scaled_codes(v, 0, inv);
+    out[1] = scaled_codes(v, 1, inv);
     return;
   }
   const float s = e4m3_value(byte), unit = s * ts;
@@ -99,17 +135,12 @@ __device__ __forceinline__ void codes16(const float (&v)[16], uint32_t byte, flo
     return;
   }
   const bool plain = unit >= 0x1p-100f && unit <= 0x1p100f;
-  const float inv = 1.0f / unit, below = inv * (1.0f - 0x1p-21f), above = inv * (1.0f + 0x1p-21f);
+  const float inv = __frcp_rn(unit), below = inv * (1.0f - 0x1p-21f), above = inv * (1.0f + 0x1p-21f);
   uint32_t hi[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i] * below;
-    out[h] = to_codes8(y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i] * above;
-    hi[h] = to_codes8(y);
+    out[h] = scaled_codes(v, h, below);
+    hi[h] = scaled_codes(v, h, above);
   }
   if (out[0] == hi[0] && out[1] == hi[1] && plain) return;
   const double exact_unit = (double)s * (double)ts;
@@ -118,13 +149,15 @@ __device__ __forceinline__ void codes16(const float (&v)[16], uint32_t byte, flo
     const int sh = 4 * (i & 7);
     const uint32_t lo = (out[i >> 3] >> sh) & 15u, up = (hi[i >> 3] >> sh) & 15u;
     if (lo != up || !plain) {
-      const double ax = fabs((double)v[i]);
+      const float2 q = v.two(i >> 1);
+      const float x = (i & 1) ? q.y : q.x;
+      const double ax = fabs((double)x);
       uint32_t c;
       if (plain) {
         const double b = border_above(lo & 7u) * exact_unit;
         c = ax > b || (ax == b && (lo & 1u)) ? up : lo;
       } else {
-        c = code_by_borders(ax, exact_unit) | (v[i] < 0.0f ? 8u : 0u);
+        c = code_by_borders(ax, exact_unit) | (__float_as_uint(x) >> 28 & 8u);
       }
       out[i >> 3] = (out[i >> 3] & ~(15u << sh)) | (c << sh);
     }
@@ -133,8 +166,10 @@ __device__ __forceinline__ void codes16(const float (&v)[16], uint32_t byte, flo
 
 struct EncodeParams {
   const void* x;
-  int64_t ldx, batch_stride, rows, rows_padded, tasks;
-  int k, k_tiles, spans;
+  int64_t ldx, batch_stride;
+  int64_t rows, row_groups;  // groups of kRowsPerCta, scale tiles' padding rows among them
+  int64_t batch;
+  int k, k_tiles;
   const float* ts;
   uint8_t* codes;
   uint8_t* scales;
@@ -142,59 +177,66 @@ struct EncodeParams {
 
 template <int FMT, class T>
 __global__ void __launch_bounds__(kWarps * 32) encode_fp4_kernel(const EncodeParams p, bool activations) {
-  const int lane = threadIdx.x & 31;
-  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1, kAhead = 2;  // rows on their way
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seg = (int)blockIdx.x * 32 + lane, k0 = seg * 16, q = seg / (4 * kLanesPerBlock);
   griddep_wait();
   // (weights, scales and zero points are never written by a kernel that lets its dependents start: matmuls may read them
   // ahead of their wait)
   if (activations) griddep_launch_dependents();
-  if (task >= p.tasks) return;
-  const int64_t row_all = task / p.spans;  // rows of all batches, padded to whole tiles
-  const int span = (int)(task - row_all * p.spans);
-  const int64_t e = row_all / p.rows_padded, row = row_all - e * p.rows_padded;
-  const int seg = span * 32 + lane, k0 = seg * 16;
-  const bool real = row < p.rows && k0 < p.k;
-  uint32_t byte = 0u;
-  if (row < p.rows) {
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-    if (real) load16(static_cast<const T*>(p.x) + e * p.batch_stride + row * p.ldx + k0, v);
-    uint32_t top = 0u;  // bits of max |x|: a NaN's are above infinity's
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    if (FMT == kMx) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  for (int64_t e = blockIdx.z; e < p.batch; e += gridDim.z) {
     const float ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
-    bool nan = top >= 0x7f800000u;
-    if (FMT == kMx) {
-      byte = top >> 23;
-      byte = byte > 2u ? byte - 2u : 0u;
-    } else {
-      nan = nan || !(ts > 0.0f && ts <= 3.402823466e38f);
-      byte = nan ? 0u : e4m3_of((double)__uint_as_float(top) / (6.0 * (double)ts));
+    const bool bad = FMT == kNv && !(ts > 0.0f && ts <= 3.402823466e38f);
+    const double per_six = FMT == kNv ? 1.0 / (6.0 * (double)ts) : 0.0;
+    uint8_t* scales = p.scales + e * (p.row_groups * kRowsPerCta / 128) * p.k_tiles * 512;
+    for (int64_t group = blockIdx.y; group < p.row_groups; group += gridDim.y) {
+#pragma unroll 1
+      for (int i = 0; i < kRowsPerCta / kWarps; i += kAhead) {
+        const int64_t row = group * kRowsPerCta + i * kWarps + warp;
+        Sixteen<T> v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (row + j * kWarps < p.rows && k0 < p.k)
+            v[j].load(static_cast<const T*>(p.x) + e * p.batch_stride + (row + j * kWarps) * p.ldx + k0);
+          else
+            v[j].clear();
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int64_t r = row + j * kWarps;
+          const bool real = r < p.rows && k0 < p.k;
+          uint32_t top = v[j].top(), byte;
+          if (FMT == kMx) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          const bool nan = top >= 0x7f800000u || bad;
+          if (FMT == kMx) {
+            byte = top >> 23;
+            byte = byte > 2u ? byte - 2u : 0u;
+          } else {
+            byte = nan ? 0u : e4m3_of((double)__uint_as_float(top) * per_six);
+          }
+          uint32_t c[2] = {0u, 0u};
+          if (nan) byte = FMT == kMx ? 255u : 0x7fu;
+          else codes16<FMT>(v[j], byte, ts, c);
+          if (real)
+            *reinterpret_cast<uint2*>(p.codes + (e * p.rows + r) * (int64_t)(p.k / 2) + k0 / 2) = make_uint2(c[0], c[1]);
+          else
+            byte = 0u;
+          // four blocks of a row are one word
+          uint32_t w = byte << (8 * ((lane / kLanesPerBlock) & 3));
+          w |= __shfl_xor_sync(0xffffffffu, w, kLanesPerBlock);
+          w |= __shfl_xor_sync(0xffffffffu, w, 2 * kLanesPerBlock);
+          if (lane % (4 * kLanesPerBlock) == 0 && q < p.k_tiles) *reinterpret_cast<uint32_t*>(scales + scale_word(r, q, p.k_tiles)) = w;
+        }
+      }
     }
-    uint32_t c[2] = {0u, 0u};
-    if (nan) byte = FMT == kMx ? 255u : 0x7fu;
-    else codes16<FMT>(v, byte, ts, c);
-    if (real)
-      *reinterpret_cast<uint2*>(p.codes + (e * p.rows + row) * (int64_t)(p.k / 2) + k0 / 2) = make_uint2(c[0], c[1]);
-    else byte = 0u;
   }
-  // four blocks of a row are one word
-  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1;
-  uint32_t w = byte << (8 * ((lane / kLanesPerBlock) & 3));
-  w |= __shfl_xor_sync(0xffffffffu, w, kLanesPerBlock);
-  w |= __shfl_xor_sync(0xffffffffu, w, 2 * kLanesPerBlock);
-  const int q = seg / (4 * kLanesPerBlock);
-  if (lane % (4 * kLanesPerBlock) == 0 && q < p.k_tiles)
-    *reinterpret_cast<uint32_t*>(p.scales + e * (p.rows_padded / 128) * p.k_tiles * 512 + scale_word(row, q, p.k_tiles)) = w;
 }
 
 struct DecodeParams {
   const uint8_t* codes;
   const uint8_t* scales;
-  int64_t rows, rows_padded, tasks;
-  int k, k_tiles, spans;
+  int64_t rows, row_groups, row_tiles, batch;
+  int k, k_tiles;
   const float* ts;
   void* out;
 };
@@ -213,32 +255,47 @@ __device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
 
 template <int FMT, class T>
 __global__ void __launch_bounds__(kWarps * 32) decode_fp4_kernel(const DecodeParams p) {
+  constexpr int kAhead = 4;
   griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (task >= p.tasks) return;
-  const int64_t row_all = task / p.spans;
-  const int seg = (int)(task - row_all * p.spans) * 32 + lane, k0 = seg * 16;
+  const int warp = threadIdx.x >> 5, seg = (int)blockIdx.x * 32 + (threadIdx.x & 31), k0 = seg * 16, blk = FMT == kMx ? seg >> 1 : seg;
   if (k0 >= p.k) return;
-  const int64_t e = row_all / p.rows, row = row_all - e * p.rows;
-  const uint2 c = *reinterpret_cast<const uint2*>(p.codes + row_all * (int64_t)(p.k / 2) + k0 / 2);
-  const int blk = FMT == kMx ? seg >> 1 : seg;
-  const uint32_t byte = p.scales[e * (p.rows_padded / 128) * p.k_tiles * 512 + scale_word(row, blk >> 2, p.k_tiles) + (blk & 3)];
-  const float s = scale_value<FMT>(byte), ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
-  float v[16];
+  for (int64_t e = blockIdx.z; e < p.batch; e += gridDim.z) {
+    const float ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
+    const uint8_t* scales = p.scales + e * p.row_tiles * p.k_tiles * 512;
+    for (int64_t group = blockIdx.y; group < p.row_groups; group += gridDim.y) {
+      uint2 c[kAhead];
+      uint32_t byte[kAhead];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t w[4];
-    from_codes8(h ? c.y : c.x, w);
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t r = group * kRowsPerCta + j * kWarps + warp;
+        if (r < p.rows) {
+          c[j] = *reinterpret_cast<const uint2*>(p.codes + (e * p.rows + r) * (int64_t)(p.k / 2) + k0 / 2);
+          byte[j] = scales[scale_word(r, blk >> 2, p.k_tiles) + (blk & 3)];
+        }
+      }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[8 * h + 2 * i] = f.x * s * ts;  // code * scale is exact in fp32
-      v[8 * h + 2 * i + 1] = f.y * s * ts;
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t r = group * kRowsPerCta + j * kWarps + warp;
+        if (r >= p.rows) break;
+        const float s = scale_value<FMT>(byte[j]);
+        float v[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[4];
+          from_codes8(h ? c[j].y : c[j].x, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[8 * h + 2 * i] = FMT == kMx ? f.x * s : f.x * s * ts;  // code * scale is exact in fp32
+            v[8 * h + 2 * i + 1] = FMT == kMx ? f.y * s : f.y * s * ts;
+          }
+        }
+        store16(static_cast<T*>(p.out) + (e * p.rows + r) * (int64_t)p.k + k0, v);
+      }
     }
   }
-  store16(static_cast<T*>(p.out) + row_all * (int64_t)p.k + k0, v);
 }
+static_assert(kRowsPerCta == 4 * kWarps, "a warp's rows");
 
 // a thread per word of the result
 __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* src, uint32_t* dst, int64_t words, int64_t rows, int row_tiles,
@@ -259,9 +316,14 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t* src, ui
   dst[i] = w;
 }
 
+// a CTA per 512 k, rows and matrices beyond the grid's limits by loops
+dim3 grid_of(int spans, int64_t row_groups, int64_t batch) {
+  return dim3((unsigned)spans, (unsigned)(row_groups < 65535 ? row_groups : 65535), (unsigned)(batch < 65535 ? batch : 65535));
+}
+
 template <int FMT>
 int encode_typed(const EncodeParams& p, int dtype, bool activations, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.tasks + kWarps - 1) / kWarps));
+  const dim3 grid = grid_of((p.k_tiles * 4 * block_of(FMT) + 511) / 512, p.row_groups, p.batch);
   if (dtype == kF16)
     RB200_CUDA(launch_dependent(encode_fp4_kernel<FMT, __half>, grid, kWarps * 32, 0, stream, p, activations));
   else if (dtype == kBf16)
@@ -272,7 +334,7 @@ int encode_typed(const EncodeParams& p, int dtype, bool activations, cudaStream_
 }
 template <int FMT>
 int decode_typed(const DecodeParams& p, int dtype, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.tasks + kWarps - 1) / kWarps));
+  const dim3 grid = grid_of((p.k + 511) / 512, p.row_groups, p.batch);
   if (dtype == kF16) RB200_CUDA(launch_dependent(decode_fp4_kernel<FMT, __half>, grid, kWarps * 32, 0, stream, p));
   else if (dtype == kBf16) RB200_CUDA(launch_dependent(decode_fp4_kernel<FMT, __nv_bfloat16>, grid, kWarps * 32, 0, stream, p));
   else RB200_CUDA(launch_dependent(decode_fp4_kernel<FMT, float>, grid, kWarps * 32, 0, stream, p));
@@ -290,16 +352,14 @@ int fp4_encode_launch(const void* x, int dtype, int64_t batch, int64_t rows, int
   p.ldx = ldx;
   p.batch_stride = batch_stride;
   p.rows = rows;
-  p.rows_padded = scale_row_tiles(rows) * 128;
+  p.row_groups = scale_row_tiles(rows) * (128 / kRowsPerCta);
+  p.batch = batch;
   p.k = (int)k;
   p.k_tiles = (int)scale_k_tiles(k, fmt);
-  p.spans = (p.k_tiles * 4 * block_of(fmt) + 511) / 512;
-  p.tasks = batch * p.rows_padded * p.spans;
   p.ts = tensor_scale;
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
-  if (p.tasks == 0) return 0;
-  RB200_CHECK((p.tasks + kWarps - 1) / kWarps < (1ll << 31), "too many elements to quantise in one call");
+  if (batch == 0 || rows == 0) return 0;
   return fmt == kMx ? encode_typed<kMx>(p, dtype, activations, stream) : encode_typed<kNv>(p, dtype, activations, stream);
 }
 
@@ -342,14 +402,13 @@ int rb200_decode_fp4(const void* codes, const void* scales, int64_t batch, int64
   p.codes = static_cast<const uint8_t*>(codes);
   p.scales = static_cast<const uint8_t*>(scales);
   p.rows = rows;
-  p.rows_padded = f4::scale_row_tiles(rows) * 128;
+  p.row_groups = (rows + kRowsPerCta - 1) / kRowsPerCta;
+  p.row_tiles = f4::scale_row_tiles(rows);
+  p.batch = batch;
   p.k = (int)k;
   p.k_tiles = (int)f4::scale_k_tiles(k, format);
-  p.spans = (int)((k + 511) / 512);
-  p.tasks = batch * rows * p.spans;
   p.ts = tensor_scale;
   p.out = out;
-  RB200_CHECK((p.tasks + kWarps - 1) / kWarps < (1ll << 31), "too many elements to read back in one call");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return format == f4::kMx ? decode_typed<f4::kMx>(p, dtype, s) : decode_typed<f4::kNv>(p, dtype, s);
 }
