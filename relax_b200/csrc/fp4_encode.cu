@@ -27,9 +27,18 @@ template <class T>
 struct Sixteen {
   static constexpr int kVectors = sizeof(T);  // of 16 bytes
   uint4 raw[kVectors];
-  __device__ __forceinline__ void load(const T* p) {
+  __device__ __forceinline__ void load(const T* p, bool wide) {
+    if (wide) {  // 32-byte loads: the lanes' halves of a sector in one request
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+      for (int i = 0; i < kVectors; i += 2)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w), "=r"(raw[i + 1].x), "=r"(raw[i + 1].y),
+                       "=r"(raw[i + 1].z), "=r"(raw[i + 1].w)
+                     : "l"(reinterpret_cast<const uint4*>(p) + i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -87,6 +96,17 @@ __device__ __forceinline__ uint32_t e4m3_of(double r) {
   float f = __double2float_rz(up);
   if (up - (double)f > r * 0x1p-45) f = __uint_as_float(__float_as_uint(f) | 1u);
   return to_e4m3(f);
+}
+
+// The same from fp32 where that settles it: the quotient once too small, once too large.
+__device__ __forceinline__ uint32_t e4m3_of(float top, float per_six, double per_six_exact) {
+  const float r = top * per_six;
+  if (r >= 0x1p-12f && r <= 0x1p12f) {
+    uint16_t two;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(r * (1.0f + 0x1p-21f)), "f"(r * (1.0f - 0x1p-21f)));
+    if ((two & 0xffu) == (two >> 8)) return two & 0x7fu;
+  }
+  return e4m3_of((double)top * per_six_exact);
 }
 
 // The border between codes c and c + 1 (magnitudes).
@@ -169,7 +189,7 @@ struct EncodeParams {
   int64_t ldx, batch_stride;
   int64_t rows, row_groups;  // groups of kRowsPerCta, scale tiles' padding rows among them
   int64_t batch;
-  int k, k_tiles;
+  int k, k_tiles, wide;
   const float* ts;
   uint8_t* codes;
   uint8_t* scales;
@@ -187,7 +207,8 @@ __global__ void __launch_bounds__(kWarps * 32) encode_fp4_kernel(const EncodePar
   for (int64_t e = blockIdx.z; e < p.batch; e += gridDim.z) {
     const float ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
     const bool bad = FMT == kNv && !(ts > 0.0f && ts <= 3.402823466e38f);
-    const double per_six = FMT == kNv ? 1.0 / (6.0 * (double)ts) : 0.0;
+    const double per_six_exact = FMT == kNv ? 1.0 / (6.0 * (double)ts) : 0.0;
+    const float per_six = (float)per_six_exact;
     uint8_t* scales = p.scales + e * (p.row_groups * kRowsPerCta / 128) * p.k_tiles * 512;
     for (int64_t group = blockIdx.y; group < p.row_groups; group += gridDim.y) {
 #pragma unroll 1
@@ -197,7 +218,7 @@ __global__ void __launch_bounds__(kWarps * 32) encode_fp4_kernel(const EncodePar
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           if (row + j * kWarps < p.rows && k0 < p.k)
-            v[j].load(static_cast<const T*>(p.x) + e * p.batch_stride + (row + j * kWarps) * p.ldx + k0);
+            v[j].load(static_cast<const T*>(p.x) + e * p.batch_stride + (row + j * kWarps) * p.ldx + k0, p.wide != 0);
           else
             v[j].clear();
         }
@@ -212,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32) encode_fp4_kernel(const EncodePar
             byte = top >> 23;
             byte = byte > 2u ? byte - 2u : 0u;
           } else {
-            byte = nan ? 0u : e4m3_of((double)__uint_as_float(top) * per_six);
+            byte = nan ? 0u : e4m3_of(__uint_as_float(top), per_six, per_six_exact);
           }
           uint32_t c[2] = {0u, 0u};
           if (nan) byte = FMT == kMx ? 255u : 0x7fu;
@@ -242,10 +263,10 @@ struct DecodeParams {
 };
 
 template <class T>
-__device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-  for (int i = 0; i < 16 / kPer; ++i) {
+  for (int i = 0; i < 8 / kPer; ++i) {
     __align__(16) T t[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) t[j] = narrow<T>(v[i * kPer + j]);
@@ -253,44 +274,49 @@ __device__ __forceinline__ void store16(T* p, const float (&v)[16]) {
   }
 }
 
+// A warp takes 512 k of a row, a lane eight and eight further on by 256: what it stores is next to its neighbours'.
 template <int FMT, class T>
 __global__ void __launch_bounds__(kWarps * 32) decode_fp4_kernel(const DecodeParams p) {
   constexpr int kAhead = 4;
   griddep_wait();
-  const int warp = threadIdx.x >> 5, seg = (int)blockIdx.x * 32 + (threadIdx.x & 31), k0 = seg * 16, blk = FMT == kMx ? seg >> 1 : seg;
-  if (k0 >= p.k) return;
+  const int warp = threadIdx.x >> 5, k0 = (int)blockIdx.x * 512 + (threadIdx.x & 31) * 8;
   for (int64_t e = blockIdx.z; e < p.batch; e += gridDim.z) {
     const float ts = FMT == kNv && p.ts ? p.ts[e] : 1.0f;
     const uint8_t* scales = p.scales + e * p.row_tiles * p.k_tiles * 512;
     for (int64_t group = blockIdx.y; group < p.row_groups; group += gridDim.y) {
-      uint2 c[kAhead];
-      uint32_t byte[kAhead];
+      uint32_t c[kAhead][2], byte[kAhead][2];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int64_t r = group * kRowsPerCta + j * kWarps + warp;
-        if (r < p.rows) {
-          c[j] = *reinterpret_cast<const uint2*>(p.codes + (e * p.rows + r) * (int64_t)(p.k / 2) + k0 / 2);
-          byte[j] = scales[scale_word(r, blk >> 2, p.k_tiles) + (blk & 3)];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = k0 + h * 256, blk = k / block_of(FMT);
+          if (r < p.rows && k < p.k) {
+            c[j][h] = *reinterpret_cast<const uint32_t*>(p.codes + (e * p.rows + r) * (int64_t)(p.k / 2) + k / 2);
+            byte[j][h] = scales[scale_word(r, blk >> 2, p.k_tiles) + (blk & 3)];
+          }
         }
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int64_t r = group * kRowsPerCta + j * kWarps + warp;
-        if (r >= p.rows) break;
-        const float s = scale_value<FMT>(byte[j]);
-        float v[16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t w[4];
-          from_codes8(h ? c[j].y : c[j].x, w);
+          const int k = k0 + h * 256;
+          if (r < p.rows && k < p.k) {
+            const float s = scale_value<FMT>(byte[j][h]);
+            uint32_t w[4];
+            from_codes8(c[j][h], w);
+            float v[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            v[8 * h + 2 * i] = FMT == kMx ? f.x * s : f.x * s * ts;  // code * scale is exact in fp32
-            v[8 * h + 2 * i + 1] = FMT == kMx ? f.y * s : f.y * s * ts;
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+              v[2 * i] = FMT == kMx ? f.x * s : f.x * s * ts;  // code * scale is exact in fp32
+              v[2 * i + 1] = FMT == kMx ? f.y * s : f.y * s * ts;
+            }
+            store8(static_cast<T*>(p.out) + (e * p.rows + r) * (int64_t)p.k + k, v);
           }
         }
-        store16(static_cast<T*>(p.out) + (e * p.rows + r) * (int64_t)p.k + k0, v);
       }
     }
   }
@@ -356,6 +382,8 @@ int fp4_encode_launch(const void* x, int dtype, int64_t batch, int64_t rows, int
   p.batch = batch;
   p.k = (int)k;
   p.k_tiles = (int)scale_k_tiles(k, fmt);
+  const int64_t width = dtype == kF32 ? 4 : 2;
+  p.wide = reinterpret_cast<uintptr_t>(x) % 32 == 0 && ldx * width % 32 == 0 && batch_stride * width % 32 == 0;
   p.ts = tensor_scale;
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
