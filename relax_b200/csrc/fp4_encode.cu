@@ -196,8 +196,8 @@ struct EncodeParams {
 };
 
 template <int FMT, class T>
-__global__ void __launch_bounds__(kWarps * 32) encode_fp4_kernel(const EncodeParams p, bool activations) {
-  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1, kAhead = 2;  // rows on their way
+__global__ void __launch_bounds__(kWarps * 32, FMT == kMx ? 4 : 6) encode_fp4_kernel(const EncodeParams p, bool activations) {
+  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1, kAhead = FMT == kMx ? 2 : 1;  // rows on their way (kNv: its instructions bound it)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seg = (int)blockIdx.x * 32 + lane, k0 = seg * 16, q = seg / (4 * kLanesPerBlock);
   griddep_wait();
