@@ -14,6 +14,7 @@
 #include "fp4_gemm.h"
 #include "fp4_mma.cuh"
 #include "fp4_out.cuh"
+#include "fp4_quant.cuh"
 #include "tensormap.h"
 
 namespace rb200 {
@@ -43,23 +44,27 @@ struct Params {
   const uint8_t* w_scales;
   int k, k_tiles;
   int nb, stages, tmem_cols, m_tiles, cluster, early;
+  const void* x;  // QX: the batch as it is, of out's type
+  int64_t ldx;
 };
 
 size_t stage_bytes(int fmt, int nb) {
-  return (size_t)kWBytes + (size_t)nb * 128 + (size_t)stage_tiles(fmt) * 512 * (1 + (nb + 127) / 128);
+  return (size_t)kWBytes + (size_t)nb * 128 + (size_t)stage_tiles(fmt) * 512 * 2;
 }
 size_t smem_bytes(int fmt, int nb, int stages) { return 1024 + stages * stage_bytes(fmt, nb) + (2 * kMaxStages + 2) * 8 + 32; }
 
-template <int FMT, class T>
+// QX: `a` is quantised here, by the warps that have nothing to do before the epilogue, one chunk a warp.
+template <int FMT, class T, bool QX>
 __global__ void __launch_bounds__(kThreads)
     fp4_gemm_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a) {
   constexpr int NT = stage_tiles(FMT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int nb = p.nb, stages = p.stages, a_bytes = nb * 128, a_tiles = (nb + 127) / 128;
-  const int code_bytes = kWBytes + a_bytes, scale_bytes = NT * 512 * (1 + a_tiles);
+  const int nb = p.nb, stages = p.stages;
+  const int code_bytes = kWBytes + nb * 128;
+  constexpr int scale_bytes = NT * 512 * 2;
   uint8_t* codes = smem;                                   // [stage][w | a]
-  uint8_t* scales = smem + (size_t)stages * code_bytes;    // [stage][w tiles | a tiles of the first 128 rows | of the next]
+  uint8_t* scales = smem + (size_t)stages * code_bytes;    // [stage][w tiles | a tiles]
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + (size_t)stages * scale_bytes);
   uint64_t* empty = full + kMaxStages;
   uint64_t* d_full = empty + kMaxStages;
@@ -73,7 +78,7 @@ __global__ void __launch_bounds__(kThreads)
 
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], QX ? 2 : 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(d_full, 1);
@@ -100,17 +105,15 @@ __global__ void __launch_bounds__(kThreads)
     auto tiles_of = [&](int c) { return (uint32_t)min(NT, p.k_tiles - c * NT) * 512u; };
     auto load_w = [&](int s, int c) {
       uint8_t* at = scales + (size_t)s * scale_bytes;
-      mbar_arrive_expect_tx(&full[s], (uint32_t)code_bytes + tiles_of(c) * (1 + a_tiles));
+      mbar_arrive_expect_tx(&full[s], (uint32_t)(QX ? kWBytes : code_bytes) + tiles_of(c) * (QX ? 1 : 2));
       tma_load(codes + (size_t)s * code_bytes, &tmap_w, c * 128, n0, &full[s]);
       bulk_g2s(at, p.w_scales + ((int64_t)(n0 >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c), &full[s]);
     };
     auto load_a = [&](int s, int c) {
+      if (QX) return;
       uint8_t* at = scales + (size_t)s * scale_bytes + NT * 512;
       tma_load(codes + (size_t)s * code_bytes + kWBytes, &tmap_a, c * 128, m0, &full[s]);
-      for (int i = 0; i < a_tiles; ++i)
-        // (a second tile of 128 rows that the batch does not reach: the first one again, its rows are never stored)
-        bulk_g2s(at + i * NT * 512, p.a_scales + ((int64_t)min((m0 >> 7) + i, (p.o.m - 1) >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c),
-                 &full[s]);
+      bulk_g2s(at, p.a_scales + ((int64_t)(m0 >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c), &full[s]);
     };
     const int first = min(stages, c1 - c0);  // stages filled before any is free again
     if (leader) {
@@ -151,27 +154,30 @@ __global__ void __launch_bounds__(kThreads)
     // ============================================================ scales into tensor memory, MMAs
     const bool leader = elect_one();
     const uint32_t idesc = mma_desc<FMT>(kTileN, nb);
+    const uint64_t w_desc0 = make_b_desc(smem_u32(codes)), sc0 = scale_desc(smem_u32(scales));
     int s = 0;
     uint32_t ph = 0;
     for (int c = c0; c < c1; ++c) {
-      if (!mbar_wait_parked(&full[s], ph, &g_status)) {
-        ok = false;
-        break;
-      }
+      ok = mbar_wait_parked(&full[s], ph, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc_fence_after();
       if (leader) {
-        const uint64_t w_desc = make_b_desc(smem_u32(codes + (size_t)s * code_bytes));
-        const uint64_t a_desc = w_desc + (uint64_t)(kWBytes >> 4);
-        const uint64_t sc = scale_desc(smem_u32(scales + (size_t)s * scale_bytes));
-        const int tiles = min(NT, p.k_tiles - c * NT), mmas = (min(kStageK, p.k - c * kStageK) + kMmaK - 1) / kMmaK;
-        for (int t = 0; t < tiles; ++t) copy_scales(tmem + w_col + 4 * t, sc + (uint64_t)(t * (512 >> 4)));
-        for (int t = 0; t < tiles; ++t)
-          for (int i = 0; i < a_tiles; ++i)
-            copy_scales(tmem + a_col + (t * a_tiles + i) * 4, sc + (uint64_t)((NT + i * NT + t) * (512 >> 4)));
-        for (int j = 0; j < mmas; ++j) {
+        const uint64_t w_desc = w_desc0 + (uint64_t)(s * (code_bytes >> 4)), a_desc = w_desc + (uint64_t)(kWBytes >> 4);
+        const uint64_t sc = sc0 + (uint64_t)(s * (scale_bytes >> 4));
+        const int mmas = min(kStageK, p.k - c * kStageK + kMmaK - 1) / kMmaK;
+        // (scale tiles past the last k are copied as they lie there; no MMA reads them)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          copy_scales(tmem + w_col + 4 * t, sc + (uint64_t)(t * (512 >> 4)));
+          copy_scales(tmem + a_col + 4 * t, sc + (uint64_t)((NT + t) * (512 >> 4)));
+        }
+#pragma unroll
+        for (int j = 0; j < kStageK / kMmaK; ++j) {
           const int t = FMT == kMx ? j >> 1 : j;
-          mma_scaled<FMT>(tmem, w_desc + j * 2, a_desc + j * 2, FMT == kMx && (j & 1) ? upper_half(idesc) : idesc, tmem + w_col + 4 * t,
-                          tmem + a_col + t * a_tiles * 4, (c > c0 || j > 0) ? 1u : 0u);
+          if (j < mmas)
+            mma_scaled<FMT>(tmem, w_desc + j * 2, a_desc + j * 2, FMT == kMx && (j & 1) ? upper_half(idesc) : idesc, tmem + w_col + 4 * t,
+                            tmem + a_col + 4 * t, (c > c0 || j > 0) ? 1u : 0u);
         }
         tc_commit(&empty[s]);
       }
@@ -183,6 +189,36 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (ok && leader) tc_commit(d_full);
     __syncwarp();
+  } else if (QX) {
+    // ============================================================ the batch's rows, quantised into the stages
+    griddep_wait();
+    const TensorScale<FMT> ts(p.o.a_ts ? *p.o.a_ts : 1.0f);
+    for (int i = warp - 2; i < c1 - c0; i += kThreads / 32 - 2) {
+      const int s = i % stages, c = c0 + i;
+      ok = mbar_wait_parked(&empty[s], ((uint32_t)(i / stages) & 1u) ^ 1u, &g_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint8_t* a = codes + (size_t)s * code_bytes + kWBytes;
+      uint8_t* sc = scales + (size_t)s * scale_bytes + NT * 512;
+      for (int j = lane; j < (p.o.m * 16 + 31) / 32 * 32; j += 32) {  // (whole warps: lanes exchange maxima)
+        const int row = j >> 4, seg = j & 15, k = c * kStageK + seg * 16;
+        Sixteen<T> v;
+        const bool real = row < p.o.m && k < p.k;
+        if (real) v.load(static_cast<const T*>(p.x) + row * p.ldx + k, false);
+        else v.clear();
+        uint32_t q[2];
+        const uint32_t byte = quantise<FMT>(v, ts, q);
+        if (row < p.o.m) {
+          // 128-byte rows, their 16-byte columns swizzled as the tensor maps do it
+          *reinterpret_cast<uint2*>(a + row * 128 + (((seg >> 1) ^ (row & 7)) << 4) + (seg & 1) * 8) = make_uint2(q[0], q[1]);
+          const int blk = FMT == kMx ? seg >> 1 : seg;
+          if (FMT == kNv || (seg & 1) == 0) sc[(blk >> 2) * 512 + (row & 31) * 16 + (blk & 3)] = (uint8_t)(real ? byte : 0u);
+        }
+      }
+      fence_proxy_async();  // the tensor cores read it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+    }
   }
 
   // ============================================================ the tile, by batch rows: [nb][128] fp32 where the stages were
@@ -252,9 +288,17 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kMaxDevices = 64;
 std::atomic<bool> g_launched[kMaxDevices];  // devices whose status word a wait may have set
 
-template <int FMT, class T>
+// CTAs that share a tile's k: as many as leave two CTAs an SM and two chunks each
+int cluster_of(int tiles, int64_t k) {
+  const int chunks = (int)((k + kStageK - 1) / kStageK);
+  int c = 1;
+  while (c < 8 && tiles * c * 2 <= 2 * sm_count_current() && chunks >= 4 * c) c *= 2;
+  return c;
+}
+
+template <int FMT, class T, bool QX>
 int launch_typed(Params& p, const CUtensorMap& tw, const CUtensorMap& ta, cudaStream_t stream) {
-  auto kern = fp4_gemm_kernel<FMT, T>;
+  auto kern = fp4_gemm_kernel<FMT, T, QX>;
   static thread_local int configured_device = -1;
   int dev = 0;
   RB200_CUDA(cudaGetDevice(&dev));
@@ -262,9 +306,8 @@ int launch_typed(Params& p, const CUtensorMap& tw, const CUtensorMap& ta, cudaSt
     RB200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     configured_device = dev;
   }
-  const int n_tiles = (p.o.n + kTileN - 1) / kTileN, tiles = n_tiles * p.m_tiles, chunks = (p.k + kStageK - 1) / kStageK;
-  p.cluster = 1;
-  while (p.cluster < 8 && tiles * p.cluster * 2 <= 2 * sm_count_current() && chunks >= 4 * p.cluster) p.cluster *= 2;
+  const int tiles = (p.o.n + kTileN - 1) / kTileN * p.m_tiles;
+  p.cluster = cluster_of(tiles, p.k);
   p.stages = kMaxStages;
   const size_t room = (size_t)(p.nb <= 64 ? 113 : 226) * 1024;  // two CTAs of an SM, or one
   while (p.stages > 2 && smem_bytes(FMT, p.nb, p.stages) > room) --p.stages;
@@ -287,13 +330,22 @@ int launch_typed(Params& p, const CUtensorMap& tw, const CUtensorMap& ta, cudaSt
   return 0;
 }
 
-template <int FMT>
+template <int FMT, bool QX>
 int launch_fmt(Params& p, int dtype, const CUtensorMap& tw, const CUtensorMap& ta, cudaStream_t stream) {
   switch (dtype) {
-    case kF16: return launch_typed<FMT, __half>(p, tw, ta, stream);
-    case kBf16: return launch_typed<FMT, __nv_bfloat16>(p, tw, ta, stream);
-    default: return launch_typed<FMT, float>(p, tw, ta, stream);
+    case kF16: return launch_typed<FMT, __half, QX>(p, tw, ta, stream);
+    case kBf16: return launch_typed<FMT, __nv_bfloat16, QX>(p, tw, ta, stream);
+    default: return launch_typed<FMT, float, QX>(p, tw, ta, stream);
   }
+}
+
+// Few rows are quantised by the product's CTAs, each its share of k for itself, where that takes less than a kernel before it:
+// one or two rows (k 4096 x n 4096: 8.3 -> 6.2 us; k 28672 x n 8192: 25.1 -> 23.0), and more where a CTA's four warps have at
+// most four turns of 256 k x two rows each (n 4096, eight rows, two turns of two: 8.6 -> 7.9; n 11008, eight turns: 10.9 -> 12.2).
+bool quantises_itself(int64_t m, int64_t n, int64_t k) {
+  if (m <= 2) return true;
+  const int tiles = (int)((n + kTileN - 1) / kTileN), per = (int)((k + kStageK - 1) / kStageK + cluster_of(tiles, k) - 1) / cluster_of(tiles, k);
+  return m <= 16 && (per + 3) / 4 * ((m + 1) / 2) <= 4;
 }
 
 }  // namespace
@@ -315,12 +367,8 @@ int fp4_gemm_read_status(int* status_out) {
   return 0;
 }
 
-int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
+static int fp4_few_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t ldx, cudaStream_t stream) {
   using namespace f4;
-  int dev = 0;
-  RB200_CUDA(cudaGetDevice(&dev));
-  if (dev >= 0 && dev < kMaxDevices) g_launched[dev].store(true, std::memory_order_relaxed);
-  if (d.m > 128) return fp4_pair_launch(d, stream);
   Params p;
   memset(&p, 0, sizeof(p));
   p.o = output_of(d);
@@ -329,17 +377,31 @@ int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
   p.k = (int)d.k;
   p.k_tiles = (int)scale_k_tiles(d.k, d.format);
   p.early = launch_overlap_enabled() ? 1 : 0;
-  p.nb = d.m <= 256 ? (int)((d.m + 15) / 16 * 16) : 256;
+  p.nb = d.m <= 128 ? (int)((d.m + 15) / 16 * 16) : 128;
   p.m_tiles = (int)((d.m + p.nb - 1) / p.nb);
-  const int cols = (p.nb + 31) / 32 * 32 + 4 * stage_tiles(d.format) * (1 + (p.nb + 127) / 128);
-  p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
+  const int cols = (p.nb + 31) / 32 * 32 + 4 * stage_tiles(d.format) * 2;
+  p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
   CUtensorMap tw, ta;
   if (make_tensor_map_2d(&tw, d.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.n,
                          (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0 ||
-      make_tensor_map_2d(&ta, d.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.m,
-                         (unsigned long long)d.k / 2, 128, (unsigned)p.nb, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+      (!x &&
+       make_tensor_map_2d(&ta, d.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.m,
+                          (unsigned long long)d.k / 2, 128, (unsigned)p.nb, CU_TENSOR_MAP_SWIZZLE_128B) != 0))
     return -1;
-  return d.format == kMx ? launch_fmt<kMx>(p, d.out_dtype, tw, ta, stream) : launch_fmt<kNv>(p, d.out_dtype, tw, ta, stream);
+  if (x) {
+    ta = tw;
+    p.x = x;
+    p.ldx = ldx;
+    return d.format == kMx ? launch_fmt<kMx, true>(p, d.out_dtype, tw, ta, stream) : launch_fmt<kNv, true>(p, d.out_dtype, tw, ta, stream);
+  }
+  return d.format == kMx ? launch_fmt<kMx, false>(p, d.out_dtype, tw, ta, stream) : launch_fmt<kNv, false>(p, d.out_dtype, tw, ta, stream);
+}
+
+int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t ldx, cudaStream_t stream) {
+  int dev = 0;
+  RB200_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < f4::kMaxDevices) f4::g_launched[dev].store(true, std::memory_order_relaxed);
+  return d.m > 128 ? fp4_pair_launch(d, stream) : fp4_few_launch(d, x, ldx, stream);
 }
 
 }  // namespace rb200
@@ -378,7 +440,7 @@ int rb200_gemm_fp4(const rb200_gemm_fp4_desc* d, void* stream) {
   if (check_gemm(d) != 0) return -1;
   if (d->m == 0) return 0;
   RB200_CHECK(d->a && d->a_scales && aligned16(d->a) && aligned16(d->a_scales), "a and a_scales must be non-NULL and 16-byte aligned");
-  return fp4_gemm_launch(*d, static_cast<cudaStream_t>(stream));
+  return fp4_gemm_launch(*d, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
 
 size_t rb200_linear_fp4_workspace_bytes(int64_t m, int64_t k, int format) {
@@ -398,6 +460,7 @@ int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb200_gemm_f
   RB200_CHECK(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                   workspace_bytes >= rb200_linear_fp4_workspace_bytes(d.m, d.k, d.format),
               "the workspace must be 256-byte aligned and hold rb200_linear_fp4_workspace_bytes");
+  if (x_dtype == d.out_dtype && f4::quantises_itself(d.m, d.n, d.k)) return fp4_gemm_launch(d, x, ldx, static_cast<cudaStream_t>(stream));
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + (d.m * (d.k / 2) + 255) / 256 * 256;
   if (fp4_encode_launch(x, x_dtype, 1, d.m, d.k, ldx, 0, d.format, d.a_tensor_scale, codes, scales, true,
@@ -405,7 +468,7 @@ int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb200_gemm_f
     return -1;
   d.a = codes;
   d.a_scales = scales;
-  return fp4_gemm_launch(d, static_cast<cudaStream_t>(stream));
+  return fp4_gemm_launch(d, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -280,7 +280,7 @@ def test_gemm_keeps_a_bad_row_to_itself(fmt):
 
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
-@pytest.mark.parametrize("m, n, k, dtype", [(1, 512, 1024, "fp16"), (9, 300, 544, "bf16"), (65, 129, 96, "fp16"), (300, 256, 2048, "fp32")])
+@pytest.mark.parametrize("m, n, k, dtype", [(1, 512, 1024, "fp16"), (2, 4096, 4096, "bf16"), (9, 300, 544, "bf16"), (16, 130, 2080, "fp32"), (13, 257, 32, "fp16"), (17, 300, 544, "fp16"), (65, 129, 96, "fp16"), (300, 256, 2048, "fp32")])
 def test_linear(fmt, m, n, k, dtype):
     g = _gen(m + n + k)
     x = (torch.randn(m, k, device="cuda", generator=g) * torch.exp(torch.randn(k, device="cuda", generator=g))).to(TYPES[dtype])
