@@ -377,7 +377,7 @@ static int fp4_few_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t l
   p.k = (int)d.k;
   p.k_tiles = (int)scale_k_tiles(d.k, d.format);
   p.early = launch_overlap_enabled() ? 1 : 0;
-  p.nb = d.m <= 128 ? (int)((d.m + 15) / 16 * 16) : 128;
+  p.nb = (int)((d.m + 15) / 16 * 16);
   p.m_tiles = (int)((d.m + p.nb - 1) / p.nb);
   const int cols = (p.nb + 31) / 32 * 32 + 4 * stage_tiles(d.format) * 2;
   p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
@@ -401,7 +401,7 @@ int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t ldx, cu
   int dev = 0;
   RB200_CUDA(cudaGetDevice(&dev));
   if (dev >= 0 && dev < f4::kMaxDevices) f4::g_launched[dev].store(true, std::memory_order_relaxed);
-  return d.m > 128 ? fp4_pair_launch(d, stream) : fp4_few_launch(d, x, ldx, stream);
+  return d.m > 64 ? fp4_pair_launch(d, stream) : fp4_few_launch(d, x, ldx, stream);
 }
 
 }  // namespace rb200

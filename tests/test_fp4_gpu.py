@@ -188,7 +188,8 @@ def _check_product(got, a, w, alpha=1.0, tail=None):
 
 SHAPES = [(1, 1, 32), (1, 128, 64), (3, 130, 96), (8, 256, 256), (16, 64, 288), (17, 200, 320), (33, 127, 512), (64, 384, 1056),
           (100, 129, 2080), (129, 256, 800), (200, 100, 256), (257, 300, 544), (520, 257, 1024), (1, 4096, 4096), (40, 96, 8192),
-          (1000, 513, 96), (300, 9600, 64), (1300, 4100, 288), (385, 1024, 1536), (256, 128, 32)]
+          (1000, 513, 96), (300, 9600, 64), (1300, 4100, 288), (385, 1024, 1536), (256, 128, 32),
+          (70, 300, 4096), (128, 257, 8224), (333, 2600, 3104), (600, 9500, 2592)]
 
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
