@@ -359,7 +359,8 @@ RB200_API int rb200_preprocess_fp4_scales(const void* src, void* dst, int64_t ba
  *   rb200_linear_fp4  quantises x [m, k] (F16, BF16 or F32) first, as rb200_encode_fp4 does; desc->a and a_scales are not
  *                     read; workspace: rb200_linear_fp4_workspace_bytes(m, k, format) bytes, 256-byte aligned, of the call's
  *                     own until it has run.
- * Nothing is allocated.  With launch overlap on, w and w_scales are read ahead of the previous kernel's end.
+ * Nothing is allocated.  With launch overlap on, w and w_scales are read ahead of the previous kernel's end.  out must not
+ * overlap what is read, but may be the residual itself.
  */
 typedef struct rb200_gemm_fp4_desc {
   uint32_t struct_size;         /* sizeof(rb200_gemm_fp4_desc) */
@@ -395,7 +396,8 @@ RB200_API int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb
  * rows first; w_down codes [num_experts, hidden, ffn / 2]; scales of each expert in tiles, experts after one another;
  * tensor scales [num_experts] (nv only; NULL: 1).  hidden and ffn multiples of 64, num_experts <= 256, top_k <= 8.
  * workspace: rb200_moe_layer_fp4_workspace_bytes(tokens, top_k, hidden, ffn) bytes, of the call's own until it has run.
- * The weights, scales and logits must not be written between this call and its end.
+ * The weights, scales and logits must not be written between this call and its end; out may be x.  Sums are put together in an
+ * order that depends on the batch's routing, the GPU's SM count and whether hand-over words were to be had, never on timing.
  * Takes the place of rb200_moe_route, rb200_moe_gather, two grouped matmuls and rb200_moe_combine.
  */
 typedef struct rb200_moe_layer_fp4_desc {

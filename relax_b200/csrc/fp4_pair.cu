@@ -401,6 +401,8 @@ int fp4_pair_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
   p.k = (int)d.k;
   p.k_tiles = (int)scale_k_tiles(d.k, d.format);
   p.early = launch_overlap_enabled() ? 1 : 0;
+  RB200_CHECK((d.n + 2 * kTileN - 1) / (2 * kTileN) * ((d.m + kNb - 1) / kNb) < (1ll << 30), "the product is too large (m=%lld, n=%lld)", (long long)d.m,
+              (long long)d.n);
   p.n_tiles = (int)((d.n + 2 * kTileN - 1) / (2 * kTileN));
   p.m_tiles = (int)((d.m + kNb - 1) / kNb);
   // Two tiles of a, the second one usually smaller: all the large ones first.  More: neighbours share a tile of w.
