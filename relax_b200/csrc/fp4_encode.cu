@@ -18,12 +18,14 @@ namespace {
 using namespace f4;
 
 constexpr int kWarps = 8;
-constexpr int kRowsPerCta = 32;  // a CTA's rows, of 512 k
+constexpr int kRowsPerCta = 32;  // a CTA's rows, of 512 k (the quantiser's, of a small input: fewer)
 
 struct EncodeParams {
   const void* x;
   int64_t ldx, batch_stride;
-  int64_t rows, row_groups;  // groups of kRowsPerCta, scale tiles' padding rows among them
+  int64_t rows, row_groups;  // groups of turns * kWarps, scale tiles' padding rows among them
+  int64_t scale_stride;      // bytes from matrix to matrix
+  int turns;                 // rows of a warp
   int64_t batch;
   int k, k_tiles, wide;
   const float* ts;
@@ -31,9 +33,14 @@ struct EncodeParams {
   uint8_t* scales;
 };
 
+template <int FMT>
+constexpr int kCtas = FMT == kMx ? 4 : 6;  // of an SM
+template <int FMT>
+constexpr int kRowsAhead = FMT == kMx ? 2 : 1;  // rows on their way to a warp (kNv: its instructions bound it)
+
 template <int FMT, class T>
-__global__ void __launch_bounds__(kWarps * 32, FMT == kMx ? 4 : 6) encode_fp4_kernel(const EncodeParams p, bool activations) {
-  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1, kAhead = FMT == kMx ? 2 : 1;  // rows on their way (kNv: its instructions bound it)
+__global__ void __launch_bounds__(kWarps * 32, kCtas<FMT>) encode_fp4_kernel(const EncodeParams p, bool activations) {
+  constexpr int kLanesPerBlock = FMT == kMx ? 2 : 1, kAhead = kRowsAhead<FMT>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seg = (int)blockIdx.x * 32 + lane, k0 = seg * 16, q = seg / (4 * kLanesPerBlock);
   griddep_wait();
@@ -42,11 +49,11 @@ __global__ void __launch_bounds__(kWarps * 32, FMT == kMx ? 4 : 6) encode_fp4_ke
   if (activations) griddep_launch_dependents();
   for (int64_t e = blockIdx.z; e < p.batch; e += gridDim.z) {
     const TensorScale<FMT> ts(p.ts ? p.ts[e] : 1.0f);
-    uint8_t* scales = p.scales + e * (p.row_groups * kRowsPerCta / 128) * p.k_tiles * 512;
+    uint8_t* scales = p.scales + e * p.scale_stride;
     for (int64_t group = blockIdx.y; group < p.row_groups; group += gridDim.y) {
 #pragma unroll 1
-      for (int i = 0; i < kRowsPerCta / kWarps; i += kAhead) {
-        const int64_t row = group * kRowsPerCta + i * kWarps + warp;
+      for (int i = 0; i < p.turns; i += kAhead) {
+        const int64_t row = (group * p.turns + i) * kWarps + warp;
         Sixteen<T> v[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
@@ -170,8 +177,15 @@ dim3 grid_of(int spans, int64_t row_groups, int64_t batch) {
 }
 
 template <int FMT>
-int encode_typed(const EncodeParams& p, int dtype, bool activations, cudaStream_t stream) {
-  const dim3 grid = grid_of((p.k_tiles * 4 * block_of(FMT) + 511) / 512, p.row_groups, p.batch);
+int encode_typed(EncodeParams& p, int dtype, bool activations, cudaStream_t stream) {
+  // A warp's rows come one after another (kMx: two by two), each a trip to memory: as few as fill the SMs once
+  // (kNv, 48 rows of 28672: 8.9 us with four, 4.8 with one; 256 of 4096: 7.5 and 4.2).
+  const int spans = (p.k_tiles * 4 * block_of(FMT) + 511) / 512;
+  const int64_t room = (int64_t)kCtas<FMT> * sm_count_current();
+  p.turns = kRowsPerCta / kWarps;
+  while (p.turns > kRowsAhead<FMT> && p.rows * spans * p.batch <= room * kWarps * (p.turns / 2)) p.turns /= 2;
+  p.row_groups = scale_row_tiles(p.rows) * 128 / (p.turns * kWarps);
+  const dim3 grid = grid_of(spans, p.row_groups, p.batch);
   if (dtype == kF16)
     RB200_CUDA(launch_dependent(encode_fp4_kernel<FMT, __half>, grid, kWarps * 32, 0, stream, p, activations));
   else if (dtype == kBf16)
@@ -200,10 +214,10 @@ int fp4_encode_launch(const void* x, int dtype, int64_t batch, int64_t rows, int
   p.ldx = ldx;
   p.batch_stride = batch_stride;
   p.rows = rows;
-  p.row_groups = scale_row_tiles(rows) * (128 / kRowsPerCta);
   p.batch = batch;
   p.k = (int)k;
   p.k_tiles = (int)scale_k_tiles(k, fmt);
+  p.scale_stride = scale_row_tiles(rows) * p.k_tiles * 512;
   const int64_t width = dtype == kF32 ? 4 : 2;
   p.wide = reinterpret_cast<uintptr_t>(x) % 32 == 0 && ldx * width % 32 == 0 && batch_stride * width % 32 == 0;
   p.ts = tensor_scale;

@@ -1,11 +1,16 @@
 // out = unary(binary(act(ta tw sum_k a[m, k] w[n, k] + bias[n]), residual[m, n])) of two microscaled 4-bit operands.
 //
-// The tensor cores take codes and block scales as they are (tcgen05.mma, block_scale): nothing is decoded.  The tile is
-// out^T, 128 rows of w by nb rows of a, so that a batch of any size is the MMA's N; a stage is 256 k: two tensor-map loads of
-// codes and the scale tiles, which the MMA's thread copies into tensor memory ahead of the MMAs that read them.
+// The tensor cores take codes and block scales as they are (tcgen05.mma, block_scale): nothing is decoded.  Here are batches
+// of at most 64 rows, fp4_pair.cu has the larger ones.  The tile is out^T, 128 rows of w by the batch (nb, rounded up to 16,
+// is the MMA's N); a stage is 256 k: two tensor-map loads of codes and the scale tiles, which the MMA's thread copies into
+// tensor memory ahead of the MMAs that read them.
 // With few tiles k is cut over the CTAs of a cluster: each keeps its partial tile in shared memory (the stages' memory, done
 // with by then), and each adds up its share of the batch rows in the order of the ranks, so that a result does not depend
 // on timing.
+//
+// What bounds it is reading w once: k 28672 x n 8192 in the mx format, 125 MB, takes 21.5 us for one row (5.8 TB/s) out of
+// memory; two CTAs an SM keep some 200 KB on their way there.  Small ones are launch and one trip to memory and back through
+// the cluster: k 4096 x n 4096 in the nv format, 9.4 MB, 6.5 us with everything, of which the reading is 1.5.
 #include <atomic>
 
 #include <cstring>
@@ -43,7 +48,7 @@ struct Params {
   const uint8_t* a_scales;
   const uint8_t* w_scales;
   int k, k_tiles;
-  int nb, stages, tmem_cols, m_tiles, cluster, early;
+  int nb, stages, tmem_cols, cluster, early;
   const void* x;  // QX: the batch as it is, of out's type
   int64_t ldx;
 };
@@ -71,8 +76,7 @@ __global__ void __launch_bounds__(kThreads)
   uint32_t* holder = reinterpret_cast<uint32_t*>(d_full + 2);  // [0] tensor memory, [1] a CTA of the cluster failed
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)cluster_rank(), tile = blockIdx.x / p.cluster;
-  const int m0 = (tile % p.m_tiles) * nb, n0 = (tile / p.m_tiles) * kTileN;
+  const int rank = (int)cluster_rank(), n0 = (int)blockIdx.x / p.cluster * kTileN;
   const int chunks = (p.k + kStageK - 1) / kStageK;
   const int c0 = (int)((int64_t)chunks * rank / p.cluster), c1 = (int)((int64_t)chunks * (rank + 1) / p.cluster);
 
@@ -112,8 +116,8 @@ __global__ void __launch_bounds__(kThreads)
     auto load_a = [&](int s, int c) {
       if (QX) return;
       uint8_t* at = scales + (size_t)s * scale_bytes + NT * 512;
-      tma_load(codes + (size_t)s * code_bytes + kWBytes, &tmap_a, c * 128, m0, &full[s]);
-      bulk_g2s(at, p.a_scales + ((int64_t)(m0 >> 7) * p.k_tiles + c * NT) * 512, tiles_of(c), &full[s]);
+      tma_load(codes + (size_t)s * code_bytes + kWBytes, &tmap_a, c * 128, 0, &full[s]);
+      bulk_g2s(at, p.a_scales + (int64_t)c * NT * 512, tiles_of(c), &full[s]);
     };
     const int first = min(stages, c1 - c0);  // stages filled before any is free again
     if (leader) {
@@ -224,6 +228,14 @@ __global__ void __launch_bounds__(kThreads)
   // ============================================================ the tile, by batch rows: [nb][128] fp32 where the stages were
   float* part = reinterpret_cast<float*>(smem);
   griddep_wait();
+  const float alpha = out_scale(p.o);
+  const int lo = p.o.m * rank / p.cluster, hi = p.o.m * (rank + 1) / p.cluster;  // this CTA's rows of the result
+  const int n = n0 + lane * 4;
+  float bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bias[i] = bias_at<T>(p.o, n + i);
+  if (p.o.residual && n < p.o.n)
+    for (int m = lo + warp; m < hi; m += kThreads / 32) prefetch_line(static_cast<const T*>(p.o.residual) + m * p.o.ld_res + n);
   ok = mbar_wait_parked(d_full, 0, &g_status) && ok;  // every stage has been read
   ok = __all_sync(0xffffffffu, ok);
   if (!ok) {
@@ -235,7 +247,6 @@ __global__ void __launch_bounds__(kThreads)
     const int quad = warp & 3;
     const uint32_t lane_taddr = (uint32_t)(32 * quad) << 16;
     for (int c = 0; c < nb; c += 16) {
-      if (m0 + c >= p.o.m) break;
       float v[16];
       tc_ld16(lane_taddr | (tmem + c), v);
 #pragma unroll
@@ -246,13 +257,10 @@ __global__ void __launch_bounds__(kThreads)
   if (p.cluster > 1) cluster_sync();
   else __syncthreads();
   if (holder[1] == 0u) {
-    const float alpha = out_scale(p.o);
-    const int rows = min(nb, p.o.m - m0), lo = rows * rank / p.cluster, hi = rows * (rank + 1) / p.cluster;
-    const int n = n0 + lane * 4;
     T* out = static_cast<T*>(p.o.out);
     const bool wide = n + 4 <= p.o.n && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && p.o.ldo % 4 == 0;
-    for (int r = lo + warp; r < hi; r += kThreads / 32) {
-      const uint32_t at = smem_u32(part + r * kTileN + lane * 4);
+    for (int m = lo + warp; m < hi; m += kThreads / 32) {
+      const uint32_t at = smem_u32(part + m * kTileN + lane * 4);
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int q = 0; q < p.cluster; ++q) {
         const float4 o = ld_cluster4(p.cluster > 1 ? at_rank(at, q) : at);
@@ -261,11 +269,13 @@ __global__ void __launch_bounds__(kThreads)
         v.z += o.z;
         v.w += o.w;
       }
-      const float f[4] = {v.x, v.y, v.z, v.w};
-      const int m = m0 + r;
+      float f[4] = {v.x, v.y, v.z, v.w};
+      float x[4];
+      if (p.o.residual) load_residual<T, false>(p.o, x, m, n);
+      finish<false>(p.o, f, alpha, bias, x);
       __align__(16) T t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = n + i < p.o.n ? narrow<T>(finish<T>(p.o, f[i], alpha, m, n + i)) : narrow<T>(0.0f);
+      for (int i = 0; i < 4; ++i) t[i] = narrow<T>(f[i]);
       T* dst = out + m * p.o.ldo + n;
       if (wide) {
         if (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
@@ -306,13 +316,11 @@ int launch_typed(Params& p, const CUtensorMap& tw, const CUtensorMap& ta, cudaSt
     RB200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     configured_device = dev;
   }
-  const int tiles = (p.o.n + kTileN - 1) / kTileN * p.m_tiles;
+  const int tiles = (p.o.n + kTileN - 1) / kTileN;
   p.cluster = cluster_of(tiles, p.k);
   p.stages = kMaxStages;
-  const size_t room = (size_t)(p.nb <= 64 ? 113 : 226) * 1024;  // two CTAs of an SM, or one
-  while (p.stages > 2 && smem_bytes(FMT, p.nb, p.stages) > room) --p.stages;
-  size_t smem = smem_bytes(FMT, p.nb, p.stages);
-  RB200_CHECK(smem <= 227 * 1024 && (size_t)p.nb * kTileN * 4 <= p.stages * stage_bytes(FMT, p.nb), "no room for the tile");
+  while (smem_bytes(FMT, p.nb, p.stages) > 113 * 1024) --p.stages;  // two CTAs an SM; three stages or more
+  const size_t smem = smem_bytes(FMT, p.nb, p.stages);  // (three stages hold 48 KB of w, a tile of sums 32)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.cluster), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
@@ -378,9 +386,8 @@ static int fp4_few_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t l
   p.k_tiles = (int)scale_k_tiles(d.k, d.format);
   p.early = launch_overlap_enabled() ? 1 : 0;
   p.nb = (int)((d.m + 15) / 16 * 16);
-  p.m_tiles = (int)((d.m + p.nb - 1) / p.nb);
   const int cols = (p.nb + 31) / 32 * 32 + 4 * stage_tiles(d.format) * 2;
-  p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+  p.tmem_cols = cols <= 64 ? 64 : 128;
   CUtensorMap tw, ta;
   if (make_tensor_map_2d(&tw, d.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.n,
                          (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != 0 ||

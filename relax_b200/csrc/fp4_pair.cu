@@ -29,13 +29,14 @@ constexpr int kDrainWarps = 8;
 constexpr int kTileN = 128;  // rows of w in a CTA
 constexpr int kNb = 256;     // rows of a
 constexpr int kMaxStages = 6;
-constexpr int kStoreBytes = 2048;  // a warp's store: 32 columns by 32 (four-byte types: 16) rows
+constexpr int kRows = 16;    // of a, that a drain warp finishes and stores at once, by 32 columns
+constexpr int kBuffers = 4;  // for that many of them, each warp
 
 __device__ int g_status;
 
 struct Params {
   Output o;
-  int n_tiles, m_tiles, n_first, stages, early, tma_store, k, k_tiles;
+  int n_tiles, m_tiles, n_first, stages, early, tma_store, staged, k;
 };
 
 template <int FMT>
@@ -75,10 +76,10 @@ template <int LEFT>
 __device__ __forceinline__ void stores_read() {  // all but the last LEFT stores have read shared memory
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
 }
-__device__ __forceinline__ void commit2(uint64_t* bar) {  // arrives at both CTAs' barrier
+__device__ __forceinline__ void commit2(uint64_t* bar, int first) {  // arrives at both CTAs' barrier
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)(3 << first))
       : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
@@ -118,7 +119,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {  // 32 col
       : "memory");
 }
 
-template <int FMT, class T>
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// SPLIT: the k of a tile is cut over the two pairs of a cluster.
+template <int FMT, class T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     fp4_pair_kernel(const Params p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
                     const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_as,
@@ -128,16 +142,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int stages = p.stages;
-  uint8_t* store = smem + (size_t)stages * stage_bytes<FMT>();  // [drain warp][2][kStoreBytes]
-  uint64_t* full = reinterpret_cast<uint64_t*>(store + kDrainWarps * 2 * kStoreBytes);  // rank 0's are used
+  T* store = reinterpret_cast<T*>(smem + (size_t)stages * stage_bytes<FMT>());  // [drain warp][kBuffers][kRows][32]
+  uint64_t* full = reinterpret_cast<uint64_t*>(store + kDrainWarps * kBuffers * kRows * 32);  // the first CTA's are used
   uint64_t* empty = full + kMaxStages;
   uint64_t* d_full = empty + kMaxStages;
-  uint64_t* d_empty = d_full + 1;  // rank 0's is used
-  uint32_t* holder = reinterpret_cast<uint32_t*>(d_empty + 1);
+  uint64_t* d_empty = d_full + 1;  // the first CTA's is used
+  uint32_t* holder = reinterpret_cast<uint32_t*>(d_empty + 1);  // [0] tensor memory, [1] a CTA of the cluster failed
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)cluster_rank();
-  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  constexpr int split = SPLIT ? 2 : 1;
+  // rank in the pair, the pair's place in the cluster, its first CTA
+  const int rank = (int)cluster_rank() & 1, part = (int)cluster_rank() >> 1, first = part * 2;
+  const int pair = (int)blockIdx.x / (2 * split), pairs = (int)gridDim.x / (2 * split);
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -145,17 +161,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(d_full, 1);
     mbar_init(d_empty, 2 * kDrainWarps);
+    holder[1] = 0u;
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc2(holder, 512u);
   fence_proxy_async();
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // both CTAs' barriers exist before any remote arrival
+  cluster_sync();  // every CTA's barriers exist before any remote arrival
   tc_fence_after();
   griddep_launch_dependents();
   const uint32_t tmem = holder[0];
   const int chunks = (p.k + kStageK - 1) / kStageK, items = p.n_tiles * p.m_tiles;
+  const int c0 = chunks * part / split, c1 = chunks * (part + 1) / split;
   struct Item {
     int n0, m0, width;  // this CTA's first row of w, the tile's first row of a, columns of the MMA
   };
@@ -168,29 +186,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     return it;
   };
 
+  bool ok = true;
   if (warp == 0) {
     // ============================================================ loads
     const bool leader = elect_one();
     int s = 0;
     uint32_t ph = 1;
-    bool ok = true, waited = false;
+    bool waited = false;
     auto load_w = [&](const Item& it, int c, int s) {
       uint8_t* at = smem + (size_t)s * stage_bytes<FMT>();
-      const uint32_t bar0 = at_rank(smem_u32(&full[s]), 0);
+      const uint32_t bar0 = at_rank(smem_u32(&full[s]), first);
       if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * (uint32_t)stage_bytes<FMT>());
       tma_load2(at, &tmap_w, c * 128, it.n0, bar0);
       tma_load3(at + kWs, &tmap_ws, 0, c * NT, it.n0 >> 7, bar0);
     };
     auto load_a = [&](const Item& it, int c, int s) {
       uint8_t* at = smem + (size_t)s * stage_bytes<FMT>();
-      const uint32_t bar0 = at_rank(smem_u32(&full[s]), 0);
+      const uint32_t bar0 = at_rank(smem_u32(&full[s]), first);
       tma_load2(at + kA, &tmap_a, c * 128, it.m0 + rank * (it.width / 2), bar0);
       tma_load3(at + kAs, &tmap_as, 0, c * NT, it.m0 >> 7, bar0);
     };
     if (!p.early) {
       if (leader && pair < items) {
         const Item it = item_at(pair);
-        for (int c = 0; c < min(stages, chunks); ++c) tma_prefetch(&tmap_w, c * 128, it.n0);
+        for (int c = c0; c < min(c0 + stages, c1); ++c) tma_prefetch(&tmap_w, c * 128, it.n0);
       }
       griddep_wait();
       waited = true;
@@ -198,17 +217,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // before the wait only weights are read: as many stages as there are, in the first tile
     int ahead = 0;
     if (!waited) {
-      ahead = pair < items ? min(stages, chunks) : 0;
+      ahead = pair < items ? min(stages, c1 - c0) : 0;
       if (leader) {
         const Item it = item_at(pair);
-        for (int c = 0; c < ahead; ++c) load_w(it, c, c);
+        for (int c = 0; c < ahead; ++c) load_w(it, c0 + c, c);
       }
       __syncwarp();
       griddep_wait();
     }
     for (int i = pair; ok && i < items; i += pairs) {
       const Item it = item_at(i);
-      for (int c = 0; c < chunks; ++c) {
+      for (int c = c0; c < c1; ++c) {
         ok = mbar_wait_parked(&empty[s], ph, &g_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -238,7 +257,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t w_desc0 = make_b_desc(smem_u32(smem)), ws_desc0 = scale_desc(smem_u32(smem + kWs));
     int s = 0;
     uint32_t ph = 0, dph = 1;
-    bool ok = true;
     for (int i = pair; ok && i < items; i += pairs, dph ^= 1u) {
       const uint32_t idesc = mma_desc<FMT>(256, item_at(i).width);
       const int a_tiles = item_at(i).width > 128 ? 2 : 1;
@@ -246,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      for (int c = 0; c < chunks; ++c) {
+      for (int c = c0; c < c1; ++c) {
         ok = mbar_wait_parked(&full[s], ph, &g_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -267,9 +285,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int t = FMT == kMx ? j >> 1 : j;
             if (j < mmas)
               mma_scaled2<FMT>(tmem, w_desc + j * 2, a_desc + j * 2, FMT == kMx && (j & 1) ? upper_half(idesc) : idesc,
-                               tmem + kWCol + 4 * t, tmem + kACol + 8 * t, (c > 0 || j > 0) ? 1u : 0u);
+                               tmem + kWCol + 4 * t, tmem + kACol + 8 * t, (c > c0 || j > 0) ? 1u : 0u);
           }
-          commit2(&empty[s]);
+          commit2(&empty[s], first);
         }
         __syncwarp();
         if (++s == stages) {
@@ -277,25 +295,85 @@ __global__ void __launch_bounds__(kThreads, 1)
           ph ^= 1u;
         }
       }
-      if (ok && leader) commit2(d_full);
+      if (ok && leader) commit2(d_full, first);
       __syncwarp();
     }
-  } else if (warp >= 4) {
-    // ============================================================ drain
-    const int dw = warp - 4, quad = warp & 3, half = dw >> 2;
-    uint8_t* mine = store + dw * 2 * kStoreBytes;
-    const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(half * 128);
+  }
+
+  // ============================================================ drain
+  const int dw = warp - 4, quad = warp & 3, half = dw >> 2;
+  T* mine = store + dw * kBuffers * kRows * 32;
+  const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(half * 128);
+  // A warp's columns of the accumulator (rows of a) by kRows of them.  SPLIT: of its four groups of 32 columns the first pair
+  // has the even ones, the second the odd ones.
+  constexpr int kTurns = SPLIT ? 4 : 8;
+  auto column = [&](int turn) { return SPLIT ? (turn >> 1) * 64 + part * 32 + (turn & 1) * kRows : turn * kRows; };
+  auto rows_of = [&](const Item& it) { return min(128, p.o.m - it.m0 - half * 128); };  // of a, in this warp's columns
+  // the residual goes to where the result of that turn will be stored from, two turns ahead
+  auto fetch = [&](const Item& it, int turn) {
+    constexpr int kPer = 16 / (int)sizeof(T), kPieces = 32 / kPer;
+    const int n = it.n0 + quad * 32, m = it.m0 + half * 128 + column(turn);
+    if (turn < kTurns)
+      for (int i = lane; i < kRows * kPieces; i += 32) {
+        const int r = i / kPieces, c = i % kPieces * kPer;
+        if (m + r < p.o.m && n + c < p.o.n)
+          copy16(mine + ((turn % kBuffers) * kRows + r) * 32 + c, static_cast<const T*>(p.o.residual) + (m + r) * p.o.ld_res + n + c);
+      }
+    copies_commit();
+  };
+  // before an item's sums are there; returns what a lane adds to its column of the result
+  auto prepare = [&](const Item& it) {
+    stores_read<0>();
+    __syncwarp();
+    if (p.staged) {
+      fetch(it, 0);
+      fetch(it, 1);
+    }
+    return bias_at<T>(p.o, it.n0 + quad * 32 + lane);
+  };
+  auto put = [&](const Item& it, int turn, float (&v)[kRows], float alpha, float bias) {
+    const int n = it.n0 + quad * 32, m = it.m0 + half * 128 + column(turn);
+    T* st = mine + (turn % kBuffers) * kRows * 32 + lane;
+    float x[kRows];
+    if (p.staged) {
+      stores_read<1>();
+      __syncwarp();
+      fetch(it, turn + 2);
+      copies_wait<2>();
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) x[r] = widen(st[r * 32]);
+    } else {
+      stores_read<kBuffers - 1>();
+      __syncwarp();
+      if (p.o.residual) load_residual<T, true>(p.o, x, m, n + lane);
+    }
+    finish<true>(p.o, v, alpha, &bias, x);
+    if (p.tma_store) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) st[r * 32] = narrow<T>(v[r]);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tma_store(&tmap_out, n, m, st);
+    } else if (n + lane < p.o.n) {
+      T* dst = static_cast<T*>(p.o.out) + (int64_t)m * p.o.ldo + n + lane;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (m + r < p.o.m) dst[r * p.o.ldo] = narrow<T>(v[r]);
+    }
+  };
+  if (!SPLIT && warp >= 4) {
     griddep_wait();
     const float alpha = out_scale(p.o);
     uint32_t ph = 0;
-    int buffer = 0;
     for (int i = pair; i < items; i += pairs, ph ^= 1u) {
       const Item it = item_at(i);
-      bool ok = mbar_wait_parked(d_full, ph, &g_status);
+      const float bias = prepare(it);
+      ok = mbar_wait_parked(d_full, ph, &g_status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int rows = min(it.width, p.o.m - it.m0) - half * 128;  // of a, in this warp's columns
+      const int rows = rows_of(it);
       float v[128];
       if (rows > 0) {
 #pragma unroll
@@ -304,33 +382,75 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_cluster(at_rank(smem_u32(d_empty), 0));
-      const int n = it.n0 + quad * 32;
-      if (rows <= 0 || n >= p.o.n) continue;
-      const int m = it.m0 + half * 128;
-      constexpr int kRows = kStoreBytes / (32 * (int)sizeof(T));
-#pragma unroll
-      for (int c = 0; c < 128; c += kRows) {
-        if (c >= rows) break;
-        finish_column<T, kRows>(p.o, v + c, alpha, m + c, n + lane);
-        if (p.tma_store) {
-          T* st = reinterpret_cast<T*>(mine + buffer * kStoreBytes);
-          stores_read<1>();
-          __syncwarp();
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) st[r * 32 + lane] = narrow<T>(v[c + r]);
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) tma_store(&tmap_out, n, m + c, st);
-          buffer ^= 1;
-        } else if (n + lane < p.o.n) {
-          T* dst = static_cast<T*>(p.o.out) + (int64_t)(m + c) * p.o.ldo + n + lane;
-#pragma unroll
-          for (int r = 0; r < kRows; ++r)
-            if (c + r < rows) dst[r * p.o.ldo] = narrow<T>(v[c + r]);
+      if (lane == 0) arrive_cluster(at_rank(smem_u32(d_empty), first));
+      if (it.n0 + quad * 32 >= p.o.n) continue;
+#pragma unroll 1
+      for (int turn = 0; column(turn) < rows; ++turn) {
+        float t[kRows];
+        switch (turn) {
+#define RB200_TAKE(j)                                              \
+  case j:                                                          \
+    _Pragma("unroll") for (int r = 0; r < kRows; ++r) t[r] = v[j * kRows + r]; \
+    break;
+          RB200_TAKE(0)
+          RB200_TAKE(1)
+          RB200_TAKE(2)
+          RB200_TAKE(3)
+          RB200_TAKE(4)
+          RB200_TAKE(5)
+          RB200_TAKE(6)
+          default:
+            RB200_TAKE(7)
+#undef RB200_TAKE
         }
+        put(it, turn, t, alpha, bias);
       }
     }
+    copies_wait<0>();
+    stores_read<0>();
+  }
+  if (SPLIT) {
+    // each pair sends the other what it does not keep, by columns of 128 rows of w, into the memory of its stages
+    griddep_wait();
+    const Item it = item_at(pair);
+    const float alpha = out_scale(p.o), bias = warp >= 4 ? prepare(it) : 0.0f;
+    ok = mbar_wait_parked(d_full, 0, &g_status) && ok;
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok)
+      for (int r = 0; r < 4; ++r) st_cluster(at_rank(smem_u32(holder + 1), r), 1u);
+    __syncthreads();
+    cluster_sync();  // both pairs' stages have been read
+    tc_fence_after();
+    const int rows = rows_of(it);
+    const bool work = warp >= 4 && holder[1] == 0u;
+    // [half][group / 2][32][128] fp32
+    float* slots = reinterpret_cast<float*>(smem) + half * 2 * 32 * 128 + quad * 32 + lane;
+    if (work) {
+#pragma unroll 1
+      for (int c = 32 * (1 - part); c < rows; c += 64) {
+        float v[32];
+        tmem_ld32(taddr + c, v);
+        ug::tc_wait_ld();
+        const uint32_t at = at_rank(smem_u32(slots + (c >> 6) * 32 * 128), (1 - part) * 2 + rank);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) st_cluster_f32(at + i * 512, v[i]);
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (work && it.n0 + quad * 32 < p.o.n) {
+#pragma unroll 1
+      for (int turn = 0; turn < kTurns && column(turn) < rows; ++turn) {
+        const int c = column(turn);
+        float v[kRows];
+        ug::tc_ld16(taddr + c, v);
+        const float* from = slots + ((c >> 6) * 32 + (c & 31)) * 128;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) v[i] += from[i * 128];
+        put(it, turn, v, alpha, bias);
+      }
+    }
+    copies_wait<0>();
     stores_read<0>();
   }
 
@@ -343,10 +463,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int FMT, class T>
-int launch_typed(Params& p, const CUtensorMap (&maps)[5], cudaStream_t stream) {
-  auto kern = fp4_pair_kernel<FMT, T>;
-  const size_t tail = (size_t)kDrainWarps * 2 * kStoreBytes + (2 * kMaxStages + 2) * 8 + 16 + 1024;
+// Two pairs share a tile's k where that fills empty SMs and leaves each pair eight stages: handing over half of the sums and
+// meeting twice costs about 3 us, a stage 0.27 (256 rows, k 4096 x n 4096: 18.5 -> 17.3 us, k 28672 x n 8192: 50 -> 36; at k 3328
+// it is even).  A tenth of the SMs is left out, since clusters of four do not find room everywhere: with 34 tiles one waits for
+// another to end (128 rows, k 8192: n 8448 20.4 us, n 8704 30.9, without sharing 24).
+bool splits(int tiles, int64_t k) { return tiles * 40 <= 9 * sm_count_current() && k >= 16 * kStageK; }
+
+template <int FMT, class T, bool SPLIT>
+int launch_split(Params& p, const CUtensorMap (&maps)[5], cudaStream_t stream) {
+  auto kern = fp4_pair_kernel<FMT, T, SPLIT>;
+  const size_t tail = (size_t)kDrainWarps * kBuffers * kRows * 32 * sizeof(T) + (2 * kMaxStages + 2) * 8 + 16 + 1024;
   p.stages = kMaxStages;
   while (p.stages > 2 && p.stages * (size_t)stage_bytes<FMT>() + tail > 227 * 1024) --p.stages;
   cudaLaunchConfig_t cfg = {};
@@ -355,7 +481,7 @@ int launch_typed(Params& p, const CUtensorMap (&maps)[5], cudaStream_t stream) {
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = SPLIT ? 4 : 2;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -369,9 +495,13 @@ int launch_typed(Params& p, const CUtensorMap (&maps)[5], cudaStream_t stream) {
     configured_device = dev;
   }
   const int items = p.n_tiles * p.m_tiles, pairs = sm_count_current() / 2;
-  cfg.gridDim = dim3((unsigned)(2 * (items < pairs ? items : pairs)), 1, 1);
+  cfg.gridDim = dim3((unsigned)(SPLIT ? 4 * items : 2 * (items < pairs ? items : pairs)), 1, 1);
   RB200_CUDA(cudaLaunchKernelEx(&cfg, kern, p, maps[0], maps[1], maps[2], maps[3], maps[4]));
   return 0;
+}
+template <int FMT, class T>
+int launch_typed(Params& p, const CUtensorMap (&maps)[5], cudaStream_t stream) {
+  return splits(p.n_tiles * p.m_tiles, p.k) ? launch_split<FMT, T, true>(p, maps, stream) : launch_split<FMT, T, false>(p, maps, stream);
 }
 template <int FMT>
 int launch_fmt(Params& p, int dtype, const CUtensorMap (&maps)[5], cudaStream_t stream) {
@@ -399,7 +529,6 @@ int fp4_pair_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
   memset(&p, 0, sizeof(p));
   p.o = output_of(d);
   p.k = (int)d.k;
-  p.k_tiles = (int)scale_k_tiles(d.k, d.format);
   p.early = launch_overlap_enabled() ? 1 : 0;
   RB200_CHECK((d.n + 2 * kTileN - 1) / (2 * kTileN) * ((d.m + kNb - 1) / kNb) < (1ll << 30), "the product is too large (m=%lld, n=%lld)", (long long)d.m,
               (long long)d.n);
@@ -409,6 +538,7 @@ int fp4_pair_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
   p.n_first = p.m_tiles <= 2;
   const int width = d.out_dtype == kF32 ? 4 : 2;
   p.tma_store = reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.ldo * width % 16 == 0;
+  p.staged = p.tma_store && d.residual && reinterpret_cast<uintptr_t>(d.residual) % 16 == 0 && p.o.ld_res * width % 16 == 0;
   CUtensorMap maps[5];
   if (make_tensor_map_2d(&maps[0], d.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (unsigned long long)d.k / 2, (unsigned long long)d.n,
                          (unsigned long long)d.k / 2, 128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
@@ -422,7 +552,7 @@ int fp4_pair_launch(const rb200_gemm_fp4_desc& d, cudaStream_t stream) {
                          d.out_dtype == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                          : d.out_dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                          (unsigned long long)d.n, (unsigned long long)d.m, (unsigned long long)d.ldo * width, 32,
-                         (unsigned)(kStoreBytes / (32 * width)), CU_TENSOR_MAP_SWIZZLE_NONE) != 0)
+                         (unsigned)kRows, CU_TENSOR_MAP_SWIZZLE_NONE) != 0)
     return -1;
   return d.format == kMx ? launch_fmt<kMx>(p, d.out_dtype, maps, stream) : launch_fmt<kNv>(p, d.out_dtype, maps, stream);
 }
