@@ -21,6 +21,7 @@
 
 #include "../../include/relax_b200.h"
 #include "fp4_mma.cuh"
+#include "fp4_out.cuh"
 #include "handover.h"
 #include "tensormap.h"
 
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
             const int row = j * 8 + 2 * t + (i & 1), f = f0 + fb * 16 + g + (i >> 1) * 8;
             // (h is rounded to fp16: it is the next product's operand, 2^-11 of itself at most, the error of its sum is
             // below that of the output's own rounding)
-            if (row < rows) p.h[(int64_t)(row0 + row) * p.ffn + f] = __float2half_rn(gv / (1.0f + __expf(-gv)) * uv);
+            if (row < rows) p.h[(int64_t)(row0 + row) * p.ffn + f] = __float2half_rn(silu(gv) * uv);
           }
       }
       consumers_sync();
