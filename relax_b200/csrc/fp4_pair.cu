@@ -7,7 +7,11 @@
 // from L2: 38 KB at 64 bytes a clock are 600 clocks; tiles of 128 x 256 per SM without pairing would need 54 KB.
 // Accumulator and scales leave no room for a second accumulator, so the drain takes all 256 columns into registers (eight
 // warps, 128 columns each) and hands the tensor memory back before it applies the epilogue and stores: the MMAs of the next
-// tile wait for the reading only.
+// tile wait for the reading only.  The drain itself is a loop over 16 columns: out of a cold instruction cache the same code for
+// all 128 columns took 8 to 26 us in its first tile, the loop takes 3.5 (warm, it costs 3 % at 2048 rows, k 4096).
+//
+// Measured: 4096 rows, k 8192 x n 28672 in the mx format 300 us, 6.4 PFLOP/s, 387 with the quantiser and at the power cap; 2048
+// rows, k 4096 x n 22016 in the nv format 77 us (4.8), 108; 333 rows, k 4096 x n 11008 with bias and silu 24 us (1.2), 25.5.
 #include <cstring>
 
 #include "fp4_gemm.h"
