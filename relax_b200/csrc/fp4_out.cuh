@@ -37,7 +37,7 @@ inline Output output_of(const rb200_gemm_fp4_desc& d) {
 #ifdef __CUDACC__
 __device__ __forceinline__ float out_scale(const Output& o) { return (o.a_ts ? *o.a_ts : 1.0f) * (o.w_ts ? *o.w_ts : 1.0f); }
 
-// v / (1 + exp(-v)) to 2^-20 of v; what is too small for a normal number becomes 0
+// v / (1 + exp(-v)) to 2^-20 of v; a quotient 1 / (1 + exp(-v)) below 2^-126 is taken as 0 (v < -87)
 __device__ __forceinline__ float silu(float v) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
