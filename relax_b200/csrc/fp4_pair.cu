@@ -6,12 +6,12 @@
 // memory.  What bounds a stage is the tensor cores (540 clocks at their nominal rate) and, close behind, what an SM takes
 // from L2: 38 KB at 64 bytes a clock are 600 clocks; tiles of 128 x 256 per SM without pairing would need 54 KB.
 // Accumulator and scales leave no room for a second accumulator, so the drain takes all 256 columns into registers (eight
-// warps, 128 columns each) and hands the tensor memory back before it applies the epilogue and stores: the MMAs of the next
+// warps, up to 128 columns each) and hands the tensor memory back before it applies the epilogue and stores: the MMAs of the next
 // tile wait for the reading only.  The drain itself is a loop over 16 columns: out of a cold instruction cache the same code for
 // all 128 columns took 8 to 26 us in its first tile, the loop takes 3.5 (warm, it costs 3 % at 2048 rows, k 4096).
 //
 // Measured: 4096 rows, k 8192 x n 28672 in the mx format 300 us, 6.4 PFLOP/s, 387 with the quantiser and at the power cap; 2048
-// rows, k 4096 x n 22016 in the nv format 77 us (4.8), 108; 333 rows, k 4096 x n 11008 with bias and silu 20 us (1.5), 22.
+// rows, k 4096 x n 22016 in the nv format 77 us (4.8), 108; 333 rows, k 4096 x n 11008 with bias and silu 19 us (1.6), 20.6.
 #include <cstring>
 
 #include "fp4_gemm.h"
@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto index_at = [&](int round) { return round * pairs + (round % 2 ? pairs - 1 - pair : pair); };
   struct Item {
     int n0, m0, width;  // this CTA's first row of w, the tile's first row of a, columns of the MMA
+    int share;          // of them, for the drain warps' first half (100 rows, k 4096 x n 11008, silu: 18.3 -> 16.1 us by halves)
   };
   auto item_at = [&](int i) {
     const int nt = p.n_first ? i % p.n_tiles : i / p.m_tiles, mt = p.n_first ? i / p.n_tiles : i % p.m_tiles;
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     it.n0 = (2 * nt + rank) * kTileN;
     it.m0 = mt * kNb;
     it.width = min(kNb, (p.o.m - it.m0 + 31) / 32 * 32);
+    it.share = (it.width + 63) / 64 * 32;
     return it;
   };
 
@@ -310,20 +312,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   // ============================================================ drain
   const int dw = warp - 4, quad = warp & 3, half = dw >> 2;
   T* mine = store + dw * kBuffers * kRows * 32;
-  const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(half * 128);
+  const uint32_t taddr = tmem + ((uint32_t)(32 * quad) << 16);
   // A warp's columns of the accumulator (rows of a) by kRows of them.  SPLIT: of its four groups of 32 columns the first pair
   // has the even ones, the second the odd ones.
   constexpr int kTurns = SPLIT ? 4 : 8;
   auto column = [&](int turn) { return SPLIT ? (turn >> 1) * 64 + part * 32 + (turn & 1) * kRows : turn * kRows; };
-  auto rows_of = [&](const Item& it) { return min(128, p.o.m - it.m0 - half * 128); };  // of a, in this warp's columns
+  auto first_of = [&](const Item& it) { return half * it.share; };  // this warp's first column, and how many rows of a it has
+  auto rows_of = [&](const Item& it) { return min(it.share, p.o.m - it.m0 - first_of(it)); };
   // the residual goes to where the result of that turn will be stored from, two turns ahead
   auto fetch = [&](const Item& it, int turn) {
     constexpr int kPer = 16 / (int)sizeof(T), kPieces = 32 / kPer;
-    const int n = it.n0 + quad * 32, m = it.m0 + half * 128 + column(turn);
+    const int n = it.n0 + quad * 32, m = it.m0 + first_of(it) + column(turn), rows = min(kRows, rows_of(it) - column(turn));
     if (turn < kTurns)
-      for (int i = lane; i < kRows * kPieces; i += 32) {
+      for (int i = lane; i < rows * kPieces; i += 32) {
         const int r = i / kPieces, c = i % kPieces * kPer;
-        if (m + r < p.o.m && n + c < p.o.n)
+        if (n + c < p.o.n)
           copy16(mine + ((turn % kBuffers) * kRows + r) * 32 + c, static_cast<const T*>(p.o.residual) + (m + r) * p.o.ld_res + n + c);
       }
     copies_commit();
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return bias_at<T>(p.o, it.n0 + quad * 32 + lane);
   };
   auto put = [&](const Item& it, int turn, float (&v)[kRows], float alpha, float bias) {
-    const int n = it.n0 + quad * 32, m = it.m0 + half * 128 + column(turn);
+    const int n = it.n0 + quad * 32, m = it.m0 + first_of(it) + column(turn);
     T* st = mine + (turn % kBuffers) * kRows * 32 + lane;
     float x[kRows];
     if (p.staged) {
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float v[128];
       if (rows > 0) {
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld32(taddr + c, v + c);
+        for (int c = 0; c < 128; c += 32) tmem_ld32(taddr + first_of(it) + c, v + c);
         ug::tc_wait_ld();
       }
       tc_fence_before();
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int c = 32 * (1 - part); c < rows; c += 64) {
         float v[32];
-        tmem_ld32(taddr + c, v);
+        tmem_ld32(taddr + first_of(it) + c, v);
         ug::tc_wait_ld();
         const uint32_t at = at_rank(smem_u32(slots + (c >> 6) * 32 * 128), (1 - part) * 2 + rank);
 #pragma unroll
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int turn = 0; turn < kTurns && column(turn) < rows; ++turn) {
         const int c = column(turn);
         float v[kRows];
-        ug::tc_ld16(taddr + c, v);
+        ug::tc_ld16(taddr + first_of(it) + c, v);
         const float* from = slots + ((c >> 6) * 32 + (c & 31)) * 128;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) v[i] += from[i * 128];
