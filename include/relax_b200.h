@@ -41,7 +41,8 @@ RB200_API void* rb200_get_stream(void);
  * array of rb200_gemm_fp16_intx_noalloc, that of rb200_encode_ft and that of the 4-bit float entries.  Synchronises the given stream.  0 = no error recorded,
  * 1 = a wait ran out (the kernel skipped its remaining work and left outputs unwritten).
  * Allocates nothing: a status word that no call has created yet reads as 0.  After a non-zero
- * status it synchronises the device and puts the split-k flags, tickets and hand-over words back at rest.
+ * status it synchronises the device and puts the split-k flags, tickets and hand-over words back at rest; calls
+ * launched between a wait that ran out and this one may find parts that were left there, and their results do not count.
  * Replaces nothing in the reference, whose kernels spin without a bound
  * (3rdparty/tensorrt_llm/custom_allreduce_kernels.cu:94-113) and whose collectives abort the
  * process on error (src/runtime/disco/nccl/nccl_context.h:50-56).
@@ -418,6 +419,11 @@ typedef struct rb200_moe_layer_fp4_desc {
 } rb200_moe_layer_fp4_desc;
 RB200_API size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn);
 RB200_API int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+/* Self-test of its waits: CTA `absent_cta` of the first kernel hands over nothing, so that who waits for its part gives up after the
+ * limit of rb200_set_wait_limit_ms.  Then, as after any wait of the layer that ran out, `out` stays unwritten (where a wait of the
+ * second kernel ran out, the columns that needed it).  -1: the layer itself. */
+RB200_API int rb200_moe_layer_fp4_selftest(const rb200_moe_layer_fp4_desc* desc, void* workspace, size_t workspace_bytes,
+                                           int absent_cta, void* stream);
 
 /* ------------------------------------------------------------------ low-latency all-reduce */
 

@@ -147,6 +147,7 @@ SIGNATURES = {
     "rb200_linear_fp4": (_I, [_V, _I, _I64, ctypes.POINTER(GemmFp4Desc), _V, ctypes.c_size_t, _V]),
     "rb200_moe_layer_fp4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
     "rb200_moe_layer_fp4": (_I, [ctypes.POINTER(MoeLayerFp4Desc), _V, ctypes.c_size_t, _V]),
+    "rb200_moe_layer_fp4_selftest": (_I, [ctypes.POINTER(MoeLayerFp4Desc), _V, ctypes.c_size_t, _I, _V]),
     "rb200_allreduce_workspace_bytes": (ctypes.c_size_t, [_I64]),
     "rb200_allreduce_oneshot": (_I, [ctypes.POINTER(_V), _I, _I, _V, _V, _I64, _I64, _V]),
     "rb200_allreduce_oneshot_selftest": (_I, [ctypes.POINTER(_V), ctypes.POINTER(_V), ctypes.POINTER(_V), _I,

@@ -80,6 +80,8 @@ struct Params {
   float* parts;       // down: two tiles [tokens][64] a CTA
   uint32_t* tickets;  // down: a tile's parts that are there
   uint32_t* words;    // up: hand-over words, or nullptr
+  uint32_t* states;   // of up's CTAs, written by every call
+  int absent;         // up: the CTA that hands over nothing (self-test), or -1
   uint64_t wait_ns;   // bound of the wait for them
 };
 
@@ -463,6 +465,9 @@ struct Place {
   }
 };
 
+// What `down` has to know of up's CTAs, a word of each (one for all of them would have to be cleared first).
+constexpr uint32_t kFailed = 1u;  // a wait ran out: parts of h are not there
+
 // Hand-over words (handover.h): a warp's sums of a part of a 64-row tile.  A word is its own flag, vacant (all bits set) at rest.
 constexpr uint32_t kVacant = 0xffffffffu;
 template <int NT>
@@ -625,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
       float(&acc)[NT][4] = sum[0];
       join(sum);
       if (first > 0) {
-        if (ok) publish<NT>(p.words, blockIdx.x, acc);
+        if (ok && (int)blockIdx.x != p.absent) publish<NT>(p.words, blockIdx.x, acc);
         continue;
       }
       if (n < chunks) {
@@ -656,7 +661,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
       }
       consumers_sync();
     }
+    if (!ok) r.failed = 1;
   }
+  __syncthreads();
+  if (tid == 0) p.states[blockIdx.x] = r.failed ? kFailed : 0u;
 }
 
 template <int FMT, int NT>
@@ -725,6 +733,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
     // ============================================================ h
     griddep_wait();  // the kernel before's
     griddep_launch_dependents();
+    // The words of state are asked for first and looked at when the copies of the first unit are on their way, too (one token
+    // 47.7 -> 48.1 us; looked at after the copies of every stage 48.8).
+    uint32_t state = 0u;
+    {
+      uint32_t word[kMaxCtas / 32];
+#pragma unroll
+      for (int i = 0; i < kMaxCtas / 32; ++i) word[i] = i * 32 + lane < (int)gridDim.x ? __ldcg(p.states + i * 32 + lane) : 0u;
+#pragma unroll
+      for (int i = 0; i < kMaxCtas / 32; ++i) state |= word[i];
+    }
     int issued = 0;
     Place<false> at(u0, per, r.entries);
     for (int u = u0; u < u1; ++u, at.next()) {
@@ -739,8 +757,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
         copy_rows(smem_u32(xs + ring.s * L.x_bytes) + half * (NT * 8 * kStageK * 2), p.h + (int64_t)row0 * p.ffn + (there ? k : 0), p.ffn,
                   nullptr, rows, there);
       }
-      cp_async_arrive(&full[ring.s]);
       ++issued;
+      if (u == u0 && (__reduce_or_sync(0xffffffffu, state) & kFailed)) r.failed = 1;  // (who waits for a unit sees it)
+      cp_async_arrive(&full[ring.s]);
       ring.next();
     }
     drain_ring(full, p.stages, issued);
@@ -886,7 +905,7 @@ int weight_map(CUtensorMap* map, const void* w, int64_t rows, int64_t k) {
 }
 
 template <int FMT, int NT>
-int launch(Params p, const Weights& w, cudaStream_t stream) {
+int launch(Params p, const Weights& w, int absent, cudaStream_t stream) {
   auto up = moe_fp4_up_kernel<FMT, NT>;
   auto down = moe_fp4_down_kernel<FMT, NT>;
   const int most_ctas = kCtasPerSm * sm_count_current(), ctas = most_ctas < kMaxCtas ? most_ctas : kMaxCtas;
@@ -906,6 +925,7 @@ int launch(Params p, const Weights& w, cudaStream_t stream) {
   while (p.stages > 2 && smem_bytes<NT>(l, p.stages, red) > room) --p.stages;
   CUtensorMap map;
   if (weight_map(&map, w.up, (int64_t)p.experts * 2 * p.ffn, p.hidden) != 0) return -1;
+  p.absent = absent;
   p.words = handover_words(stream, sm_count_current(), (size_t)ctas * part_words<NT>() * sizeof(uint32_t));
   p.wait_ns = (wait_limit_ms() ? (uint64_t)wait_limit_ms() : 2000ull) * 1000000ull;
   RB200_CUDA(launch_dependent(up, dim3((unsigned)ctas), kThreads, smem_bytes<NT>(l, p.stages, red), stream, p, map));
@@ -919,21 +939,22 @@ int launch(Params p, const Weights& w, cudaStream_t stream) {
 }
 
 template <int FMT>
-int launch_fmt(const Params& p, const Weights& w, cudaStream_t stream) {
+int launch_fmt(const Params& p, const Weights& w, int absent, cudaStream_t stream) {
   // Entries of eight rows, or of sixteen where experts have more than four on average: weights of an expert with more rows than
   // an entry are read again (by then from L2), rows that are not there take shared memory from the stages (29 tokens,
   // 64 experts of top 6: 100 us with sixteen, 79 with eight).
-  return p.tokens <= 8 || p.tokens * p.top_k <= 4 * p.experts ? launch<FMT, 1>(p, w, stream) : launch<FMT, 2>(p, w, stream);
+  return p.tokens <= 8 || p.tokens * p.top_k <= 4 * p.experts ? launch<FMT, 1>(p, w, absent, stream) : launch<FMT, 2>(p, w, absent, stream);
 }
 
-// [h | parts | tickets]
+// [h | parts | states | tickets]
 struct Workspace {
-  size_t parts, tickets, bytes;
+  size_t parts, states, tickets, bytes;
 };
 Workspace workspace_of(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn) {
   Workspace w;
   w.parts = (size_t)((tokens * top_k * ffn * 2 + 255) / 256 * 256);
-  w.tickets = w.parts + (size_t)kMaxCtas * 2 * tokens * kTile * 4;
+  w.states = w.parts + (size_t)kMaxCtas * 2 * tokens * kTile * 4;
+  w.tickets = w.states + (size_t)kMaxCtas * 4;
   w.bytes = w.tickets + (size_t)((hidden + kTile - 1) / kTile) * 4;
   return w;
 }
@@ -970,6 +991,10 @@ size_t rb200_moe_layer_fp4_workspace_bytes(int64_t tokens, int64_t top_k, int64_
 }
 
 int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  return rb200_moe_layer_fp4_selftest(d, workspace, workspace_bytes, -1, stream);
+}
+
+int rb200_moe_layer_fp4_selftest(const rb200_moe_layer_fp4_desc* d, void* workspace, size_t workspace_bytes, int absent, void* stream) {
   RB200_CHECK(d != nullptr && d->struct_size == sizeof(rb200_moe_layer_fp4_desc), "rb200_moe_layer_fp4_desc has a wrong struct_size");
   RB200_CHECK(d->format == f4::kMx || d->format == f4::kNv, "unknown 4-bit format %d", d->format);
   RB200_CHECK(d->tokens >= 0 && d->tokens <= f4::kMaxTokens, "tokens=%lld outside [0, %d]", (long long)d->tokens, f4::kMaxTokens);
@@ -1003,6 +1028,7 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   const f4::Workspace ws = f4::workspace_of(d->tokens, d->top_k, d->hidden, d->ffn);
   p.h = static_cast<__half*>(workspace);
   p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.parts);
+  p.states = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + ws.states);
   p.tickets = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + ws.tickets);
   p.out = static_cast<__half*>(d->out);
   p.s1_expert = f4::scale_bytes(2 * d->ffn, d->hidden, d->format);
@@ -1020,7 +1046,7 @@ int rb200_moe_layer_fp4(const rb200_moe_layer_fp4_desc* d, void* workspace, size
   RB200_CUDA(cudaGetDevice(&dev));
   if (dev >= 0 && dev < f4::kMaxDevices) f4::g_launched[dev].store(true, std::memory_order_relaxed);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return d->format == f4::kMx ? f4::launch_fmt<f4::kMx>(p, w, s) : f4::launch_fmt<f4::kNv>(p, w, s);
+  return d->format == f4::kMx ? f4::launch_fmt<f4::kMx>(p, w, absent, s) : f4::launch_fmt<f4::kNv>(p, w, absent, s);
 }
 
 }  // extern "C"
