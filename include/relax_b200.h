@@ -391,7 +391,9 @@ RB200_API int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb
  * between keep 16 bits:
  *   p = softmax(logits[t]); the top_k experts of largest logits (equal ones: lower index first; distinct);
  *   gate_j = p_j, or p_j / (sum of the chosen p) with renormalize;
- *   out[t] = sum_j gate_j (silu(x[t] Wg_j^T) * (x[t] Wu_j^T)) Wd_j^T,  fp32 sums, the factor in brackets rounded to fp16.
+ *   out[t] = sum_j gate_j (silu(x[t] Wg_j^T) * (x[t] Wu_j^T)) Wd_j^T,  fp32 sums, the factor in brackets held in 11 bits under a
+ *   power of two, over all of fp32's range down to 2^-86: off by 2^-12 of itself or by 2^-28, or, where the largest of a token and
+ *   expert is 2^11 or more or below 2^-16, by 2^-23 of that largest (such values cost some time).
  * A NaN among a token's logits, or a maximum that is infinite, makes its gates NaN, as in rb200_moe_route.
  * x and out fp16 [tokens, hidden], logits fp32 [tokens, num_experts]; w_gate_up codes [num_experts, 2 ffn, hidden / 2], gate
  * rows first; w_down codes [num_experts, hidden, ffn / 2]; scales of each expert in tiles, experts after one another;

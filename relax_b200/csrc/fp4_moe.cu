@@ -23,6 +23,7 @@
 // issued in 63 % of the clocks), few or small experts by the starts and last tiles of two kernels.
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/relax_b200.h"
 #include "fp4_mma.cuh"
@@ -55,13 +56,14 @@ struct alignas(16) Routing {
   float gate_of[kRows];        // by token and choice
   int warp_sum[kConsumers];
   int entries;
-  int failed;
+  int failed, scaled;
   uint32_t ticket;
   uint16_t first_row[kMaxExperts];  // of an expert
   uint16_t entry_row[kRows + 2];
   uint8_t entry_expert[kRows];
   uint8_t token_of_row[kRows];
   uint8_t expert_of[kRows];
+  int8_t exponent_of_row[kRows];  // down: its h is 2^exponent times what the products take
 };
 
 struct Params {
@@ -80,10 +82,30 @@ struct Params {
   float* parts;       // down: two tiles [tokens][64] a CTA
   uint32_t* tickets;  // down: a tile's parts that are there
   uint32_t* words;    // up: hand-over words, or nullptr
+  int8_t* exponents;  // of h: a row's sixteens of f
   uint32_t* states;   // of up's CTAs, written by every call
   int absent;         // up: the CTA that hands over nothing (self-test), or -1
   uint64_t wait_ns;   // bound of the wait for them
 };
+
+// h between the kernels is fp16 times 2^exponent, an exponent for 16 f of a row: fp16 alone ends at 65504, and below 2^-14 it
+// loses bits.  Where the largest of the sixteen lies in [2^-16, 2^11) the exponent is kPlain, and if it is everywhere, `down`
+// takes the numbers as they lie.  Else it is in steps of 16, such that the largest becomes 2^-1 to 2^15, and `down` brings a row
+// to its largest exponent (few sixteens have another), which multiplies the row's sums.  Either way an element is off by 2^-12 of
+// itself, or by 2^-28, or, of a row whose largest is outside [2^-16, 2^11), by 2^-23 of that largest.  (The
+// measured cases: exponents cost 48.1 -> 48.7 us for one token, 141.9 -> 142.7 for eight; with h some 2^10 times larger the same
+// layers take 52.3 and 194 to 202.)
+constexpr int kPlain = -4, kLowest = -100;
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
+// of the bits of sixteen numbers' largest finite magnitude
+__device__ __forceinline__ int h_exponent(uint32_t top) {
+  const int x = (int)(top >> 23) - 127;
+  return top == 0u ? kLowest : x >= -16 && x < 11 ? kPlain : max(kPlain + ((x + 5) >> 4) * 16, kLowest);
+}
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
 
 // order of floats as unsigned numbers, NaN lowest
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -216,6 +238,7 @@ __device__ __forceinline__ void route(const Params& p, Routing<NT>& r, float* sc
     const int e = r.expert_of[tid], t = tid / p.top_k, row = r.first_row[e] + __popc(r.mask[e] & ((1u << t) - 1u));
     r.token_of_row[row] = (uint8_t)t;
     r.gate_of_row[row] = r.gate_of[tid];
+    r.exponent_of_row[row] = kPlain;
   }
 }
 __device__ __forceinline__ void rows_sync() {
@@ -226,6 +249,11 @@ __device__ __forceinline__ void rows_sync() {
 // 16 bytes of global memory, or zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void cp_async_wait() {  // all but the last LEFT groups have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 // arrives at the barrier when this thread's copies so far have landed (the barrier counts these arrivals)
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
@@ -412,6 +440,72 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const __half* src, int64
     cp_async16(dst + i * (kStageK * 2) + x_column(i, lane) * 16, src + (tokens ? tokens[i] : i) * pitch, there);
 }
 
+// Exponents of rows: the largest of their sixteens.  By a warp, two rows at once.
+template <int NT>
+__device__ __forceinline__ void take_exponents(const Params& p, Routing<NT>& r, int row0, int rows) {
+  const int lane = threadIdx.x & 31, words = p.ffn / 64;
+#pragma unroll 1
+  for (int i = 0; i < rows; i += 2) {
+    const int more = i + 1 < rows ? words : 0;
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(p.exponents) + (int64_t)(row0 + i) * words;
+    uint32_t top[2] = {0x80808080u, 0x80808080u};
+#pragma unroll 1
+    for (int w = lane; w < words; w += 8 * 32) {
+      uint32_t v[2][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[0][j] = w + j * 32 < words ? __ldcg(from + w + j * 32) : 0x80808080u;
+        v[1][j] = w + j * 32 < more ? __ldcg(from + words + w + j * 32) : 0x80808080u;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        top[0] = __vmaxs4(top[0], v[0][j]);
+        top[1] = __vmaxs4(top[1], v[1][j]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      top[q] = __vmaxs4(top[q], top[q] >> 16 | top[q] << 16);
+      top[q] = __vmaxs4(top[q], top[q] >> 8 | top[q] << 24);
+      const int e = __reduce_max_sync(0xffffffffu, (int)(int8_t)top[q]);
+      if (lane == 0 && i + q < rows) r.exponent_of_row[row0 + i + q] = (int8_t)e;
+    }
+  }
+  __syncwarp();
+}
+// What this lane's copies brought of rows' h, eight numbers of either half at `k` and `k` + 256, from the exponents of their
+// sixteens to those of the rows.  All copies but those of the last LEFT groups are waited for.
+template <int LEFT, int NT>
+__device__ __forceinline__ void rescale_rows(const Params& p, const Routing<NT>& r, uint8_t* x, int k, int row0, int rows) {
+  const int lane = threadIdx.x & 31;
+  const signed char* const from = reinterpret_cast<const signed char*>(p.exponents) + (int64_t)row0 * (p.ffn / 16) + k / 16;
+#pragma unroll 1
+  for (int base = 0; base < rows; base += 4) {
+    int own[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        own[half][i] = base + i < rows && k + half * kStageK < p.ffn ? __ldcg(from + (int64_t)(base + i) * (p.ffn / 16) + half * (kStageK / 16)) : 127;
+    cp_async_wait<LEFT>();
+#pragma unroll 1
+    for (int i = 0; i < 4 && base + i < rows; ++i) {
+      const int row = base + i;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int e = i == 0 ? own[half][0] : i == 1 ? own[half][1] : i == 2 ? own[half][2] : own[half][3];
+        const int by = e - r.exponent_of_row[row0 + row];
+        if (e == 127 || by == 0) continue;
+        // (fp16's powers of two end at -24; a number times 2^-48 is zero, an infinity stays one)
+        const __half2 one = __float2half2_rn(power_of_two(max(by, -24))), two = __float2half2_rn(power_of_two(max(min(by + 24, 0), -24)));
+        __half2* v = reinterpret_cast<__half2*>(x + half * (NT * 8 * kStageK * 2) + row * (kStageK * 2) + x_column(row, lane) * 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __hmul2(__hmul2(v[q], one), two);
+      }
+    }
+  }
+}
+
 template <int S, int NT>
 __device__ __forceinline__ void zero(float (&sum)[S][NT][4]) {
 #pragma unroll
@@ -467,6 +561,7 @@ struct Place {
 
 // What `down` has to know of up's CTAs, a word of each (one for all of them would have to be cleared first).
 constexpr uint32_t kFailed = 1u;  // a wait ran out: parts of h are not there
+constexpr uint32_t kScaled = 2u;  // some exponent of h is not kPlain
 
 // Hand-over words (handover.h): a warp's sums of a part of a 64-row tile.  A word is its own flag, vacant (all bits set) at rest.
 constexpr uint32_t kVacant = 0xffffffffu;
@@ -538,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
   if (tid == 0) {
     tma_prefetch_map(&tmap_w);
     init_ring(full, empty, p.stages);
-    r.failed = 0;
+    r.failed = r.scaled = 0;
   }
   fence_proxy_async();
   griddep_wait();
@@ -648,23 +743,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_up_kernel(const 
       consumers_sync();
       if (!is_up && r.failed == 0) {
         const float ts = p.ts1 ? p.ts1[e] : 1.0f;
+        const int f = f0 + fb * 16;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j) {
+          float h[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float gv = acc[j][i] * ts, uv = red[((fb * NT + j) * 4 + i) * 32 + lane] * ts;
-            const int row = j * 8 + 2 * t + (i & 1), f = f0 + fb * 16 + g + (i >> 1) * 8;
-            // (h is rounded to fp16: it is the next product's operand, 2^-11 of itself at most, the error of its sum is
-            // below that of the output's own rounding)
-            if (row < rows) p.h[(int64_t)(row0 + row) * p.ffn + f] = __float2half_rn(silu(gv) * uv);
+          for (int i = 0; i < 4; ++i) h[i] = silu(acc[j][i] * ts) * (red[((fb * NT + j) * 4 + i) * 32 + lane] * ts);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t top = max(finite_bits(h[q]), finite_bits(h[2 + q]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int row = j * 8 + 2 * t + q, exponent = h_exponent(top);
+            if (row < rows) {
+              const float by = power_of_two(-exponent);
+              __half* to = p.h + (int64_t)(row0 + row) * p.ffn + f + g;
+              to[0] = __float2half_rn(h[q] * by);
+              to[8] = __float2half_rn(h[2 + q] * by);
+              if (g == 0) p.exponents[(int64_t)(row0 + row) * (p.ffn / 16) + f / 16] = (int8_t)exponent;
+              if (exponent != kPlain && top != 0u) r.scaled = 1;
+            }
           }
+        }
       }
       consumers_sync();
     }
     if (!ok) r.failed = 1;
   }
   __syncthreads();
-  if (tid == 0) p.states[blockIdx.x] = r.failed ? kFailed : 0u;
+  if (tid == 0) p.states[blockIdx.x] = (r.failed ? kFailed : 0u) | (r.scaled ? kScaled : 0u);
 }
 
 template <int FMT, int NT>
@@ -683,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
   if (tid == 0) {
     tma_prefetch_map(&tmap_w);
     init_ring(full, empty, p.stages);
-    r.failed = 0;
+    r.failed = r.scaled = 0;
   }
   for (int i = tid; i < 2 * p.tokens * kTile; i += kThreads) sums[i] = 0.0f;
   fence_proxy_async();
@@ -744,7 +851,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
       for (int i = 0; i < kMaxCtas / 32; ++i) state |= word[i];
     }
     int issued = 0;
-    Place<false> at(u0, per, r.entries);
+    Place<false> at(u0, per, r.entries), behind = at;
+    int behind_s = 0;
+    bool first = true;
+    auto finish_behind = [&](auto left) {
+      const int row0 = r.entry_row[behind.a], rows = r.entry_row[behind.a + 1] - row0;
+      if (first || behind.c == 0) take_exponents(p, r, row0, rows);
+      first = false;
+      rescale_rows<decltype(left)::value>(p, r, xs + behind_s * L.x_bytes, behind.c * kUnitK + lane * 8, row0, rows);
+      mbar_arrive(&full[behind_s]);
+      behind.next();
+      if (++behind_s == p.stages) behind_s = 0;
+    };
     for (int u = u0; u < u1; ++u, at.next()) {
       bool ok = mbar_wait_parked(&empty[ring.s], ring.ph ^ 1u, &g_status);
       ok = __all_sync(0xffffffffu, ok);
@@ -758,8 +876,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
                   nullptr, rows, there);
       }
       ++issued;
-      if (u == u0 && (__reduce_or_sync(0xffffffffu, state) & kFailed)) r.failed = 1;  // (who waits for a unit sees it)
-      cp_async_arrive(&full[ring.s]);
+      if (u == u0) {
+        state = __reduce_or_sync(0xffffffffu, state);
+        if (state & kFailed) r.failed = 1;  // (who waits for a unit sees it)
+      }
+      if (state & kScaled) {  // one unit's copies are on their way while the unit before is seen to
+        cp_async_commit();
+        if (u > u0) finish_behind(std::integral_constant<int, 1>());
+        if (u + 1 == u1) finish_behind(std::integral_constant<int, 0>());
+      } else {
+        cp_async_arrive(&full[ring.s]);
+      }
       ring.next();
     }
     drain_ring(full, p.stages, issued);
@@ -805,9 +932,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
       const bool tile_ends = u + 1 == u1 || at.last_of_tile();
       if (tile_ends || at.last_of_entry()) {
         join(sum);
-        // this entry's part is complete here: gate times it, into the tokens' sums (a word belongs to one lane at a time)
+        // this entry's part is complete here: gate times it and the row's power of two, into the tokens' sums (a word belongs to one lane at a time)
         float* word[NT][2];
-        float had[NT][4];
+        float had[NT][4], gate_here[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -815,14 +942,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) moe_fp4_down_kernel(cons
             word[j][q] = sums + (kh * p.tokens + token[j][q]) * kTile + fb * 16 + g;
             had[j][q] = word[j][q][0];
             had[j][2 + q] = word[j][q][8];
+            gate_here[j][q] = gate[j][q] * power_of_two(r.exponent_of_row[r.entry_row[at.a] + min(j * 8 + 2 * t + q, rows - 1)]);
           }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int q = 0; q < 2; ++q)
             if (j * 8 + 2 * t + q < rows) {
-              word[j][q][0] = fmaf(gate[j][q], acc[j][q], had[j][q]);
-              word[j][q][8] = fmaf(gate[j][q], acc[j][2 + q], had[j][2 + q]);
+              word[j][q][0] = fmaf(gate_here[j][q], acc[j][q], had[j][q]);
+              word[j][q][8] = fmaf(gate_here[j][q], acc[j][2 + q], had[j][2 + q]);
             }
         __syncwarp();
       }
@@ -946,13 +1074,14 @@ int launch_fmt(const Params& p, const Weights& w, int absent, cudaStream_t strea
   return p.tokens <= 8 || p.tokens * p.top_k <= 4 * p.experts ? launch<FMT, 1>(p, w, absent, stream) : launch<FMT, 2>(p, w, absent, stream);
 }
 
-// [h | parts | states | tickets]
+// [h | its exponents | parts | states | tickets]
 struct Workspace {
-  size_t parts, states, tickets, bytes;
+  size_t exponents, parts, states, tickets, bytes;
 };
 Workspace workspace_of(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn) {
   Workspace w;
-  w.parts = (size_t)((tokens * top_k * ffn * 2 + 255) / 256 * 256);
+  w.exponents = (size_t)((tokens * top_k * ffn * 2 + 255) / 256 * 256);
+  w.parts = w.exponents + (size_t)((tokens * top_k * ((ffn + 15) / 16) + 255) / 256 * 256);
   w.states = w.parts + (size_t)kMaxCtas * 2 * tokens * kTile * 4;
   w.tickets = w.states + (size_t)kMaxCtas * 4;
   w.bytes = w.tickets + (size_t)((hidden + kTile - 1) / kTile) * 4;
@@ -1027,6 +1156,7 @@ int rb200_moe_layer_fp4_selftest(const rb200_moe_layer_fp4_desc* d, void* worksp
   p.ts2 = d->down_tensor_scale;
   const f4::Workspace ws = f4::workspace_of(d->tokens, d->top_k, d->hidden, d->ffn);
   p.h = static_cast<__half*>(workspace);
+  p.exponents = reinterpret_cast<int8_t*>(static_cast<uint8_t*>(workspace) + ws.exponents);
   p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.parts);
   p.states = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + ws.states);
   p.tickets = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + ws.tickets);
