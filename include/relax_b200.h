@@ -361,7 +361,7 @@ RB200_API int rb200_preprocess_fp4_scales(const void* src, void* dst, int64_t ba
  *                     read; workspace: rb200_linear_fp4_workspace_bytes(m, k, format) bytes, 256-byte aligned, of the call's
  *                     own until it has run.
  * Nothing is allocated.  With launch overlap on, w and w_scales are read ahead of the previous kernel's end.  out must not
- * overlap what is read, but may be the residual itself.
+ * overlap what is read, but may be the residual itself, and rb200_linear_fp4's may lie over x.
  */
 typedef struct rb200_gemm_fp4_desc {
   uint32_t struct_size;         /* sizeof(rb200_gemm_fp4_desc) */

@@ -468,7 +468,11 @@ int rb200_linear_fp4(const void* x, int x_dtype, int64_t ldx, const rb200_gemm_f
   RB200_CHECK(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                   workspace_bytes >= rb200_linear_fp4_workspace_bytes(d.m, d.k, d.format),
               "the workspace must be 256-byte aligned and hold rb200_linear_fp4_workspace_bytes");
-  if (x_dtype == d.out_dtype && f4::quantises_itself(d.m, d.n, d.k)) return fp4_gemm_launch(d, x, ldx, static_cast<cudaStream_t>(stream));
+  // (a product that quantises x reads it in the CTAs of every tile, while others already store: not where out lies over x)
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), out0 = reinterpret_cast<uintptr_t>(d.out);
+  const uintptr_t x1 = x0 + ((d.m - 1) * ldx + d.k) * width, out1 = out0 + ((d.m - 1) * d.ldo + d.n) * (d.out_dtype == f4::kF32 ? 4 : 2);
+  const bool apart = x1 <= out0 || out1 <= x0;
+  if (apart && x_dtype == d.out_dtype && f4::quantises_itself(d.m, d.n, d.k)) return fp4_gemm_launch(d, x, ldx, static_cast<cudaStream_t>(stream));
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + (d.m * (d.k / 2) + 255) / 256 * 256;
   if (fp4_encode_launch(x, x_dtype, 1, d.m, d.k, ldx, 0, d.format, d.a_tensor_scale, codes, scales, true,

@@ -210,7 +210,7 @@ def linear_fp4(x, w, w_scales, fmt: str, x_tensor_scale=None, w_tensor_scale=Non
                workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A linear layer over a weight in 4-bit floats: ``x`` [.., k] is quantised as :func:`encode_fp4` does, then multiplied
     as :func:`gemm_fp4` does; the result has ``x``'s type.  ``workspace`` (uint8, :func:`linear_fp4_workspace_bytes`) and
-    ``out`` make the call allocation-free."""
+    ``out`` make the call allocation-free; ``out`` may be ``x`` or the residual, and must not overlap what else is read."""
     return native.linear_fp4(x, w, w_scales, fmt, x_tensor_scale, w_tensor_scale, bias, residual, activation, binary_op, unary_op,
                              workspace, out)
 

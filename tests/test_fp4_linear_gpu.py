@@ -1,0 +1,39 @@
+"""Linears over 4-bit floats: results over their own inputs, batches around the rules that choose a kernel, odd values."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from relax_b200 import _lib, ops
+from tests import fp4_ref as ref
+from tests.test_fp4_gpu import TYPES, _check_product, _gen, _np, _operand
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m, n", [(1, 512), (2, 4096), (4, 288), (20, 512), (64, 288), (70, 512), (300, 512)])
+def test_result_over_the_activations(fmt, dtype, m, n):
+    """Tiles of a small batch store while others still need all of x: with out = x it has to be quantised first."""
+    g = _gen(m + n)
+    (wc, wsc, _) = _operand(g, fmt, n, n)
+    ts = torch.tensor([2.0 ** -10], device="cuda") if fmt == "nv" else None
+    x = (torch.randn(m, n, device="cuda", generator=g)).to(TYPES[dtype])
+    call = lambda v, **kw: ops.linear_fp4(v, wc, wsc, fmt, x_tensor_scale=ts, w_tensor_scale=ts, **kw)
+    want, with_x = call(x), call(x, residual=x, binary_op="plus")
+    for _ in range(5):
+        y = x.clone()
+        assert call(y, out=y) is y and torch.equal(y, want)
+        y = x.clone()
+        assert torch.equal(call(y, residual=y, binary_op="plus", out=y), with_x)
+
+
+def test_result_over_a_part_of_the_activations():
+    """The last row of x is the first of out."""
+    g, k = _gen(1), 256
+    wc, wsc, _ = _operand(g, "mx", k, k)
+    base = torch.randn(3, k, device="cuda", generator=g).half()
+    want = ops.linear_fp4(base[:2].clone(), wc, wsc, "mx")
+    assert torch.equal(ops.linear_fp4(base[:2], wc, wsc, "mx", out=base[1:]), want)
