@@ -355,7 +355,7 @@ RB200_API int rb200_preprocess_fp4_scales(const void* src, void* dst, int64_t ba
 
 /*
  * out[m, n] = unary(binary(act(ta tw sum_k a[m, k] w[n, k] + bias[n]), residual[m, n])), products of 4-bit floats summed in
- * fp32 on the tensor cores, one rounding to out's type.  RB200_ACT_SWIGLU is refused.
+ * fp32 on the tensor cores, one rounding to out's type.  RB200_ACT_SWIGLU is refused.  A NaN stays one through RELU.
  *   rb200_gemm_fp4    both operands quantised already
  *   rb200_linear_fp4  quantises x [m, k] (F16, BF16 or F32) first, as rb200_encode_fp4 does; desc->a and a_scales are not
  *                     read; workspace: rb200_linear_fp4_workspace_bytes(m, k, format) bytes, 256-byte aligned, of the call's

@@ -44,6 +44,12 @@ __device__ __forceinline__ float silu(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return v * r;
 }
+// (a NaN stays one: it says that a block of an operand was not finite)
+__device__ __forceinline__ float relu(float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(0.0f));
+  return r;
+}
 __device__ __forceinline__ float gelu(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f)); }
 
 // unary(binary(act(alpha v + bias), x)) for R elements of a column (one bias) or of a row (R of them), x the residual's.
@@ -55,7 +61,7 @@ __device__ __forceinline__ void finish(const Output& o, float (&v)[R], float alp
   for (int i = 0; i < R; ++i) v[i] = v[i] * alpha + bias[COLUMN ? 0 : i];
   if (o.act == RB200_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) v[i] = fmaxf(v[i], 0.0f);
+    for (int i = 0; i < R; ++i) v[i] = relu(v[i]);
   } else if (o.act == RB200_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = silu(v[i]);
@@ -69,7 +75,7 @@ __device__ __forceinline__ void finish(const Output& o, float (&v)[R], float alp
   }
   if (o.unop == RB200_UN_RELU) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) v[i] = fmaxf(v[i], 0.0f);
+    for (int i = 0; i < R; ++i) v[i] = relu(v[i]);
   }
 }
 __device__ __forceinline__ void prefetch_line(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }

@@ -37,3 +37,28 @@ def test_result_over_a_part_of_the_activations():
     base = torch.randn(3, k, device="cuda", generator=g).half()
     want = ops.linear_fp4(base[:2].clone(), wc, wsc, "mx")
     assert torch.equal(ops.linear_fp4(base[:2], wc, wsc, "mx", out=base[1:]), want)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m", [1, 3, 40, 80, 300])
+@pytest.mark.parametrize("act, un", [("relu", "identity"), ("identity", "relu"), ("silu", "relu")])
+def test_a_bad_block_is_seen_through_relu(fmt, dtype, m, act, un):
+    """A row of x, a row of w and an element of bias that are not finite: their outputs are NaN, the others as without."""
+    g, n, k = _gen(m), 200, 320
+    x = torch.randn(m, k, device="cuda", generator=g).to(TYPES[dtype])
+    w = torch.randn(n, k, device="cuda", generator=g).to(TYPES[dtype])
+    bias = torch.randn(n, device="cuda", generator=g).to(TYPES[dtype])
+
+    def call(x, w, bias):
+        wc, wsc = ops.encode_fp4(w, fmt)
+        return ops.linear_fp4(x, wc, wsc, fmt, bias=bias, activation=act, unary_op=un)
+
+    base = call(x, w, bias)
+    assert (base >= 0).all()
+    y, v, b = x.clone(), w.clone(), bias.clone()
+    y[m // 2, 100], v[150, 5], b[7] = float("inf"), float("nan"), float("nan")
+    got = call(y, v, b)
+    assert torch.isnan(got[m // 2]).all() and torch.isnan(got[:, [7, 150]]).all()
+    got[m // 2], got[:, [7, 150]] = base[m // 2], base[:, [7, 150]]
+    assert torch.equal(got, base)
