@@ -15,6 +15,7 @@
 #include <cstring>
 
 #include "fp4_gemm.h"
+#include "fp4_index.h"
 #include "fp4_mma.cuh"
 #include "fp4_out.cuh"
 #include "tensormap.h"
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Item it;
     it.n0 = (2 * nt + rank) * kTileN;
     it.m0 = mt * kNb;
-    it.width = min(kNb, (p.o.m - it.m0 + 31) / 32 * 32);
+    it.width = tile_width(p.o.m, it.m0, kNb);
     it.share = (it.width + 63) / 64 * 32;
     return it;
   };

@@ -113,3 +113,24 @@ def test_large_batches_in_a_graph_beside_a_stream():
             beside = run()
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(beside, want)
+
+
+def test_as_many_rows_as_there_may_be():
+    """2^31 - 1 rows of 32 k by one column: the last rows, the first, and rows around 2^30."""
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GB")
+    m, k = 2 ** 31 - 1, 32
+    a = torch.zeros(m, k // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.full(((m + 127) // 128, 1, 512), 127, dtype=torch.uint8, device="cuda")
+    rows = [0, 1, 255, 2 ** 30 - 1, 2 ** 30, m - 300, m - 257, m - 256, m - 33, m - 32, m - 2, m - 1]
+    for i, r in enumerate(rows):
+        a[r, 0] = 1 + i % 7  # 0.5 .. 6 in k 0
+    w = torch.zeros(1, k // 2, dtype=torch.uint8, device="cuda")
+    w[0, 0] = 2  # one
+    out = ops.gemm_fp4(a, scales, w, ops.preprocess_fp4_scales(torch.full((1, 1), 127, dtype=torch.uint8, device="cuda")), "mx")
+    for i, r in enumerate(rows):
+        assert out[r].item() == ref.GRID[1 + i % 7]
+        out[r] = 0
+    assert out.view(torch.int16).max() == 0 and out.view(torch.int16).min() == 0
+    del a, scales, out
+    torch.cuda.empty_cache()
