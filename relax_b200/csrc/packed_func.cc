@@ -862,7 +862,8 @@ int pf_decode_fp4(RB200Value* v, int* tc, int n_args, RB200Value*, int* ret_tc, 
   if (a.tensor(0, &codes) || a.tensor(1, &scales) || fp4_format(a, 2, &fmt) || a.tensor(3, &ts, true) || a.tensor(4, &out) ||
       float_type(fname, "out", out, &type) || same_type(fname, "out", out, out) || fp4_matrix(fname, "codes", 0, fmt, codes, scales, ts, &q))
     return -1;
-  PF_CHECK(numel(out) == q.batch * q.rows * q.k, "%s: out must be [.., n, k]", fname);
+  PF_CHECK(numel(out) == q.batch * q.rows * q.k && (numel(out) == 0 || out->shape[out->ndim - 1] == q.k), "%s: out must be [.., n, %lld]",
+           fname, (long long)q.k);
   if (ret_tc) *ret_tc = RB200_ARG_NULL;
   return rb200_decode_fp4(q.codes, q.scales, q.batch, q.rows, q.k, fmt, q.ts, data_of(out), type, rb200_get_stream());
 }
@@ -900,7 +901,8 @@ int fp4_epilogue(const Args& a, int i, const DLTensor* out, rb200_gemm_fp4_desc*
   }
   if (res) {
     if (same_type(a.fname, "residual", res, out)) return -1;
-    PF_CHECK(numel(res) == d->m * d->n, "%s: residual must have the shape of out", a.fname);
+    PF_CHECK(numel(res) == d->m * d->n && (d->m == 0 || (res->ndim > 0 && res->shape[res->ndim - 1] == d->n)),
+             "%s: residual must be [.., %lld] of out's m*n elements", a.fname, (long long)d->n);
     d->residual = data_of(res);
   }
   rb200_gemm_desc names;

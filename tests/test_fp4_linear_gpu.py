@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import relax_b200
 from relax_b200 import _lib, ops
 from tests import fp4_ref as ref
 from tests.test_fp4_gpu import TYPES, _check_product, _gen, _np, _operand
@@ -62,3 +63,24 @@ def test_a_bad_block_is_seen_through_relu(fmt, dtype, m, act, un):
     assert torch.isnan(got[m // 2]).all() and torch.isnan(got[:, [7, 150]]).all()
     got[m // 2], got[:, [7, 150]] = base[m // 2], base[:, [7, 150]]
     assert torch.equal(got, base)
+
+
+def test_a_residual_or_a_result_of_another_shape_is_refused():
+    """As many elements in another order are not the same matrix."""
+    g, m, n, k = _gen(2), 6, 96, 64
+    wc, wsc, _ = _operand(g, "mx", n, k)
+    x = torch.randn(m, k, device="cuda", generator=g).half()
+    r = torch.randn(m, n, device="cuda", generator=g).half()
+    ac, asc = ops.encode_fp4(x, "mx")
+    calls = [lambda **kw: ops.linear_fp4(x, wc, wsc, "mx", binary_op="plus", **kw),
+             lambda **kw: ops.gemm_fp4(ac, asc, wc, wsc, "mx", binary_op="plus", **kw)]
+    for call in calls:
+        want = call(residual=r)
+        assert torch.equal(call(residual=r.view(1, m, n)), want)
+        for bad in (r.view(n, m), r.view(-1), r.view(m, n // 2, 2)):
+            with pytest.raises(relax_b200.RB200Error, match="residual must be"):
+                call(residual=bad)
+    decode = relax_b200.get_global_func("relax_b200.decode_fp4")
+    with pytest.raises(relax_b200.RB200Error, match="out must be"):
+        decode(ac, asc, "mx", None, torch.empty(k, m, dtype=torch.float16, device="cuda"))
+    assert ops.linear_fp4(x[0], wc, wsc, "mx", residual=r[0], binary_op="plus").shape == (n,)
