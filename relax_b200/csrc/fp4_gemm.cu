@@ -428,10 +428,10 @@ int check_gemm(const rb200_gemm_fp4_desc* d) {
   RB200_CHECK(d->activation >= RB200_ACT_IDENTITY && d->activation <= RB200_ACT_GELU, "unknown activation %d", d->activation);
   RB200_CHECK(d->binary_op >= RB200_BIN_NONE && d->binary_op <= RB200_BIN_MULTIPLY, "unknown binary op %d", d->binary_op);
   RB200_CHECK(d->unary_op >= RB200_UN_IDENTITY && d->unary_op <= RB200_UN_RELU, "unknown unary op %d", d->unary_op);
-  RB200_CHECK((d->binary_op != RB200_BIN_NONE) == (d->residual != nullptr), "a residual needs a binary op, and the other way round");
   RB200_CHECK(d->ldo >= d->n, "ldo=%lld is less than n", (long long)d->ldo);
   RB200_CHECK(d->format == f4::kNv || (!d->a_tensor_scale && !d->w_tensor_scale), "the mx format has no tensor scale");
-  if (d->m == 0) return 0;
+  if (d->m == 0) return 0;  // (an empty residual has no address)
+  RB200_CHECK((d->binary_op != RB200_BIN_NONE) == (d->residual != nullptr), "a residual needs a binary op, and the other way round");
   RB200_CHECK(d->w && d->w_scales && d->out, "w, w_scales and out must be non-NULL");
   RB200_CHECK(aligned16(d->w) && aligned16(d->w_scales), "codes and scales must be 16-byte aligned");
   const uintptr_t width = d->out_dtype == f4::kF32 ? 4 : 2;

@@ -159,3 +159,9 @@ def test_python_refusals():
         ops.gemm_fp4(c[0], c, c, c, "mx")
     with pytest.raises(relax_b200.RB200Error, match="CUDA device"):
         ops.linear_fp4(x, c, torch.zeros(1, 1, 512, dtype=torch.uint8), "mx")
+
+
+def test_an_empty_batch_has_a_residual_without_an_address():
+    lib = _lib.load()
+    assert lib.rb200_gemm_fp4(ctypes.byref(_desc(m=0, binary_op=1)), None) == 0
+    assert lib.rb200_gemm_fp4(ctypes.byref(_desc(m=0, binary_op=3)), None) == -1

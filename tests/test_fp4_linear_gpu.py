@@ -84,3 +84,17 @@ def test_a_residual_or_a_result_of_another_shape_is_refused():
     with pytest.raises(relax_b200.RB200Error, match="out must be"):
         decode(ac, asc, "mx", None, torch.empty(k, m, dtype=torch.float16, device="cuda"))
     assert ops.linear_fp4(x[0], wc, wsc, "mx", residual=r[0], binary_op="plus").shape == (n,)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+def test_no_rows_with_everything_a_call_can_have(fmt):
+    g, n, k = _gen(6), 96, 64
+    wc, wsc, _ = _operand(g, fmt, n, k)
+    x, r, b = torch.empty(0, k, device="cuda").half(), torch.empty(0, n, device="cuda").half(), torch.zeros(n, device="cuda").half()
+    ts = torch.ones(1, device="cuda") if fmt == "nv" else None
+    kw = dict(bias=b, residual=r, activation="silu", binary_op="plus", unary_op="relu")
+    assert ops.linear_fp4(x, wc, wsc, fmt, ts, ts, **kw).shape == (0, n)
+    assert ops.linear_fp4(x.view(0, 3, k), wc, wsc, fmt, ts, ts, **{**kw, "residual": r.view(0, 3, n)}).shape == (0, 3, n)
+    ac, asc = ops.encode_fp4(x, fmt, tensor_scale=ts)
+    assert ops.gemm_fp4(ac, asc, wc, wsc, fmt, ts, ts, **kw).shape == (0, n)
+    assert ops.decode_fp4(ac, asc, fmt, tensor_scale=ts).shape == (0, k)
