@@ -348,13 +348,13 @@ int launch_fmt(Params& p, int dtype, const CUtensorMap& tw, const CUtensorMap& t
 }
 
 // Few rows are quantised by the product's CTAs, each its share of k for itself, where that takes less than a kernel before it:
-// one or two rows (k 4096 x n 4096: 13.3 -> 12.3 us with the launches and cold, k 28672 x n 8192: 33.8 -> 30.7), and more where
-// a CTA's four warps have at most two turns of 256 k x two rows each (k 4096 x n 4096: four rows, two turns, 13.3 -> 12.4;
+// one or two rows (k 4096 x n 4096: 13.3 -> 12.3 us with the launches and cold, k 28672 x n 8192: 33.8 -> 30.7), and three or four
+// where a CTA's four warps have at most two turns of 256 k x two rows each (k 4096 x n 4096: four rows, two turns, 13.3 -> 12.4;
 // eight rows, four turns, 13.3 -> 14.3; k 4096 x n 11008, four rows, four turns, 15.4 -> 16.4).
 bool quantises_itself(int64_t m, int64_t n, int64_t k) {
   if (m <= 2) return true;
   const int tiles = (int)((n + kTileN - 1) / kTileN), per = (int)((k + kStageK - 1) / kStageK + cluster_of(tiles, k) - 1) / cluster_of(tiles, k);
-  return m <= 16 && (per + 3) / 4 * ((m + 1) / 2) <= 2;
+  return m <= 4 && (per + 3) / 4 * ((m + 1) / 2) <= 2;
 }
 
 }  // namespace

@@ -98,3 +98,37 @@ def test_no_rows_with_everything_a_call_can_have(fmt):
     ac, asc = ops.encode_fp4(x, fmt, tensor_scale=ts)
     assert ops.gemm_fp4(ac, asc, wc, wsc, fmt, ts, ts, **kw).shape == (0, n)
     assert ops.decode_fp4(ac, asc, fmt, tensor_scale=ts).shape == (0, k)
+
+
+# Batches quantised by the product's CTAs: one and two rows; three and four with at most four chunks of 256 k a CTA (a cluster shares
+# k 8192 and k 10240 by eight, k 1024 and k 1280 are one CTA's at 19000 columns).  Next to each its neighbour that is not.
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m, n, k", [(1, 130, 32), (1, 300, 992), (2, 200, 288), (2, 129, 4128), (3, 130, 288), (3, 300, 992), (4, 130, 288),
+                                     (4, 129, 992), (5, 129, 992), (4, 136, 8192), (4, 136, 8224), (4, 130, 10240), (3, 19000, 1024),
+                                     (4, 19000, 1024), (4, 19000, 1280), (5, 19000, 1024)])
+def test_few_rows(fmt, dtype, m, n, k):
+    g = _gen(m * n + k)
+    x = (torch.randn(m, k, device="cuda", generator=g) * torch.exp(torch.randn(k, device="cuda", generator=g))).to(TYPES[dtype])
+    x[m - 1, k // 2:] *= 2.0 ** -6  # rows of other scales
+    wc, wsc, w = _operand(g, fmt, n, k)
+    ts = (x.abs().amax().float() / 2688).reshape(1) if fmt == "nv" else None
+    tsv = 1.0 if ts is None else float(ts)
+    out = ops.linear_fp4(x, wc, wsc, fmt, x_tensor_scale=ts)
+    codes, scales = ref.encode(_np(x), fmt, tsv)
+    _check_product(out, ref.decode(codes, scales, fmt), w, tsv)
+    ac, asc = ops.encode_fp4(x, fmt, tensor_scale=ts)
+    assert torch.equal(ops.gemm_fp4(ac, asc, wc, wsc, fmt, a_tensor_scale=ts, dtype=x.dtype), out)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+def test_few_rows_that_are_not_finite(fmt, m):
+    """A bad block of one row, in the product that quantises: NaN in that row, the others as without."""
+    g, n, k = _gen(m), 200, 288
+    x = torch.randn(m, k, device="cuda", generator=g).half()
+    wc, wsc, _ = _operand(g, fmt, n, k)
+    base = ops.linear_fp4(x, wc, wsc, fmt)
+    x[m - 1, k - 1] = float("-inf")
+    got = ops.linear_fp4(x, wc, wsc, fmt)
+    assert torch.isnan(got[m - 1]).all() and torch.equal(got[:m - 1], base[:m - 1])
