@@ -1068,10 +1068,12 @@ int launch(Params p, const Weights& w, int absent, cudaStream_t stream) {
 
 template <int FMT>
 int launch_fmt(const Params& p, const Weights& w, int absent, cudaStream_t stream) {
-  // Entries of eight rows, or of sixteen where experts have more than four on average: weights of an expert with more rows than
-  // an entry are read again (by then from L2), rows that are not there take shared memory from the stages (29 tokens,
-  // 64 experts of top 6: 100 us with sixteen, 79 with eight).
-  return p.tokens <= 8 || p.tokens * p.top_k <= 4 * p.experts ? launch<FMT, 1>(p, w, absent, stream) : launch<FMT, 2>(p, w, absent, stream);
+  // Entries of eight rows, or of sixteen where experts have more than eight on average: weights of an expert with more rows than
+  // an entry are read again (by then from L2), rows that are not there take shared memory from the stages and clocks from the
+  // products.  us with eight / sixteen: hidden 4096, ffn 14336, eight experts of top 2, mx, 9 tokens 130 / 180, 24 (6 rows on average)
+  // 168 / 227, 32 (8) 206 / 245; ffn 1536, 16 experts of top 4, nv, 24 (6) 57 / 69, 32 (8) 74.3 / 76.0; hidden = ffn = 4096, four
+  // experts of top 2, mx, 32 (16) 74.3 / 72.5.
+  return p.tokens * p.top_k <= 8 * p.experts ? launch<FMT, 1>(p, w, absent, stream) : launch<FMT, 2>(p, w, absent, stream);
 }
 
 // [h | its exponents | parts | states | tickets]
