@@ -132,3 +132,23 @@ def test_few_rows_that_are_not_finite(fmt, m):
     x[m - 1, k - 1] = float("-inf")
     got = ops.linear_fp4(x, wc, wsc, fmt)
     assert torch.isnan(got[m - 1]).all() and torch.equal(got[:m - 1], base[:m - 1])
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("m", [1, 20, 70, 300])
+def test_a_weight_quantised_by_the_call_before(fmt, m):
+    """With launch overlap off: codes and scales written over and over into the same memory, each used by the next call."""
+    assert not relax_b200.get_launch_overlap()
+    g, n, k, times = _gen(m), 520, 1056, 30
+    x = torch.randn(m, k, device="cuda", generator=g).half()
+    weights = [torch.randn(n, k, device="cuda", generator=g).half() for _ in range(times)]
+    codes, scales = ops.encode_fp4(weights[0], fmt)
+    encode = relax_b200.get_global_func("relax_b200.encode_fp4")
+    got = []
+    for w in weights:
+        encode(w, fmt, None, codes, scales)
+        got.append(ops.linear_fp4(x, codes, scales, fmt))
+    for w, y in zip(weights, got):
+        c, s = ops.encode_fp4(w, fmt)
+        torch.cuda.synchronize()
+        assert torch.equal(ops.linear_fp4(x, c, s, fmt), y)
