@@ -338,7 +338,7 @@ RB200_API int rb200_encode_ft(const void* a, void* packed, void* scales, int64_t
  *   nv  s = RNE_e4m3(max |x| / (6 ts)) <= 448, q = RNE(x / (s ts)), |q| <= 6; s = 0: q = 0
  *   A code has the sign of its x, that of a zero too.  A block with an infinity or a NaN, or under a tensor scale that is
  *   not positive and finite, gets the NaN scale and codes 0.
- * rb200_decode_fp4  codes, scales -> code * scale * tensor scale, rounded to the element type.
+ * rb200_decode_fp4  codes, scales -> code * scale, exactly, times the tensor scale in fp32, rounded to the element type.
  */
 #define RB200_FP4_MX 0
 #define RB200_FP4_NV 1

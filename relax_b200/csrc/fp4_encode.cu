@@ -11,6 +11,8 @@
 // instructions, most of them for the two products of every element, issued in 74 % of the clocks.
 // Measured (fp16 and bf16, inputs out of memory): 1733 x 11008 in kMx 11.0 us (48 MB, 4.4 TB/s), back 9.2 us; 28672 x 8192 in
 // kNv 150 us (602 MB, 4.0 TB/s), back 90 us (6.7 TB/s); one row of 4096 in kNv 3.1 us, back 2.1 us.
+// A checkpoint's scales into tiles: 14.7 MB (28672 x 8192 in kNv) 56 us, 0.5 TB/s: a warp reads four bytes each of 32 rows, an
+// eighth of each sector.  Done once per weight, so left as simple as it is.
 #include "../../include/relax_b200.h"
 #include "fp4_encode.h"
 #include "fp4_quant.cuh"

@@ -8,9 +8,10 @@
 // with by then), and each adds up its share of the batch rows in the order of the ranks, so that a result does not depend
 // on timing.
 //
-// What bounds it is reading w once: k 28672 x n 8192 in the mx format, 125 MB, takes 21.5 us for one row (5.8 TB/s) out of
-// memory; two CTAs an SM keep some 200 KB on their way there.  Small ones are launch and one trip to memory and back through
-// the cluster: k 4096 x n 4096 in the nv format, 9.4 MB, 6.5 us with everything, of which the reading is 1.5.
+// What bounds it is reading w once: k 28672 x n 8192 in the mx format, 125 MB, takes 24.1 us for one row out of memory (the
+// kernel alone, 5.2 TB/s), 22.1 a call in a row of calls; two CTAs an SM keep some 200 KB on their way there.  Small ones are
+// launch and one trip to memory and back through the cluster: k 4096 x n 4096 in the nv format, 9.4 MB, 6.5 us a call in a row,
+// 8.2 to 8.8 the kernel alone out of memory, of which the reading is 1.5.
 #include <atomic>
 
 #include <cstring>
@@ -298,7 +299,12 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kMaxDevices = 64;
 std::atomic<bool> g_launched[kMaxDevices];  // devices whose status word a wait may have set
 
-// CTAs that share a tile's k: as many as leave two CTAs an SM and two chunks each
+// CTAs that share a tile's k: as many as leave two CTAs an SM and two chunks each.  The kernel alone out of memory, us, with
+// 1 / 2 / 4 / 8 of them: mx, one row, k 28672 x n 8192 33.9 / 26.0 / 24.2 / 28.3 (4 taken); mx, 7 rows, k 4096 x n 32016
+// 16.2 / 20.0 / 27.6 / 46.8 (1); nv, 48 rows, k 28672 x n 8192 40.3 / 29.6 / 26.5 / 32.4 (4); mx, 16 rows, k 8192 x n 2048
+// 13.1 / 10.2 / 8.2 / 8.3 (8); mx, 4 rows, k 4096 x n 1024 9.0 / 7.9 / 6.9 / 6.5 (8); nv, one row, k = n = 4096
+// 8.9 / 8.1 / 7.6 / 8.2 (8: four would be 7 % less); nv, 16 rows, k 4096 x n 14336 10.9 / 11.7 / 15.6 / 25.2 (2: one would be
+// 7 % less).
 int cluster_of(int tiles, int64_t k) {
   const int chunks = (int)((k + kStageK - 1) / kStageK);
   int c = 1;
@@ -405,6 +411,10 @@ static int fp4_few_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t l
   return d.format == kMx ? launch_fmt<kMx, false>(p, d.out_dtype, tw, ta, stream) : launch_fmt<kNv, false>(p, d.out_dtype, tw, ta, stream);
 }
 
+// Up to 64 rows here, more by pairs of CTAs (us out of memory, this kernel / pairs; it can be built for 128 rows): 64 rows
+// k 4096 x n 11008 12.2 / 11.5, k = n = 4096 10.8 / 10.6, k 28672 x n 8192 27.9 / 30.6, k 14336 x n 4096 13.8 / 16.2, k 4096 x
+// n 22016 16.3 / 18.3, x n 1024 8.0 / 10.3; 96 rows 13.4 / 12.4, 11.8 / 10.6, 29.0 / 30.5, 14.9 / 16.5, 18.3 / 19.8, 8.2 / 10.3; 128 rows
+// 14.9 / 12.7, 13.1 / 10.7, 30.4 / 31.3, 16.2 / 16.6, 20.0 / 20.0, 9.1 / 10.4.  A limit by shape would save up to a fifth between.
 int fp4_gemm_launch(const rb200_gemm_fp4_desc& d, const void* x, int64_t ldx, cudaStream_t stream) {
   int dev = 0;
   RB200_CUDA(cudaGetDevice(&dev));

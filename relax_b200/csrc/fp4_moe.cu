@@ -8,7 +8,8 @@
 // k for that and multiply the fp16 pairs, exactly (two and four significant bits, at least 2^-10, at most 2688).
 //
 // Routing is a few hundred clocks for a few tokens, so every CTA does it for itself from the logits: no kernel before these
-// two, no hand-over through memory.  `down` does it, and asks for its first weights, while `up` still runs.
+// two, no hand-over through memory.  `down` does it, and asks for its first weights, as soon as CTAs of `up` leave it room on
+// their SM: two of either fill one.
 //
 // Weights come by tensor-map loads in 128-byte rows, swizzled; a lane's code words are then free of bank conflicts.  A
 // warp's lane (g, t) holds, of the 32 k of a chunk, k 8t .. 8t + 7 of rows g and g + 8: the MMAs' k slots are a permutation
@@ -17,8 +18,9 @@
 // memory, every word by one thread at a time in the order of the sequence; what it has of a column tile that is not its own
 // alone goes to the workspace, and the last CTA to come adds the parts up in the order of the CTAs: nothing depends on timing.
 //
-// Measured, hidden 4096, ffn 14336, eight experts, two a token: one token in the mx format 49 us, 187 MB (3.8 TB/s), eight in
-// the nv format 167 us, 712 MB (4.3 TB/s); 29 tokens, hidden 2048, ffn 1408, 64 experts, six a token 78 us, 277 MB (3.6 TB/s).
+// Measured, hidden 4096, ffn 14336, eight experts, two a token: one token in the mx format 50 us, 187 MB (3.7 TB/s), in nv 52; eight
+// in the nv format 143 to 175 us by where their weights lie, 712 MB (5.0 to 4.1 TB/s); 29 tokens, hidden 2048, ffn 1408, 64 experts,
+// six a token 80 us, 277 MB (3.5 TB/s).
 // Boxes out of memory come at 6 TB/s at the most.  Below that, kNv is held by issue (63 instructions per 512 bytes of codes,
 // issued in 63 % of the clocks), few or small experts by the starts and last tiles of two kernels.
 #include <atomic>

@@ -9,6 +9,8 @@
 // warps, up to 128 columns each) and hands the tensor memory back before it applies the epilogue and stores: the MMAs of the next
 // tile wait for the reading only.  The drain itself is a loop over 16 columns: out of a cold instruction cache the same code for
 // all 128 columns took 8 to 26 us in its first tile, the loop takes 3.5 (warm, it costs 3 % at 2048 rows, k 4096).
+// The 128 sums and the loop want more than the 168 registers a thread that 384 threads share evenly: the form without shared k
+// spills 120 to 128 bytes a thread (192 to 204 bytes of stores), written and read back once a tile.
 //
 // Measured: 4096 rows, k 8192 x n 28672 in the mx format 300 us, 6.4 PFLOP/s, 387 with the quantiser and at the power cap; 2048
 // rows, k 4096 x n 22016 in the nv format 77 us (4.8), 108; 333 rows, k 4096 x n 11008 with bias and silu 19 us (1.6), 20.6.
